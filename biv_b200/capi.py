@@ -30,7 +30,9 @@ SYMBOLS = ["bivmoe_create", "bivmoe_destroy", "bivmoe_forward", "bivmoe_forward_
            "bivmoe_host_wait", "bivmoe_int8_peak", "bivmoe_dense_create", "bivmoe_ep_peer_info",
            "bivmoe_ep_peer_attach", "bivmoe_ep_peer_dispatch", "bivmoe_ep_peer_experts",
            "bivmoe_ep_peer_combine", "bivmoe_status", "bivmoe_last_oom_bytes", "bivmoe_ep_peer_signal",
-           "bivmoe_ep_peer_wait", "bivmoe_ep_peer_barrier", "bivmoe_ep_peer_wait_limit"]
+           "bivmoe_ep_peer_wait", "bivmoe_ep_peer_barrier", "bivmoe_ep_peer_wait_limit",
+           "bivmoe_cache_create", "bivmoe_cache_destroy", "bivmoe_cache_extend", "bivmoe_cache_store",
+           "bivmoe_cache_attend", "bivmoe_cache_status"]
 
 
 class BivMoeError(RuntimeError):
@@ -56,6 +58,44 @@ class Desc(C.Structure):
                 ("gate", Experts), ("up", Experts), ("down", Experts),
                 ("sh_gate", Experts), ("sh_up", Experts), ("sh_down", Experts),
                 ("sh_gate_inp", C.c_void_p)]
+
+
+class CacheDesc(C.Structure):
+    _fields_ = [("ggml_type", C.c_int32), ("n_head", C.c_int32), ("n_head_kv", C.c_int32), ("head_dim", C.c_int32),
+                ("page_size", C.c_int32), ("max_seqs", C.c_int32), ("max_tokens", C.c_int32), ("device", C.c_int32),
+                ("n_rot", C.c_int32), ("rope_axes", C.c_int32), ("rope_sections", C.c_int32 * 4),
+                ("rope_interleaved", C.c_int32), ("rope_adjacent", C.c_int32), ("rope_base", C.c_double)]
+
+
+def _flat(prefix, kind):
+    """The fields of a ``bivmoe_rows`` or ``bivmoe_pool`` inside an argument struct, set without a
+    Python object of their own (a call's arguments are filled in on the host for every launch)."""
+    names = {"rows": ("stride_token", "stride_head"), "pool": ("stride_page", "stride_token", "stride_head", "n_pages")}[kind]
+    fields = [(prefix, C.c_void_p)] + [(prefix + "_" + n, C.c_int64) for n in names]
+    return fields + ([(prefix + "_type", C.c_int32), (prefix + "_reserved", C.c_int32)] if kind == "rows" else [])
+
+
+class ExtendArgs(C.Structure):
+    _fields_ = [("past", C.c_void_p), ("added", C.c_void_p), ("held", C.c_void_p), ("free_pages", C.c_void_p),
+                ("free_count", C.c_void_p), ("table", C.c_void_p), ("table_stride", C.c_int64),
+                ("table_width", C.c_int32), ("n_free", C.c_int32), ("n_seq", C.c_int32), ("n_tokens", C.c_int32),
+                ("length", C.c_void_p), ("first", C.c_void_p), ("positions", C.c_void_p), ("left", C.c_void_p),
+                ("held_out", C.c_void_p), ("slots", C.c_void_p)]
+
+
+class StoreArgs(C.Structure):
+    _fields_ = (_flat("q", "rows") + _flat("k", "rows") + _flat("v", "rows") + _flat("q_out", "rows")
+                + _flat("k_pool", "pool") + _flat("v_pool", "pool")
+                + [("slots", C.c_void_p), ("positions", C.c_void_p), ("positions_stride", C.c_int64),
+                   ("n_tokens", C.c_int32), ("reserved", C.c_int32)])
+
+
+class AttendArgs(C.Structure):
+    _fields_ = (_flat("q", "rows") + _flat("out", "rows") + _flat("k_pool", "pool") + _flat("v_pool", "pool")
+                + [("table", C.c_void_p), ("table_stride", C.c_int64), ("table_width", C.c_int32),
+                   ("n_seq", C.c_int32), ("n_tokens", C.c_int32), ("max_new", C.c_int32), ("first", C.c_void_p),
+                   ("length", C.c_void_p), ("scale", C.c_float), ("window", C.c_int32), ("sinks", C.c_int32),
+                   ("reserved", C.c_int32)])
 
 
 _lib = None
@@ -111,6 +151,13 @@ def lib():
         L.bivmoe_ep_peer_wait_limit.argtypes = [vp, C.c_uint64]
         L.bivmoe_numerics.argtypes = [vp, C.c_char_p, C.c_size_t]
         L.bivmoe_memory.argtypes = [vp, C.POINTER(C.c_uint64), C.POINTER(C.c_uint64)]
+        L.bivmoe_cache_create.argtypes = [C.POINTER(CacheDesc), C.POINTER(vp)]
+        L.bivmoe_cache_destroy.argtypes = [vp]
+        L.bivmoe_cache_destroy.restype = None
+        L.bivmoe_cache_extend.argtypes = [vp, C.POINTER(ExtendArgs), vp]
+        L.bivmoe_cache_store.argtypes = [vp, C.POINTER(StoreArgs), vp]
+        L.bivmoe_cache_attend.argtypes = [vp, C.POINTER(AttendArgs), vp]
+        L.bivmoe_cache_status.argtypes = [vp, vp]
         L.bivmoe_launch_count.restype = C.c_uint64
         L.bivmoe_last_error.argtypes = [vp]
         L.bivmoe_last_error.restype = C.c_char_p

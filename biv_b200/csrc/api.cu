@@ -27,7 +27,7 @@ static thread_local std::string g_error;
 static thread_local uint64_t g_oom_bytes = 0;   // size of the device allocation that failed last
 
 // cudaMalloc that remembers the size of a failed request (Error::OutOfMemory{bytes})
-static cudaError_t dev_alloc(void** p, size_t bytes) {
+cudaError_t dev_alloc(void** p, size_t bytes) {
     const cudaError_t e = cudaMalloc(p, bytes);
     if (e == cudaErrorMemoryAllocation) {
         g_oom_bytes = bytes;
@@ -45,6 +45,8 @@ static int set_err(std::string* dst, int code, const char* fmt, ...) {
     (dst ? *dst : g_error) = buf;
     return code;
 }
+
+int global_error(int code, const char* text) { return set_err(nullptr, code, "%s", text); }
 
 struct Arena {   // carves 256-byte aligned pieces out of one allocation
     size_t off = 0;

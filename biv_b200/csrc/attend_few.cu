@@ -1,0 +1,310 @@
+// Attention over the pages for tiles of 16 rows: one pass over the keys with the running maximum and
+// sum of the softmax, products on the warp-level tensor cores.
+//
+//   s_j = scale q . k_j,  m = max s_j,  l = sum 2^(s_j - m),  o = sum 2^(s_j - m) v_j / l   (s in powers of two)
+//
+// A block is four warps; of a tile of 64 keys warp w takes 16, in a ring of its own in shared memory
+// that its own cp.async copies fill, with its own running maximum, sum and o: the warps meet at the
+// item's end only, where the four o are joined.  A long axis is cut into pieces over blocks (cache.cuh);
+// the block that is last to finish a tile joins the pieces, in the pieces' order whoever is last.
+// With one new token a request the keys are read once: bound by memory.
+#include "cache.cuh"
+#include "common.cuh"
+#include "launch.cuh"
+#include "tcgen05.cuh"
+
+namespace bivmoe {
+
+constexpr int kFewWarps = 4, kFewThreads = 32 * kFewWarps, kFewKeys = 16 * kFewWarps, kFewStages = 3;
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool there) {
+    // nothing is read, and zeros are written, where there is nothing
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void ldm4(uint32_t a, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ void ldm4t(uint32_t a, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+template <class T> __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <> __device__ __forceinline__ void mma16<__nv_bfloat16>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <> __device__ __forceinline__ void mma16<__half>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+template <int D> struct FewBytes {
+    static constexpr int stage = 2 * 16 * D * 2;      // 16 keys' k and v
+    static constexpr int ring = kFewWarps * kFewStages * stage;
+    static constexpr int fixed = ring + 16 * D * 2;   // and the 16 rows of q
+};
+
+// 16-byte piece `c` of row `r`: the low three bits of the piece's place are turned by the row, so that
+// eight rows' pieces c lie in different banks
+template <int D> __device__ __forceinline__ uint32_t few_at(int r, int c) {
+    return (uint32_t)(r * (D * 2) + ((c ^ (r & 7)) << 4));
+}
+
+template <int D, class T>
+__global__ void __launch_bounds__(kFewThreads, D == 256 ? 1 : 2) attend_few_kernel(AttendCall a) {
+    extern __shared__ __align__(1024) uint8_t sm[];
+    __shared__ float s_m[kFewWarps][16], s_l[kFewWarps][16];
+    __shared__ int s_bad[16], s_last;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    uint8_t* ring_p = sm + warp * kFewStages * FewBytes<D>::stage;
+    const uint32_t ring = pf_smem(ring_p), qs = pf_smem(sm + FewBytes<D>::ring);
+    pdl_enter();
+    const Items it = find_items<kFewKeys, kFewRows, kFewThreads>(a, 2, (int*)(sm + FewBytes<D>::fixed));
+    const int g = lane >> 2, quad = lane & 3;
+    constexpr int CH = D / 8, RPI = 32 / CH;      // 16-byte pieces of a row, rows of a warp's copy
+
+    for (int index = blockIdx.x; index < it.total; index += gridDim.x) {
+        const Item x = item_at<kFewKeys, kFewRows>(a, it, index);
+        if (item_void(x)) continue;
+        __syncthreads();                          // the item before is done with the rings and the rows
+        const int32_t* table = a.table + (int64_t)x.b * a.table_stride;
+        // the rows: past the tile's, zeros
+        for (int i = tid; i < 16 * CH; i += kFewThreads) {
+            const int r = i / CH, c = i % CH, R = x.row0 + r, tok = (int)a.group.div(R), h = x.head * (int)a.group.d + R - tok * (int)a.group.d;
+            const bool there = r < x.rows;
+            cp16(qs + few_at<D>(r, c), there ? a.q + (int64_t)(x.r.begin + tok) * a.q_token + (int64_t)h * a.q_head + c * 16 : a.q, there);
+        }
+        cp_commit();
+        const int n = max(x.i1 - x.i0, 0), p_top = x.r.past + (int)a.group.div(x.row0 + x.rows - 1);
+        const uint8_t *k_base = a.k.data + x.head * a.k.head, *v_base = a.v.data + x.head * a.v.head;
+        // lane r of the first 16: where key r of the warp's next stage lies
+        auto find = [&](int i, int64_t& ko, int64_t& vo, bool& ok) {
+            const int j = x.tiles.tile(x.i0 + i) * kFewKeys + warp * 16 + (lane & 15);
+            int at = 0;
+            const int page = i < n && j <= p_top ? page_of(a, table, j, at) : -1;
+            ok = page >= 0;
+            ko = ok ? page * a.k.page + at * a.k.token : 0;
+            vo = ok ? page * a.v.page + at * a.v.token : 0;
+        };
+        uint32_t there[kFewStages];               // which of a stage's keys there are
+        int64_t ko, vo;
+        bool ok;
+        find(0, ko, vo, ok);
+        auto copy = [&](int i, int slot) {        // stage i, whose keys have been found; finds the next one's
+            const uint32_t mask = __ballot_sync(0xffffffffu, ok) & 0xffffu;
+            const uint32_t dst = ring + slot * FewBytes<D>::stage;
+            if (i < n) {
+#pragma unroll
+                for (int e = 0; e < 16 / RPI; e++) {
+                    const int r = e * RPI + lane / CH, c = lane % CH;
+                    const int64_t kr = __shfl_sync(0xffffffffu, ko, r), vr = __shfl_sync(0xffffffffu, vo, r);
+                    cp16(dst + few_at<D>(r, c), k_base + kr + c * 16, mask >> r & 1);
+                    cp16(dst + 16 * D * 2 + few_at<D>(r, c), v_base + vr + c * 16, mask >> r & 1);
+                }
+            }
+            cp_commit();
+            find(i + 1, ko, vo, ok);
+            return mask;
+        };
+#pragma unroll
+        for (int i = 0; i < kFewStages - 1; i++) there[i] = copy(i, i);
+        cp_wait<kFewStages - 1>();                // the rows, which were asked for first
+        __syncthreads();
+        // D 256: a row's fragments take as many registers as half of o: read again at each use
+        constexpr bool HOLD = D <= 128;
+        uint32_t qf[HOLD ? D / 16 : 1][4];
+        if (HOLD)
+#pragma unroll
+            for (int k = 0; k < D / 16; k++) ldm4(qs + few_at<D>(lane & 15, 2 * k + (lane >> 4)), qf[k % (HOLD ? D / 16 : 1)]);
+        int p[2];
+#pragma unroll
+        for (int i = 0; i < 2; i++) p[i] = g + 8 * i < x.rows ? x.r.past + (int)a.group.div(x.row0 + g + 8 * i) : -1;
+        float o[D / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < D / 8; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+#pragma unroll 1
+        for (int i0 = 0; i0 < n; i0 += kFewStages) {
+#pragma unroll
+            for (int u = 0; u < kFewStages; u++) {
+                const int i = i0 + u;
+                if (i >= n) break;
+                there[(u + kFewStages - 1) % kFewStages] = copy(i + kFewStages - 1, (u + kFewStages - 1) % kFewStages);
+                cp_wait<kFewStages - 1>();
+                __syncwarp();
+                const uint32_t ks = ring + u * FewBytes<D>::stage, vs = ks + 16 * D * 2;
+                float s[2][4] = {};
+#pragma unroll
+                for (int k = 0; k < D / 16; k++) {
+                    uint32_t b[4], again[4];
+                    ldm4(ks + few_at<D>((lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1)), b);
+                    if (!HOLD) ldm4(qs + few_at<D>(lane & 15, 2 * k + (lane >> 4)), again);
+                    const uint32_t(&qk)[4] = HOLD ? qf[HOLD ? k : 0] : again;
+                    mma16<T>(s[0], qk, b[0], b[1]);
+                    mma16<T>(s[1], qk, b[2], b[3]);
+                }
+                const int j0 = x.tiles.tile(x.i0 + i) * kFewKeys + warp * 16;
+                float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                for (int t = 0; t < 2; t++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const int r = t * 8 + quad * 2 + (e & 1);
+                        const bool see = (there[u] >> r & 1) && sees(a, p[e >> 1], j0 + r);
+                        s[t][e] = see ? s[t][e] * a.scale_log2 : -INFINITY;
+                        top[e >> 1] = fmaxf(top[e >> 1], s[t][e]);
+                    }
+                float keep[2];
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 1));
+                    top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 2));
+                    const float mn = fmaxf(m[e], top[e]);
+                    keep[e] = mn == -INFINITY ? 1.0f : exp2_of(m[e] - mn);
+                    m[e] = mn;
+                    top[e] = mn == -INFINITY ? 0.0f : mn;
+                    l[e] *= keep[e];
+                }
+#pragma unroll
+                for (int t = 0; t < 2; t++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        s[t][e] = exp2_of(s[t][e] - top[e >> 1]);
+                        l[e >> 1] += s[t][e];
+                    }
+                // the weights, at most 1, rounded to the cache's type for the second product (relative
+                // error 2^-9 or 2^-12 each); l sums them unrounded
+                const uint32_t w[4] = {pack2<T>(s[0][0], s[0][1]), pack2<T>(s[0][2], s[0][3]), pack2<T>(s[1][0], s[1][1]),
+                                       pack2<T>(s[1][2], s[1][3])};
+#pragma unroll
+                for (int c = 0; c < D / 8; c += 2) {
+                    uint32_t b[4];
+                    ldm4t(vs + few_at<D>((lane & 7) + ((lane >> 3 & 1) << 3), c + (lane >> 4)), b);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) { o[c][e] *= keep[e >> 1]; o[c + 1][e] *= keep[e >> 1]; }
+                    mma16<T>(o[c], w, b[0], b[1]);
+                    mma16<T>(o[c + 1], w, b[2], b[3]);
+                }
+                __syncwarp();
+            }
+        }
+        cp_wait<0>();
+        // the four warps' o, maxima and sums through shared memory: [16][D] f32 in the warp's own ring
+        float* om = (float*)ring_p;
+        __syncwarp();
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
+            l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
+            if (quad == 0) { s_m[warp][g + 8 * e] = m[e]; s_l[warp][g + 8 * e] = l[e]; }
+        }
+#pragma unroll
+        for (int c = 0; c < D / 8; c++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) *(float2*)(om + (g + 8 * e) * D + 8 * c + 2 * quad) = make_float2(o[c][2 * e], o[c][2 * e + 1]);
+        if (tid < 16) s_bad[tid] = 0;
+        __syncthreads();
+        // eight threads to a row, 4 values at a time
+        const int row = tid >> 3, sub = tid & 7;
+        float M = -INFINITY, f[kFewWarps], L = 0.0f;
+        for (int w = 0; w < kFewWarps; w++) M = fmaxf(M, s_m[w][row]);
+        for (int w = 0; w < kFewWarps; w++) {
+            f[w] = s_m[w][row] == -INFINITY ? 0.0f : exp2_of(s_m[w][row] - M);
+            L += s_l[w][row] * f[w];
+        }
+        float4 y[D / 32];
+        bool fine = L - L == 0.0f;
+#pragma unroll
+        for (int i = 0; i < D / 32; i++) {
+            float4 v = make_float4(0, 0, 0, 0);
+#pragma unroll
+            for (int w = 0; w < kFewWarps; w++) {
+                const float4 z = *(const float4*)(sm + w * kFewStages * FewBytes<D>::stage + (row * D + sub * 4 + 32 * i) * 4);
+                if (f[w] != 0.0f) { v.x += z.x * f[w]; v.y += z.y * f[w]; v.z += z.z * f[w]; v.w += z.w * f[w]; }
+            }
+            y[i] = v;
+            const float z = (v.x - v.x) + (v.y - v.y) + (v.z - v.z) + (v.w - v.w);
+            fine = fine && z == 0.0f;
+        }
+        if (!fine && row < x.rows) s_bad[row] = 1;
+        if (__syncthreads_or(!fine && row < x.rows)) {
+            for (int r = warp; r < x.rows; r += kFewWarps) {
+                if (!s_bad[r]) continue;
+                float c[D / 32], cm, cl;
+                careful_row<D, T>(a, x, r, kFewKeys, c, cm, cl);
+                for (int e = 0; e < D / 32; e++) ((float*)sm)[r * D + lane + 32 * e] = c[e];
+                if (lane == 0) { s_m[0][r] = cm; s_l[0][r] = cl; }
+            }
+            __syncthreads();
+            if (s_bad[row]) {
+                M = s_m[0][row];
+                L = s_l[0][row];
+                for (int i = 0; i < D / 32; i++) y[i] = *(const float4*)(sm + (row * D + sub * 4 + 32 * i) * 4);
+            }
+        }
+        bool write = true;
+        if (x.splits > 1) {
+            float* po = a.part_o + ((int64_t)(x.part + x.split) * kFewRows + row) * D + sub * 4;
+            for (int i = 0; i < D / 32; i++) __stcg((float4*)(po + 32 * i), y[i]);
+            if (sub == 0) __stcg(a.part_ml + (int64_t)(x.part + x.split) * kFewRows + row, make_float2(M, L));
+            __threadfence();
+            __syncthreads();
+            if (tid == 0) {
+                s_last = atomicAdd(a.arrived + x.part, 1) == x.splits - 1;
+                if (s_last) a.arrived[x.part] = 0;
+            }
+            __syncthreads();
+            write = s_last;
+            if (write) {
+                __threadfence();
+                M = -INFINITY;
+                L = 0.0f;
+                for (int s = 0; s < x.splits; s++) M = fmaxf(M, __ldcg(a.part_ml + (int64_t)(x.part + s) * kFewRows + row).x);
+#pragma unroll
+                for (int i = 0; i < D / 32; i++) y[i] = make_float4(0, 0, 0, 0);
+                for (int s = 0; s < x.splits; s++) {
+                    const float2 ml = __ldcg(a.part_ml + (int64_t)(x.part + s) * kFewRows + row);
+                    // a NaN part has a finite maximum, or none, and a sum that is one
+                    const float e = ml.x == -INFINITY && ml.y == 0.0f ? 0.0f : ml.x == -INFINITY ? 1.0f : exp2_of(ml.x - M);
+                    const float* z = a.part_o + ((int64_t)(x.part + s) * kFewRows + row) * D + sub * 4;
+                    L += ml.y * e;
+#pragma unroll
+                    for (int i = 0; i < D / 32; i++) {
+                        const float4 v = __ldcg((const float4*)(z + 32 * i));
+                        if (e != 0.0f) { y[i].x += v.x * e; y[i].y += v.y * e; y[i].z += v.z * e; y[i].w += v.w * e; }
+                    }
+                }
+            }
+        }
+        if (write && row < x.rows) {
+            const int R = x.row0 + row, tok = (int)a.group.div(R), h = x.head * (int)a.group.d + R - tok * (int)a.group.d;
+            T* out = (T*)(a.out + (int64_t)(x.r.begin + tok) * a.out_token + (int64_t)h * a.out_head) + sub * 4;
+            const float by = L == 0.0f ? 0.0f : 1.0f / L;
+            for (int i = 0; i < D / 32; i++)
+                *(uint2*)(out + 32 * i) = make_uint2(pack2<T>(y[i].x * by, y[i].y * by), pack2<T>(y[i].z * by, y[i].w * by));
+        }
+    }
+}
+
+template <int D, class T> static cudaError_t few(const AttendCall& a, int sm_count, cudaStream_t stream) {
+    const size_t smem = FewBytes<D>::fixed + items_smem(a.n_seq, kFewThreads);
+    const cudaError_t set = cudaFuncSetAttribute(attend_few_kernel<D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                 (int)(FewBytes<D>::fixed + items_smem(kCacheSeqs, kFewThreads)));
+    if (set != cudaSuccess) return set;
+    count_launch();
+    return launch_with(false, stream, attend_few_kernel<D, T>, dim3(sm_count * (D == 256 ? 1 : 2)), dim3(kFewThreads), smem, a);
+}
+template <int D> static cudaError_t few_as(const AttendCall& a, int ggml_type, int sm_count, cudaStream_t stream) {
+    return ggml_type == BIVMOE_F16 ? few<D, __half>(a, sm_count, stream) : few<D, __nv_bfloat16>(a, sm_count, stream);
+}
+cudaError_t launch_attend_few(const AttendCall& a, int head_dim, int ggml_type, int sm_count, cudaStream_t stream) {
+    switch (head_dim) {
+        case 64: return few_as<64>(a, ggml_type, sm_count, stream);
+        case 128: return few_as<128>(a, ggml_type, sm_count, stream);
+        default: return few_as<256>(a, ggml_type, sm_count, stream);
+    }
+}
+
+}  // namespace bivmoe

@@ -374,6 +374,10 @@ inline bool is_kernel(const void* func, const void* kernel) {
 }
 
 void count_launch(int n = 1);
+// for the entry points outside api.cu: cudaMalloc that remembers the size of a failed request, and the
+// message bivmoe_global_error returns (gives `code` back)
+cudaError_t dev_alloc(void** p, size_t bytes);
+int global_error(int code, const char* text);
 
 // Makes a device current for the duration of an entry point and puts the caller's
 // back afterwards (a caller with several GPUs in one process need not switch).

@@ -358,6 +358,117 @@ BIVMOE_API int bivmoe_ep_peer_wait(bivmoe_layer* layer, void* stream);
 BIVMOE_API int bivmoe_ep_peer_barrier(bivmoe_layer* layer, void* stream);
 BIVMOE_API int bivmoe_ep_peer_wait_limit(bivmoe_layer* layer, uint64_t microseconds);
 
+/* ---- The paged key/value cache of a decoder layer's attention half ----
+ *
+ * What an engine calls beside the feed-forward layer so that a decoder layer's rows stay on the
+ * device: pages for new tokens, rotary positions fused with the store of k and v into the pages,
+ * and the attention of each request's new tokens over its pages (the reference keeps a contiguous
+ * cache per sequence, engine/src/model.rs:900-1116, and runs `attn_prep`, `attn_split_*` and
+ * `attn_flash*` on it, engine/src/metal/kernels.metal:959-1573).
+ *
+ * A handle holds the geometry and the workspace; pools, tables and rows are the caller's device
+ * memory.  No call waits for the device, allocates, or reads a length on the host: everything that
+ * depends on the requests' lengths is decided on the device, so that a step can be captured into a
+ * graph.  Lengths, page numbers and slots that do not fit (a negative page, a page past the pool, a
+ * position past the table) are never followed: their keys are not visible, their rows not stored.
+ * Pointers need the alignment of their type; pools, and attend's q and out, 16 bytes, strides that
+ * are multiples of 8 values there.  Strides are in values; the head_dim values of a row's head are
+ * neighbours.  Calls of one handle use one workspace: on several streams they are ordered one after
+ * another by the handle (not while a stream is captured: there the caller orders them). */
+typedef struct bivmoe_cache bivmoe_cache;
+
+typedef struct bivmoe_cache_desc {
+    int32_t ggml_type;          /* BIVMOE_F16 or BIVMOE_BF16: pools, attend's q and out, store's q_out */
+    int32_t n_head, n_head_kv;  /* n_head a multiple of n_head_kv */
+    int32_t head_dim;           /* 64, 128 or 256 */
+    int32_t page_size;          /* tokens of a page, 1 to 65536 */
+    int32_t max_seqs;           /* requests of a call, up to 1024 */
+    int32_t max_tokens;         /* new tokens of a call, over all requests, up to 2^20 */
+    int32_t device;
+    /* rotary positions (n_rot 0: none; q and k are then stored as they are) */
+    int32_t n_rot;              /* the head's first n_rot values are turned: a multiple of 16 */
+    int32_t rope_axes;          /* 1 to 4 positions to a token (time, height, width, ...) */
+    int32_t rope_sections[4];   /* pairs turned by each axis; together n_rot / 2 */
+    int32_t rope_interleaved;   /* 0: the axes' pairs follow one another; 1: pair i belongs to axis
+                                   a = i % axes if i < axes * sections[a], else to axis 0 */
+    int32_t rope_adjacent;      /* 0: pair i is values i and i + n_rot/2; 1: values 2i and 2i + 1 */
+    double rope_base;           /* pair i turns by position * base^(-2i / n_rot) */
+} bivmoe_cache_desc;
+
+/* rows [token][head][head_dim] */
+typedef struct bivmoe_rows {
+    void* data;
+    int64_t stride_token, stride_head;
+    int32_t ggml_type;          /* F32, F16, BF16 where store reads; the cache's type elsewhere */
+    int32_t reserved;
+} bivmoe_rows;
+
+/* pages [page][token of the page][kv head][head_dim], in any order of the strides */
+typedef struct bivmoe_pool {
+    void* data;
+    int64_t stride_page, stride_token, stride_head;
+    int64_t n_pages;
+} bivmoe_pool;
+
+BIVMOE_API int bivmoe_cache_create(const bivmoe_cache_desc* desc, bivmoe_cache** out);
+BIVMOE_API void bivmoe_cache_destroy(bivmoe_cache* cache);
+
+/* Pages, slots and positions for `added[b]` new tokens of each request b, which has `past[b]`.
+ * A request holds held[b] pages (held null: ceil(past / page_size)) and gets what it needs for
+ * past + added from the end of the free list: the j-th new page of the call, in the requests' order,
+ * is free_pages[free_count - 1 - j], or -1 when there is none.  Written: the new entries of `table`;
+ * length[b] = past + added; first[b], the first row of request b among the call's new tokens, and
+ * first[n_seq], their number; for each of the n_tokens rows its slot (page * page_size + place; -1
+ * without a page and for rows past first[n_seq]) and its position (0 there); left[0] = what remains
+ * of the free list, left[1] = how many pages were missing; held_out[b] (may be null) = the pages
+ * request b holds now.  The lists given are not changed: the next call's past is this call's length. */
+typedef struct bivmoe_extend_args {
+    const int32_t *past, *added, *held;      /* device, [n_seq]; held may be null */
+    const int32_t *free_pages, *free_count;  /* device, [n_free], [1] */
+    int32_t* table;                          /* device, [n_seq][table_stride] */
+    int64_t table_stride;
+    int32_t table_width, n_free, n_seq, n_tokens;
+    int32_t *length, *first, *positions, *left, *held_out;   /* device, [n_seq], [n_seq + 1], [n_tokens], [2], [n_seq] */
+    int64_t* slots;                          /* device, [n_tokens] */
+} bivmoe_extend_args;
+BIVMOE_API int bivmoe_cache_extend(bivmoe_cache* cache, const bivmoe_extend_args* args, void* stream);
+
+/* q and k turned by the tokens' positions, q to q_out, k and v into the pages at the tokens' slots
+ * (a negative slot, or one past the pool: only q).  positions [axes][positions_stride] int32, or null
+ * where n_rot is 0.  Computed in f32 (the angle in f64, in turns), rounded once. */
+typedef struct bivmoe_store_args {
+    bivmoe_rows q, k, v, q_out;
+    bivmoe_pool k_pool, v_pool;
+    const int64_t* slots;                    /* device, [n_tokens] */
+    const int32_t* positions;
+    int64_t positions_stride;
+    int32_t n_tokens, reserved;
+} bivmoe_store_args;
+BIVMOE_API int bivmoe_cache_store(bivmoe_cache* cache, const bivmoe_store_args* args, void* stream);
+
+/* out[t] = sum over the visible keys j of softmax_j(scale * q[t] . k[j]) * v[j].  Rows first[b] to
+ * first[b + 1] - 1 are the last tokens of request b, of length[b] tokens, which the pages of
+ * table[b] hold.  A token at position p sees the positions j <= p; with window > 0 of these
+ * p - window < j and j < sinks.  A row that sees nothing is zeros; what lies in places it does not
+ * see (infinities, NaN) does not reach it.  max_new: no request has more new rows (0: not known); it
+ * decides the kernel.  Sums and softmax in f32; the weights are rounded to the cache's type for the
+ * second product.  Rows past first[n_seq] are not written. */
+typedef struct bivmoe_attend_args {
+    bivmoe_rows q, out;
+    bivmoe_pool k_pool, v_pool;
+    const int32_t* table;                    /* device, [n_seq][table_stride] */
+    int64_t table_stride;
+    int32_t table_width, n_seq, n_tokens, max_new;
+    const int32_t *first, *length;           /* device, [n_seq + 1], [n_seq] */
+    float scale;
+    int32_t window, sinks, reserved;
+} bivmoe_attend_args;
+BIVMOE_API int bivmoe_cache_attend(bivmoe_cache* cache, const bivmoe_attend_args* args, void* stream);
+
+/* Waits for the stream; BIVMOE_ERR_TIMEOUT if a bounded wait of one of the cache's kernels gave up
+ * since the last report (the results of that call are not to be used). */
+BIVMOE_API int bivmoe_cache_status(bivmoe_cache* cache, void* stream);
+
 /* The int8 tensor-pipe peak of the layer's GPU in tera-operations per second (two per
  * multiply-add), measured with back-to-back tcgen05.mma kind::i8 on resident operands
  * (about 10 ms).  A benchmark hook with no reference counterpart: the roofline
