@@ -16,12 +16,18 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import struct
 from typing import NamedTuple, Optional, Sequence
 
 import torch
 
 from . import capi
 
+# bivmoe_extend_args, bivmoe_store_args and bivmoe_attend_args field by field (native order, C's alignment)
+_ROWS, _POOL = "Pqqii", "Pqqqq"
+_EXTEND = struct.Struct("6Pq4i6P").pack_into
+_STORE = struct.Struct(_ROWS * 4 + _POOL * 2 + "2Pq2i").pack_into
+_ATTEND = struct.Struct(_ROWS * 2 + _POOL * 2 + "Pq4i2Pf3i").pack_into
 _GGML = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
 
 
@@ -72,12 +78,20 @@ class PagedCache:
         self._h = h
         self.n_head, self.n_head_kv, self.head_dim, self.page_size = n_head, n_head_kv, head_dim, page_size
         self.max_seqs, self.max_tokens, self.dtype, self.rope, self.device = max_seqs, max_tokens, dtype, rope, device
-        self._dev = torch.device("cuda", device)
-        self._scale = 1.0 / math.sqrt(head_dim)
-        # the structs of a call, filled in anew each time: what does not change is set here
-        self._e, self._s, self._a = capi.ExtendArgs(), capi.StoreArgs(), capi.AttendArgs()
-        self._s.q_out_type = self._a.q_type = self._a.out_type = _GGML[dtype]
-        self._refs = C.byref(self._e), C.byref(self._s), C.byref(self._a)
+        self._set_up(torch.device("cuda", device))
+
+    def _set_up(self, dev):
+        self._dev = dev
+        L = capi.lib()
+        self._calls = L.bivmoe_cache_extend, L.bivmoe_cache_store, L.bivmoe_cache_attend
+        self._scale = 1.0 / math.sqrt(self.head_dim)
+        # A call's arguments are packed anew for every launch, into a buffer of the struct's size; a step
+        # of small kernels is bound by the host, so one pack and few attribute look-ups.
+        self._bufs = [C.create_string_buffer(C.sizeof(t)) for t in (capi.ExtendArgs, capi.StoreArgs, capi.AttendArgs)]
+        self._refs = [C.cast(b, C.POINTER(t)) for b, t in zip(self._bufs, (capi.ExtendArgs, capi.StoreArgs, capi.AttendArgs))]
+        self._ggml = _GGML[self.dtype]
+        self._pool_shape = (self.page_size, self.n_head_kv, self.head_dim)
+        self._axes = len(self.rope.sections) if self.rope is not None else 0
 
     def close(self):
         if self._h is not None:
@@ -90,11 +104,14 @@ class PagedCache:
         except Exception:
             pass
 
-    def _stream(self):
-        return torch.cuda.current_stream(self._dev).cuda_stream
+    def _call(self, i, pack, *values):
+        pack(self._bufs[i], 0, *values)
+        code = self._calls[i](self._h, self._refs[i], torch.cuda.current_stream(self._dev).cuda_stream)
+        if code:
+            capi.check(code)
 
     def _ints(self, t, what, n, dtype=torch.int32):
-        if t.dtype != dtype or t.device != self._dev or not t.is_contiguous() or t.numel() < n:
+        if t.dtype is not dtype or t.device != self._dev or not t.is_contiguous() or t.numel() < n:
             raise ValueError(f"{what}: {n} contiguous {dtype} on {self._dev} are wanted")
         return t.data_ptr()
 
@@ -103,29 +120,36 @@ class PagedCache:
         shape = (n_pages, self.page_size, self.n_head_kv, self.head_dim)
         return tuple(torch.empty(shape, dtype=self.dtype, device=self._dev) for _ in range(2))
 
-    def _table(self, a, table, n_seq):
-        if table.dtype != torch.int32 or table.device != self._dev or table.dim() != 2 or table.shape[0] < n_seq or \
-                (table.shape[1] > 1 and table.stride(1) != 1):
-            raise ValueError("table: [n_seq, pages] int32 with neighbouring pages is wanted")
-        a.table, a.table_stride, a.table_width, a.n_seq = table.data_ptr(), table.stride(0), table.shape[1], n_seq
+    def _table(self, t, n_seq):
+        """address, stride, width"""
+        if t.dtype is not torch.int32 or t.device != self._dev or t.dim() != 2:
+            raise ValueError("table: [n_seq, pages] int32 is wanted")
+        rows, width = t.shape
+        stride, one = t.stride()
+        if rows < n_seq or (width > 1 and one != 1):
+            raise ValueError("table: [n_seq, pages] with neighbouring pages is wanted")
+        return t.data_ptr(), stride, width
 
-    def _pool(self, a, name, t):
-        shape = t.shape
-        if t.dtype != self.dtype or t.device != self._dev or len(shape) != 4 or shape[1] != self.page_size or \
-                shape[2] != self.n_head_kv or shape[3] != self.head_dim or t.stride(3) != 1:
+    def _pool(self, t, name):
+        """address, strides of a page, a token and a head, pages: a ``bivmoe_pool``"""
+        shape, stride = t.shape, t.stride()
+        if t.dtype is not self.dtype or t.device != self._dev or shape[1:] != self._pool_shape or stride[3] != 1:
             raise ValueError(f"{name}: [pages, {self.page_size}, {self.n_head_kv}, {self.head_dim}] of {self.dtype} is wanted")
-        p, k, h, _ = t.stride()
-        if name == "k_pool":
-            a.k_pool, a.k_pool_stride_page, a.k_pool_stride_token, a.k_pool_stride_head, a.k_pool_n_pages = t.data_ptr(), p, k, h, shape[0]
-        else:
-            a.v_pool, a.v_pool_stride_page, a.v_pool_stride_token, a.v_pool_stride_head, a.v_pool_n_pages = t.data_ptr(), p, k, h, shape[0]
+        return t.data_ptr(), stride[0], stride[1], stride[2], shape[0]
 
-    def _rows(self, t, what, heads, n=None):
-        shape = t.shape
-        if t.device != self._dev or len(shape) != 3 or shape[1] != heads or shape[2] != self.head_dim or t.stride(2) != 1 or \
-                (n is not None and shape[0] != n):
+    def _rows(self, t, what, heads, n):
+        """address, strides of a token and a head"""
+        stride = t.stride()
+        if t.shape != (n, heads, self.head_dim) or stride[2] != 1 or t.device != self._dev:
             raise ValueError(f"{what}: [tokens, {heads}, {self.head_dim}] rows on {self._dev} are wanted")
-        return t.data_ptr(), t.stride(0), t.stride(1)
+        return t.data_ptr(), stride[0], stride[1]
+
+    def _out(self, out, q):
+        if out is None:
+            return torch.empty_like(q, dtype=self.dtype)
+        if out.dtype is not self.dtype:
+            raise ValueError(f"out: {self.dtype} is wanted")
+        return out
 
     def extend(self, past, added, free_pages, free_count, table, n_tokens: int, held=None, out: Optional[Step] = None) -> Step:
         """Pages for ``added[b]`` new tokens of each request b, which has ``past[b]`` (int32 device
@@ -134,52 +158,40 @@ class PagedCache:
         more than the requests add (a padded batch) have slot -1.  ``held``: pages each request holds
         already, where that is not what ``past`` needs (drafted tokens that were taken back); ``out``:
         a step to write into."""
-        n_seq, a = past.numel(), self._e
+        n_seq = past.numel()
         if out is None:
-            i32 = dict(dtype=torch.int32, device=self._dev)
-            room = torch.empty(3 * n_seq + 3 + n_tokens, **i32)
-            length, first, left, kept, positions = room.split([n_seq, n_seq + 1, 2, n_seq, n_tokens])
+            room = torch.empty(3 * n_seq + 3 + n_tokens, dtype=torch.int32, device=self._dev)
+            length, first, left, kept, positions = room.split((n_seq, n_seq + 1, 2, n_seq, n_tokens))
             out = Step(length, first, torch.empty(n_tokens, dtype=torch.int64, device=self._dev), positions, left, kept)
-        a.past, a.added = self._ints(past, "past", n_seq), self._ints(added, "added", n_seq)
-        a.held = None if held is None else self._ints(held, "held", n_seq)
-        a.free_pages, a.n_free = self._ints(free_pages, "free_pages", 0), free_pages.numel()
-        a.free_count = self._ints(free_count, "free_count", 1)
-        self._table(a, table, n_seq)
-        a.n_tokens = n_tokens
-        a.length, a.first = self._ints(out.length, "length", n_seq), self._ints(out.first, "first", n_seq + 1)
-        a.slots = self._ints(out.slots, "slots", n_tokens, torch.int64)
-        a.positions, a.left = self._ints(out.positions, "positions", n_tokens), self._ints(out.left, "left", 2)
-        a.held_out = self._ints(out.held, "held", n_seq)
-        capi.check(capi.lib().bivmoe_cache_extend(self._h, self._refs[0], self._stream()))
+            wrote = [t.data_ptr() for t in (length, first, positions, left, kept, out.slots)]
+        else:
+            wrote = [self._ints(out.length, "length", n_seq), self._ints(out.first, "first", n_seq + 1),
+                     self._ints(out.positions, "positions", n_tokens), self._ints(out.left, "left", 2),
+                     self._ints(out.held, "held", n_seq), self._ints(out.slots, "slots", n_tokens, torch.int64)]
+        self._call(0, _EXTEND, self._ints(past, "past", n_seq), self._ints(added, "added", n_seq),
+                   0 if held is None else self._ints(held, "held", n_seq), self._ints(free_pages, "free_pages", 0),
+                   self._ints(free_count, "free_count", 1), *self._table(table, n_seq), free_pages.numel(), n_seq, n_tokens, *wrote)
         return out
 
     def store(self, q, k, v, k_pool, v_pool, slots, positions=None, out=None):
         """q and k [n, heads, head_dim] (float32, float16 or bfloat16; any strides of the first two)
         turned by ``positions`` ([n], or [axes, n]), k and v into the pages at ``slots``; returns the
         turned q in the cache's type."""
-        n, a = q.shape[0], self._s
-        a.q, a.q_stride_token, a.q_stride_head = self._rows(q, "q", self.n_head)
-        a.k, a.k_stride_token, a.k_stride_head = self._rows(k, "k", self.n_head_kv, n)
-        a.v, a.v_stride_token, a.v_stride_head = self._rows(v, "v", self.n_head_kv, n)
-        if q.dtype not in _GGML or k.dtype != q.dtype or v.dtype != q.dtype:
+        n, ty = q.shape[0], _GGML.get(q.dtype)
+        if ty is None or k.dtype is not q.dtype or v.dtype is not q.dtype:
             raise ValueError("q, k and v: rows of one type, float32, float16 or bfloat16, are wanted")
-        a.q_type = a.k_type = a.v_type = _GGML[q.dtype]
-        if out is None:
-            out = torch.empty((n, self.n_head, self.head_dim), dtype=self.dtype, device=self._dev)
-        elif out.dtype != self.dtype:
-            raise ValueError(f"out: {self.dtype} is wanted")
-        a.q_out, a.q_out_stride_token, a.q_out_stride_head = self._rows(out, "out", self.n_head, n)
-        self._pool(a, "k_pool", k_pool)
-        self._pool(a, "v_pool", v_pool)
-        a.slots, a.n_tokens = self._ints(slots, "slots", n, torch.int64), n
-        a.positions, a.positions_stride = None, 0
-        if self.rope is not None:
-            axes = len(self.rope.sections)
-            if positions is None or positions.dtype != torch.int32 or positions.device != self._dev or \
-                    positions.numel() != axes * n or (n > 1 and positions.stride(-1) != 1):
-                raise ValueError(f"positions: [{axes}, n] int32 are wanted" if axes > 1 else "positions: [n] int32 are wanted")
-            a.positions, a.positions_stride = positions.data_ptr(), positions.stride(0) if positions.dim() > 1 else n
-        capi.check(capi.lib().bivmoe_cache_store(self._h, self._refs[1], self._stream()))
+        out = self._out(out, q)
+        where, stride = 0, 0
+        if self._axes:
+            if positions is None or positions.dtype is not torch.int32 or positions.device != self._dev or \
+                    positions.numel() != self._axes * n or (n > 1 and positions.stride(-1) != 1):
+                raise ValueError(f"positions: [{self._axes}, n] int32 are wanted" if self._axes > 1 else "positions: [n] int32 are wanted")
+            where, stride = positions.data_ptr(), positions.stride(0) if positions.dim() > 1 else n
+        kv = self.n_head_kv
+        self._call(1, _STORE, *self._rows(q, "q", self.n_head, n), ty, 0, *self._rows(k, "k", kv, n), ty, 0,
+                   *self._rows(v, "v", kv, n), ty, 0, *self._rows(out, "out", self.n_head, n), self._ggml, 0,
+                   *self._pool(k_pool, "k_pool"), *self._pool(v_pool, "v_pool"),
+                   self._ints(slots, "slots", n, torch.int64), where, stride, n, 0)
         return out
 
     def attend(self, q, k_pool, v_pool, table, first, length, max_new: int = 0, scale: Optional[float] = None,
@@ -188,26 +200,17 @@ class PagedCache:
         the last tokens of its length[b] tokens.  A token at position p sees p and what is before it;
         with ``window`` the last ``window`` positions up to its own and the first ``sinks``.  ``max_new``:
         the most new rows of a request, where the caller knows it."""
-        n_seq, a = length.numel(), self._a
-        if q.dtype != self.dtype:
+        n, n_seq = q.shape[0], length.numel()
+        if q.dtype is not self.dtype:
             raise ValueError(f"q: {self.dtype} is wanted")
-        a.q, a.q_stride_token, a.q_stride_head = self._rows(q, "q", self.n_head)
-        n = q.shape[0]
-        if out is None:
-            out = torch.empty((n, self.n_head, self.head_dim), dtype=self.dtype, device=self._dev)
-        elif out.dtype != self.dtype:
-            raise ValueError(f"out: {self.dtype} is wanted")
-        a.out, a.out_stride_token, a.out_stride_head = self._rows(out, "out", self.n_head, n)
-        self._pool(a, "k_pool", k_pool)
-        self._pool(a, "v_pool", v_pool)
-        self._table(a, table, n_seq)
-        a.first, a.length = self._ints(first, "first", n_seq + 1), self._ints(length, "length", n_seq)
-        a.n_tokens, a.max_new = n, max_new
-        a.scale, a.window, a.sinks = self._scale if scale is None else scale, window, sinks
-        capi.check(capi.lib().bivmoe_cache_attend(self._h, self._refs[2], self._stream()))
+        out = self._out(out, q)
+        self._call(2, _ATTEND, *self._rows(q, "q", self.n_head, n), self._ggml, 0, *self._rows(out, "out", self.n_head, n), self._ggml, 0,
+                   *self._pool(k_pool, "k_pool"), *self._pool(v_pool, "v_pool"), *self._table(table, n_seq), n_seq, n, max_new,
+                   self._ints(first, "first", n_seq + 1), self._ints(length, "length", n_seq),
+                   self._scale if scale is None else scale, window, sinks, 0)
         return out
 
     def status(self):
         """Waits for the current stream and raises if a kernel of this cache gave up on a bounded wait
         since the last report."""
-        capi.check(capi.lib().bivmoe_cache_status(self._h, self._stream()))
+        capi.check(capi.lib().bivmoe_cache_status(self._h, torch.cuda.current_stream(self._dev).cuda_stream))

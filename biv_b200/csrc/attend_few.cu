@@ -3,10 +3,11 @@
 //
 //   s_j = scale q . k_j,  m = max s_j,  l = sum 2^(s_j - m),  o = sum 2^(s_j - m) v_j / l   (s in powers of two)
 //
-// A block is four warps; of a tile of 64 keys warp w takes 16, in a ring of its own in shared memory
+// A block is four warps; of a tile of 64 keys (heads of 64 values: 128) a warp takes a quarter, in a ring of its own in shared memory
 // that its own cp.async copies fill, with its own running maximum, sum and o: the warps meet at the
-// item's end only, where the four o are joined.  A long axis is cut into pieces over blocks (cache.cuh);
-// the block that is last to finish a tile joins the pieces, in the pieces' order whoever is last.
+// piece's end only, where the four o are joined.  The work is shared out over blocks wherever that cuts a
+// long axis (cache.cuh); the block that is last to finish a tile joins its pieces, in their own order
+// whoever is last.
 // With one new token a request the keys are read once: bound by memory.
 #include "cache.cuh"
 #include "common.cuh"
@@ -15,7 +16,8 @@
 
 namespace bivmoe {
 
-constexpr int kFewWarps = 4, kFewThreads = 32 * kFewWarps, kFewKeys = 16 * kFewWarps, kFewStages = 3;
+constexpr int kFewWarps = 4, kFewThreads = 32 * kFewWarps, kFewStages = 3;
+constexpr int kFewLeast = 2;      // key tiles that are worth a block
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool there) {
     // nothing is read, and zeros are written, where there is nothing
@@ -41,10 +43,13 @@ template <> __device__ __forceinline__ void mma16<__half>(float (&d)[4], const u
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-template <int D> struct FewBytes {
-    static constexpr int stage = 2 * 16 * D * 2;      // 16 keys' k and v
+// Keys of a warp's stage: what a stage costs beside its copies and products (pages, barriers, the running
+// maximum) is the same for 16 keys of 64 values and of 256.
+template <int D> struct Few {
+    static constexpr int keys = D == 64 ? 32 : 16, tile = keys * kFewWarps;
+    static constexpr int half = keys * D * 2, stage = 2 * half;   // bytes: k, then v
     static constexpr int ring = kFewWarps * kFewStages * stage;
-    static constexpr int fixed = ring + 16 * D * 2;   // and the 16 rows of q
+    static constexpr int fixed = ring + 16 * D * 2;               // and the 16 rows of q
 };
 
 // 16-byte piece `c` of row `r`: the low three bits of the piece's place are turned by the row, so that
@@ -56,20 +61,20 @@ template <int D> __device__ __forceinline__ uint32_t few_at(int r, int c) {
 template <int D, class T>
 __global__ void __launch_bounds__(kFewThreads, D == 256 ? 1 : 2) attend_few_kernel(AttendCall a) {
     extern __shared__ __align__(1024) uint8_t sm[];
+    constexpr int KW = Few<D>::keys, KT = Few<D>::tile;
     __shared__ float s_m[kFewWarps][16], s_l[kFewWarps][16];
     __shared__ int s_bad[16], s_last;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    uint8_t* ring_p = sm + warp * kFewStages * FewBytes<D>::stage;
-    const uint32_t ring = pf_smem(ring_p), qs = pf_smem(sm + FewBytes<D>::ring);
+    uint8_t* ring_p = sm + warp * kFewStages * Few<D>::stage;
+    const uint32_t ring = pf_smem(ring_p), qs = pf_smem(sm + Few<D>::ring);
     pdl_enter();
-    const Items it = find_items<kFewKeys, kFewRows, kFewThreads>(a, 2, (int*)(sm + FewBytes<D>::fixed));
+    const Share share = find_share<KT, kFewRows, kFewThreads>(a, kFewLeast, (int64_t*)(sm + Few<D>::fixed));
     const int g = lane >> 2, quad = lane & 3;
     constexpr int CH = D / 8, RPI = 32 / CH;      // 16-byte pieces of a row, rows of a warp's copy
 
-    for (int index = blockIdx.x; index < it.total; index += gridDim.x) {
-        const Item x = item_at<kFewKeys, kFewRows>(a, it, index);
-        if (item_void(x)) continue;
-        __syncthreads();                          // the item before is done with the rings and the rows
+    Walk<KT, kFewRows> walk(a, share);
+    for (Piece x; walk.next(x);) {
+        __syncthreads();                          // the piece before is done with the rings and the rows
         const int32_t* table = a.table + (int64_t)x.b * a.table_stride;
         // the rows: past the tile's, zeros
         for (int i = tid; i < 16 * CH; i += kFewThreads) {
@@ -78,11 +83,11 @@ __global__ void __launch_bounds__(kFewThreads, D == 256 ? 1 : 2) attend_few_kern
             cp16(qs + few_at<D>(r, c), there ? a.q + (int64_t)(x.r.begin + tok) * a.q_token + (int64_t)h * a.q_head + c * 16 : a.q, there);
         }
         cp_commit();
-        const int n = max(x.i1 - x.i0, 0), p_top = x.r.past + (int)a.group.div(x.row0 + x.rows - 1);
+        const int n = x.n, p_first = x.r.past + (int)a.group.div(x.row0), p_top = x.r.past + (int)a.group.div(x.row0 + x.rows - 1);
         const uint8_t *k_base = a.k.data + x.head * a.k.head, *v_base = a.v.data + x.head * a.v.head;
-        // lane r of the first 16: where key r of the warp's next stage lies
+        // lane r: where key r of the warp's next stage lies
         auto find = [&](int i, int64_t& ko, int64_t& vo, bool& ok) {
-            const int j = x.tiles.tile(x.i0 + i) * kFewKeys + warp * 16 + (lane & 15);
+            const int j = x.tiles.tile(x.i0 + i) * KT + warp * KW + (lane & (KW - 1));
             int at = 0;
             const int page = i < n && j <= p_top ? page_of(a, table, j, at) : -1;
             ok = page >= 0;
@@ -94,15 +99,15 @@ __global__ void __launch_bounds__(kFewThreads, D == 256 ? 1 : 2) attend_few_kern
         bool ok;
         find(0, ko, vo, ok);
         auto copy = [&](int i, int slot) {        // stage i, whose keys have been found; finds the next one's
-            const uint32_t mask = __ballot_sync(0xffffffffu, ok) & 0xffffu;
-            const uint32_t dst = ring + slot * FewBytes<D>::stage;
+            const uint32_t mask = __ballot_sync(0xffffffffu, ok);   // KW 16: twice the same
+            const uint32_t dst = ring + slot * Few<D>::stage;
             if (i < n) {
 #pragma unroll
-                for (int e = 0; e < 16 / RPI; e++) {
+                for (int e = 0; e < KW / RPI; e++) {
                     const int r = e * RPI + lane / CH, c = lane % CH;
                     const int64_t kr = __shfl_sync(0xffffffffu, ko, r), vr = __shfl_sync(0xffffffffu, vo, r);
                     cp16(dst + few_at<D>(r, c), k_base + kr + c * 16, mask >> r & 1);
-                    cp16(dst + 16 * D * 2 + few_at<D>(r, c), v_base + vr + c * 16, mask >> r & 1);
+                    cp16(dst + Few<D>::half + few_at<D>(r, c), v_base + vr + c * 16, mask >> r & 1);
                 }
             }
             cp_commit();
@@ -134,28 +139,42 @@ __global__ void __launch_bounds__(kFewThreads, D == 256 ? 1 : 2) attend_few_kern
                 there[(u + kFewStages - 1) % kFewStages] = copy(i + kFewStages - 1, (u + kFewStages - 1) % kFewStages);
                 cp_wait<kFewStages - 1>();
                 __syncwarp();
-                const uint32_t ks = ring + u * FewBytes<D>::stage, vs = ks + 16 * D * 2;
-                float s[2][4] = {};
+                const uint32_t ks = ring + u * Few<D>::stage, vs = ks + Few<D>::half;
+                float s[KW / 8][4] = {};
 #pragma unroll
                 for (int k = 0; k < D / 16; k++) {
-                    uint32_t b[4], again[4];
-                    ldm4(ks + few_at<D>((lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1)), b);
+                    uint32_t again[4];
                     if (!HOLD) ldm4(qs + few_at<D>(lane & 15, 2 * k + (lane >> 4)), again);
                     const uint32_t(&qk)[4] = HOLD ? qf[HOLD ? k : 0] : again;
-                    mma16<T>(s[0], qk, b[0], b[1]);
-                    mma16<T>(s[1], qk, b[2], b[3]);
+#pragma unroll
+                    for (int t = 0; t < KW / 16; t++) {
+                        uint32_t b[4];
+                        ldm4(ks + few_at<D>(16 * t + (lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1)), b);
+                        mma16<T>(s[2 * t], qk, b[0], b[1]);
+                        mma16<T>(s[2 * t + 1], qk, b[2], b[3]);
+                    }
                 }
-                const int j0 = x.tiles.tile(x.i0 + i) * kFewKeys + warp * 16;
+                const int j0 = x.tiles.tile(x.i0 + i) * KT + warp * KW;
+                // most stages lie where all rows see all keys: no comparison by key
+                const bool all = there[u] == 0xffffffffu && j0 + KW - 1 <= p_first &&
+                                 (a.window <= 0 || p_top - j0 < a.window || j0 + KW <= a.sinks);
                 float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-                for (int t = 0; t < 2; t++)
+                for (int t = 0; t < KW / 8; t++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const int r = t * 8 + quad * 2 + (e & 1);
-                        const bool see = (there[u] >> r & 1) && sees(a, p[e >> 1], j0 + r);
-                        s[t][e] = see ? s[t][e] * a.scale_log2 : -INFINITY;
-                        top[e >> 1] = fmaxf(top[e >> 1], s[t][e]);
-                    }
+                    for (int e = 0; e < 4; e++) s[t][e] *= a.scale_log2;
+                if (!all)
+#pragma unroll
+                    for (int t = 0; t < KW / 8; t++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const int r = t * 8 + quad * 2 + (e & 1);
+                            if (!(there[u] >> r & 1) || !sees(a, p[e >> 1], j0 + r)) s[t][e] = -INFINITY;
+                        }
+#pragma unroll
+                for (int t = 0; t < KW / 8; t++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) top[e >> 1] = fmaxf(top[e >> 1], s[t][e]);
                 float keep[2];
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
@@ -168,7 +187,7 @@ __global__ void __launch_bounds__(kFewThreads, D == 256 ? 1 : 2) attend_few_kern
                     l[e] *= keep[e];
                 }
 #pragma unroll
-                for (int t = 0; t < 2; t++)
+                for (int t = 0; t < KW / 8; t++)
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
                         s[t][e] = exp2_of(s[t][e] - top[e >> 1]);
@@ -176,16 +195,22 @@ __global__ void __launch_bounds__(kFewThreads, D == 256 ? 1 : 2) attend_few_kern
                     }
                 // the weights, at most 1, rounded to the cache's type for the second product (relative
                 // error 2^-9 or 2^-12 each); l sums them unrounded
-                const uint32_t w[4] = {pack2<T>(s[0][0], s[0][1]), pack2<T>(s[0][2], s[0][3]), pack2<T>(s[1][0], s[1][1]),
-                                       pack2<T>(s[1][2], s[1][3])};
+                uint32_t w[KW / 16][4];
+#pragma unroll
+                for (int t = 0; t < KW / 16; t++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) w[t][e] = pack2<T>(s[2 * t + (e >> 1)][2 * (e & 1)], s[2 * t + (e >> 1)][2 * (e & 1) + 1]);
 #pragma unroll
                 for (int c = 0; c < D / 8; c += 2) {
-                    uint32_t b[4];
-                    ldm4t(vs + few_at<D>((lane & 7) + ((lane >> 3 & 1) << 3), c + (lane >> 4)), b);
 #pragma unroll
                     for (int e = 0; e < 4; e++) { o[c][e] *= keep[e >> 1]; o[c + 1][e] *= keep[e >> 1]; }
-                    mma16<T>(o[c], w, b[0], b[1]);
-                    mma16<T>(o[c + 1], w, b[2], b[3]);
+#pragma unroll
+                    for (int t = 0; t < KW / 16; t++) {
+                        uint32_t b[4];
+                        ldm4t(vs + few_at<D>(16 * t + (lane & 7) + ((lane >> 3 & 1) << 3), c + (lane >> 4)), b);
+                        mma16<T>(o[c], w[t], b[0], b[1]);
+                        mma16<T>(o[c + 1], w[t], b[2], b[3]);
+                    }
                 }
                 __syncwarp();
             }
@@ -221,7 +246,7 @@ __global__ void __launch_bounds__(kFewThreads, D == 256 ? 1 : 2) attend_few_kern
             float4 v = make_float4(0, 0, 0, 0);
 #pragma unroll
             for (int w = 0; w < kFewWarps; w++) {
-                const float4 z = *(const float4*)(sm + w * kFewStages * FewBytes<D>::stage + (row * D + sub * 4 + 32 * i) * 4);
+                const float4 z = *(const float4*)(sm + w * kFewStages * Few<D>::stage + (row * D + sub * 4 + 32 * i) * 4);
                 if (f[w] != 0.0f) { v.x += z.x * f[w]; v.y += z.y * f[w]; v.z += z.z * f[w]; v.w += z.w * f[w]; }
             }
             y[i] = v;
@@ -233,7 +258,7 @@ __global__ void __launch_bounds__(kFewThreads, D == 256 ? 1 : 2) attend_few_kern
             for (int r = warp; r < x.rows; r += kFewWarps) {
                 if (!s_bad[r]) continue;
                 float c[D / 32], cm, cl;
-                careful_row<D, T>(a, x, r, kFewKeys, c, cm, cl);
+                careful_row<D, T>(a, x, r, KT, c, cm, cl);
                 for (int e = 0; e < D / 32; e++) ((float*)sm)[r * D + lane + 32 * e] = c[e];
                 if (lane == 0) { s_m[0][r] = cm; s_l[0][r] = cl; }
             }
@@ -245,15 +270,16 @@ __global__ void __launch_bounds__(kFewThreads, D == 256 ? 1 : 2) attend_few_kern
             }
         }
         bool write = true;
-        if (x.splits > 1) {
-            float* po = a.part_o + ((int64_t)(x.part + x.split) * kFewRows + row) * D + sub * 4;
+        if (x.parts > 1) {
+            const int mine = x.slot(x.part);
+            float* po = a.part_o + ((int64_t)mine * kFewRows + row) * D + sub * 4;
             for (int i = 0; i < D / 32; i++) __stcg((float4*)(po + 32 * i), y[i]);
-            if (sub == 0) __stcg(a.part_ml + (int64_t)(x.part + x.split) * kFewRows + row, make_float2(M, L));
+            if (sub == 0) __stcg(a.part_ml + (int64_t)mine * kFewRows + row, make_float2(M, L));
             __threadfence();
             __syncthreads();
             if (tid == 0) {
-                s_last = atomicAdd(a.arrived + x.part, 1) == x.splits - 1;
-                if (s_last) a.arrived[x.part] = 0;
+                s_last = atomicAdd(a.arrived + x.c0, 1) == x.parts - 1;
+                if (s_last) a.arrived[x.c0] = 0;
             }
             __syncthreads();
             write = s_last;
@@ -261,14 +287,14 @@ __global__ void __launch_bounds__(kFewThreads, D == 256 ? 1 : 2) attend_few_kern
                 __threadfence();
                 M = -INFINITY;
                 L = 0.0f;
-                for (int s = 0; s < x.splits; s++) M = fmaxf(M, __ldcg(a.part_ml + (int64_t)(x.part + s) * kFewRows + row).x);
+                for (int s = 0; s < x.parts; s++) M = fmaxf(M, __ldcg(a.part_ml + (int64_t)x.slot(s) * kFewRows + row).x);
 #pragma unroll
                 for (int i = 0; i < D / 32; i++) y[i] = make_float4(0, 0, 0, 0);
-                for (int s = 0; s < x.splits; s++) {
-                    const float2 ml = __ldcg(a.part_ml + (int64_t)(x.part + s) * kFewRows + row);
+                for (int s = 0; s < x.parts; s++) {
+                    const float2 ml = __ldcg(a.part_ml + (int64_t)x.slot(s) * kFewRows + row);
                     // a NaN part has a finite maximum, or none, and a sum that is one
                     const float e = ml.x == -INFINITY && ml.y == 0.0f ? 0.0f : ml.x == -INFINITY ? 1.0f : exp2_of(ml.x - M);
-                    const float* z = a.part_o + ((int64_t)(x.part + s) * kFewRows + row) * D + sub * 4;
+                    const float* z = a.part_o + ((int64_t)x.slot(s) * kFewRows + row) * D + sub * 4;
                     L += ml.y * e;
 #pragma unroll
                     for (int i = 0; i < D / 32; i++) {
@@ -289,12 +315,11 @@ __global__ void __launch_bounds__(kFewThreads, D == 256 ? 1 : 2) attend_few_kern
 }
 
 template <int D, class T> static cudaError_t few(const AttendCall& a, int sm_count, cudaStream_t stream) {
-    const size_t smem = FewBytes<D>::fixed + items_smem(a.n_seq, kFewThreads);
-    const cudaError_t set = cudaFuncSetAttribute(attend_few_kernel<D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                 (int)(FewBytes<D>::fixed + items_smem(kCacheSeqs, kFewThreads)));
-    if (set != cudaSuccess) return set;
+    const size_t smem = Few<D>::fixed + share_smem(a.n_seq, kFewThreads);
+    static std::atomic<uint64_t> attr_set{0};
+    if (cudaError_t e = ensure_dynamic_smem(attend_few_kernel<D, T>, (int)(Few<D>::fixed + share_smem(kCacheSeqs, kFewThreads)), attr_set)) return e;
     count_launch();
-    return launch_with(false, stream, attend_few_kernel<D, T>, dim3(sm_count * (D == 256 ? 1 : 2)), dim3(kFewThreads), smem, a);
+    return launch_with(false, stream, attend_few_kernel<D, T>, dim3(sm_count * (D == 256 ? 1 : kFewBlocks)), dim3(kFewThreads), smem, a);
 }
 template <int D> static cudaError_t few_as(const AttendCall& a, int ggml_type, int sm_count, cudaStream_t stream) {
     return ggml_type == BIVMOE_F16 ? few<D, __half>(a, sm_count, stream) : few<D, __nv_bfloat16>(a, sm_count, stream);

@@ -1,0 +1,571 @@
+// Attention over the pages for tiles of 128 and 256 rows on the fifth-generation tensor cores.
+//
+//   S = Q K^T (128 rows x 128 keys),  P = 2^(scale S - m),  O += P V,  o = O / sum P
+//
+// One block per SM takes its share of the work (cache.cuh) and has three kinds of warps:
+//
+//   warps 0-7    two groups of 128 threads, a thread to a row: S from tensor memory, its maximum, the
+//                powers, P as 16-bit values back into tensor memory over S; at a piece's start the
+//                rows' Q into shared memory, at its end O out.
+//   warp 8       one lane issues the MMAs.  K and V stand in shared memory in rows of 64 values
+//                (128-byte swizzle): K is read along the values (K-major), V along the keys (MN-major),
+//                so that neither is turned; P is read from tensor memory.
+//   warps 9-11   copy K and V from the pages, 128 keys x 64 values (16 KB) a slot, in a ring of eight:
+//                cp.async in 16-byte pieces, since a tile's keys lie in pages of any size.
+//
+// Heads of up to 128 values: two tiles of 128 rows at once, a group each, so that one group's powers
+// run while the other's products do.  Heads of 256 values, whose O alone takes half of tensor memory,
+// and pieces of up to 128 rows: one tile with two S, the next product into one while the first group
+// works on the other.
+// m is not the running maximum itself but one that follows it when it has grown by more than 2^8:
+// O is then scaled in tensor memory, which happens a few times at a piece's start and rarely after (P
+// is at most 2^8, its sum and O are held in f32).
+#include <stddef.h>
+
+#include "cache.cuh"
+#include "common.cuh"
+#include "launch.cuh"
+#include "tcgen05.cuh"
+
+namespace bivmoe {
+
+constexpr int AT_KEYS = 128, AT_SLOT = AT_KEYS * 128, AT_SLOTS = 8;
+constexpr int AT_THREADS = 384, AT_COPY_WARPS = 3, AT_MMA_WARP = 8;
+constexpr int AT_HEAD = 1024;
+constexpr float AT_GROWTH = 8.0f;     // powers of two
+enum { AT_SITE_COPY = 31, AT_SITE_MMA, AT_SITE_ROWS };
+
+template <int D> struct At {
+    static constexpr int tiles = D == 256 ? 1 : 2;           // of 128 rows
+    static constexpr int rows = 128 * tiles;
+    static constexpr int chunks = D / 64;                    // slots of a tile of K, or of V
+    static constexpr int q_tile = 128 * D * 2;
+    static constexpr int fixed = AT_HEAD + tiles * q_tile + AT_SLOTS * AT_SLOT;
+};
+
+struct AtHead {
+    uint64_t full[AT_SLOTS], empty[AT_SLOTS];
+    // [0], [1]: of the two tiles of a pair; [2], [3]: of the two S of a single tile.  Apart, because the
+    // second group passes single tiles by: a parity tells a phase from the next one only.
+    uint64_t s_full[4], p_full[4], q_full[2], pv_done[2], drained;
+    alignas(16) uint32_t there[8][4];   // read 16 bytes at once: which keys of a K tile lie in pages that there are
+    uint32_t tmem;
+    int abort;
+};
+static_assert(sizeof(AtHead) <= AT_HEAD && offsetof(AtHead, there) % 16 == 0, "");
+
+__device__ __forceinline__ bool at_wait(uint64_t* bar, uint32_t parity, const int* abort) {
+    return bounded_wait<256>(PfWait<false, false>{bar, parity, abort});
+}
+__device__ __forceinline__ bool at_wait_warp(uint64_t* bar, uint32_t parity, const int* abort) {
+    return bounded_wait_together<256>(PfWait<false, false>{bar, parity, abort});
+}
+__device__ __forceinline__ void at_cp16(uint32_t dst, const void* src, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+// the thread's arrival, once its copies so far have landed
+__device__ __forceinline__ void at_cp_arrive(uint64_t* bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(pf_smem(bar)) : "memory");
+}
+// what threads have written to shared memory, or have seen written, before what the tensor cores read
+__device__ __forceinline__ void at_fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void at_tmem_st32(uint32_t taddr, const uint32_t* v) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
+        "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
+        "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+        : "memory");
+}
+__device__ __forceinline__ void at_tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// A in tensor memory
+__device__ __forceinline__ void at_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem), "r"(a_tmem), "l"(bdesc), "r"(idesc),
+        "r"(accumulate)
+        : "memory");
+}
+// kind::f16, f32 accumulator, A and B of T; B along its rows (MN-major) or along K
+template <class T> __device__ __forceinline__ constexpr uint32_t at_idesc(int n, bool b_mn);
+template <> __device__ __forceinline__ constexpr uint32_t at_idesc<__half>(int n, bool b_mn) {
+    return (1u << 4) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
+template <> __device__ __forceinline__ constexpr uint32_t at_idesc<__nv_bfloat16>(int n, bool b_mn) {
+    return at_idesc<__half>(n, b_mn) | (1u << 7) | (1u << 10);
+}
+// MN-major, 128-byte swizzle: 64 values of N are a row of 128 bytes, 8 keys a 1024-byte atom; 1024 bytes
+// from 8 keys to the next 8, a slot from 64 values to the next 64.  A K step of 16 keys is 2048 bytes.
+__device__ __forceinline__ uint64_t at_desc_v(uint32_t smem_addr) {
+    return (uint64_t)((smem_addr & 0x3FFFFu) >> 4) | ((uint64_t)(AT_SLOT >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) |
+           (2ull << 61);
+}
+__device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
+
+// place q of the 2 n tiles of K and V in the order the products take them
+struct AtTurn { bool v; int j; };
+__device__ __forceinline__ AtTurn at_turn(int q, int n, bool pair) {
+    if (pair) return AtTurn{(q & 1) != 0, q >> 1};
+    if (q == 0) return AtTurn{false, 0};
+    if (q == 2 * n - 1) return AtTurn{true, n - 1};
+    return q & 1 ? AtTurn{false, (q + 1) >> 1} : AtTurn{true, (q >> 1) - 1};
+}
+
+template <int D, class T>
+__global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(AttendCall a) {
+    extern __shared__ __align__(1024) uint8_t sm[];
+    AtHead& H = *(AtHead*)sm;
+    constexpr int NT = At<D>::tiles, TR = At<D>::rows, CH = At<D>::chunks;
+    uint8_t* q_sm = sm + AT_HEAD;
+    uint8_t* ring = q_sm + NT * At<D>::q_tile;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const Share share = find_share<AT_KEYS, TR, AT_THREADS>(a, 1, (int64_t*)(sm + At<D>::fixed));
+    if (share.lo >= share.hi) return;
+    if (tid == 0) {
+        for (int i = 0; i < AT_SLOTS; i++) { pf_bar_init(&H.full[i], 33); pf_bar_init(&H.empty[i], 1); }
+        for (int i = 0; i < 2; i++) {
+            pf_bar_init(&H.q_full[i], 4);
+            pf_bar_init(&H.pv_done[i], 1);
+        }
+        for (int i = 0; i < 4; i++) { pf_bar_init(&H.s_full[i], 1); pf_bar_init(&H.p_full[i], 4); }
+        pf_bar_init(&H.drained, 1);
+        H.abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == AT_MMA_WARP) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(pf_smem(&H.tmem)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    pf_fence_before();
+    __syncthreads();
+    pf_fence_after();
+    const uint32_t tmem = H.tmem;
+    auto give_up = [&](int site) {
+        if (lane == 0) {
+            atomicExch(a.status, site);
+            *(volatile int*)&H.abort = 1;
+        }
+    };
+    Walk<AT_KEYS, TR> walk(a, share);
+
+    if (warp > AT_MMA_WARP) {
+        // ---- copies
+        uint32_t base = 0, ktile = 0;             // slots, K tiles of the pieces before
+        bool ok = true;
+        for (Piece x; ok && walk.next(x);) {
+            const int n = max(x.n, 0);
+            const bool pair = NT == 2 && x.rows > 128;
+            const int32_t* table = a.table + (int64_t)x.b * a.table_stride;
+            const int p_top = x.r.past + (int)a.group.div(x.row0 + x.rows - 1);
+            const int total = 2 * n * CH;
+            // this warp's slots: every third of the block's
+            for (int i = (int)((3 - base % 3 + (warp - AT_MMA_WARP - 1)) % 3); i < total; i += AT_COPY_WARPS) {
+                const uint32_t gs = base + i, slot = gs % AT_SLOTS;
+                const AtTurn turn = at_turn(i / CH, n, pair);
+                const int c = i % CH, key0 = x.tiles.tile(x.i0 + turn.j) * AT_KEYS;
+                const Pool& pool = turn.v ? a.v : a.k;
+                const uint8_t* from = pool.data + x.head * pool.head + c * 128;
+                int64_t off[4];
+                uint32_t there[4], known[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int j = key0 + 32 * e + lane;
+                    int at = 0;
+                    const int page = j <= p_top ? page_of(a, table, j, at) : -1;
+                    off[e] = page >= 0 ? page * pool.page + at * pool.token : 0;
+                    there[e] = __ballot_sync(0xffffffffu, page >= 0);
+                    known[e] = __ballot_sync(0xffffffffu, page >= 0 || j > p_top);   // what no row sees need not be masked again
+                }
+                if (!bounded_wait_together<256>(PfWait<true, true>{&H.empty[slot], ((gs / AT_SLOTS) & 1) ^ 1, &H.abort})) {
+                    give_up(AT_SITE_COPY);
+                    ok = false;
+                    break;
+                }
+                const uint32_t dst = pf_smem(ring + slot * AT_SLOT) + ((lane & 7) << 4);
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+#pragma unroll
+                    for (int s = 0; s < 8; s++) {
+                        // lanes 8 g to 8 g + 7: the eight pieces of row r
+                        const int r = 32 * e + 4 * s + (lane >> 3);
+                        const int64_t o = __shfl_sync(0xffffffffu, off[e], 4 * s + (lane >> 3));
+                        at_cp16((dst + r * 128) ^ ((r & 7) << 4), from + o + ((lane & 7) << 4), there[e] >> (4 * s + (lane >> 3)) & 1);
+                    }
+                at_cp_arrive(&H.full[slot]);
+                if (!turn.v && c == 0 && lane < 4) H.there[(ktile + turn.j) & 7][lane] = lane == 0 ? known[0] : lane == 1 ? known[1] : lane == 2 ? known[2] : known[3];
+                __syncwarp();
+                if (lane == 0) pf_bar_arrive(&H.full[slot]);
+            }
+            base += total;
+            ktile += n;
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");   // nothing is in flight when the block ends
+    } else if (warp == AT_MMA_WARP) {
+        // ---- products
+        uint32_t base = 0, pieces[2] = {0, 0};    // slots, Q tiles of the pieces before
+        uint32_t used[3] = {0, 0, 0};             // S: of each tile of the pairs; the two of single tiles
+        const uint32_t o_at = tmem, s_at = tmem + 256;
+        bool ok = true;
+        for (Piece x; ok && walk.next(x);) {
+            const int n = max(x.n, 0);
+            if (!n) continue;
+            const bool pair = NT == 2 && x.rows > 128;
+            if (pf_elect()) {
+                uint32_t cp[4] = {used[0], used[0], used[1], used[2]};
+                auto wait = [&](uint64_t* bar, uint32_t parity) { return ok = ok && at_wait(bar, parity, &H.abort); };
+                auto slot_of = [&](int q, int c) { return (base + q * CH + c) % AT_SLOTS; };
+                auto landed = [&](int q, int c) {
+                    const uint32_t gs = base + q * CH + c;
+                    wait(&H.full[gs % AT_SLOTS], (gs / AT_SLOTS) & 1);
+                    at_fence_async();
+                };
+                auto free = [&](int q) {
+                    for (int c = 0; c < CH; c++) pf_commit(&H.empty[slot_of(q, c)]);
+                };
+                // `s`: the S by its barriers (AtHead); the odd ones stand 128 columns on
+                auto scores = [&](int q, int t, int s) {          // S_s = Q_t K^T
+#pragma unroll
+                    for (int c = 0; c < CH; c++) {
+                        const uint32_t qa = pf_smem(q_sm + t * At<D>::q_tile + c * (128 * 128)), ka = pf_smem(ring + slot_of(q, c) * AT_SLOT);
+#pragma unroll
+                        for (int k = 0; k < 4; k++)
+                            pf_mma_bf16(s_at + (s & 1) * 128, pf_desc_sw128(qa + 32 * k), pf_desc_sw128(ka + 32 * k), at_idesc<T>(AT_KEYS, false),
+                                        c || k);
+                    }
+                    pf_commit(&H.s_full[s]);
+                };
+                auto values = [&](int q, int t, int s, bool first) {   // O_t += P_s V
+                    const uint32_t va = pf_smem(ring + slot_of(q, 0) * AT_SLOT);
+#pragma unroll
+                    for (int k = 0; k < AT_KEYS / 16; k++)
+                        at_mma_ts(o_at + t * D, s_at + (s & 1) * 128 + 8 * k, at_desc_v(va + 2048 * k), at_idesc<T>(D, true), !first || k);
+                    pf_commit(&H.pv_done[t]);
+                };
+                auto powers = [&](int s) {
+                    wait(&H.p_full[s], cp[s]++ & 1);
+                    pf_fence_after();
+                };
+                wait(&H.q_full[0], pieces[0] & 1);
+                if (pair) wait(&H.q_full[1], pieces[1] & 1);
+                at_fence_async();
+                if (pair) {
+                    for (int c = 0; c < CH; c++) landed(0, c);
+                    if (ok) { scores(0, 0, 0); scores(0, 1, 1); free(0); }
+                    for (int j = 0; j < n && ok; j++) {
+                        const bool more = j + 1 < n;
+                        for (int t = 0; t < 2 && ok; t++) {
+                            powers(t);
+                            if (t == 0) for (int c = 0; c < CH; c++) landed(2 * j + 1, c);
+                            if (!ok) break;
+                            values(2 * j + 1, t, t, j == 0);
+                            if (t == 1) free(2 * j + 1);
+                            if (more) {
+                                if (t == 0) for (int c = 0; c < CH; c++) landed(2 * j + 2, c);
+                                if (!ok) break;
+                                scores(2 * j + 2, t, t);
+                                if (t == 1) free(2 * j + 2);
+                            }
+                        }
+                    }
+                } else {
+                    for (int c = 0; c < CH; c++) landed(0, c);
+                    if (ok) { scores(0, 0, 2); free(0); }
+                    for (int j = 0; j < n && ok; j++) {
+                        const int kq = 2 * j + 1, vq = j + 1 < n ? 2 * j + 2 : 2 * n - 1;
+                        if (j + 1 < n) {
+                            for (int c = 0; c < CH; c++) landed(kq, c);
+                            if (!ok) break;
+                            scores(kq, 0, 2 + ((j + 1) & 1));
+                            free(kq);
+                        }
+                        powers(2 + (j & 1));
+                        for (int c = 0; c < CH; c++) landed(vq, c);
+                        if (!ok) break;
+                        values(vq, 0, 2 + (j & 1), j == 0);
+                        free(vq);
+                    }
+                }
+                if (!ok) {
+                    atomicExch(a.status, AT_SITE_MMA);
+                    *(volatile int*)&H.abort = 1;
+                }
+            }
+            __syncwarp();
+            base += 2 * n * CH;
+            pieces[0]++;
+            pieces[1] += pair;
+            if (pair) used[0] += n;
+            else { used[1] += (n + 1) / 2; used[2] += n / 2; }
+            ok = pf_together(!*(volatile int*)&H.abort);
+        }
+        // nothing is in flight when the block ends, whatever ended its loops
+        if (pf_elect()) pf_commit(&H.drained);
+        __syncwarp();
+        pf_bar_wait(&H.drained, 0);
+        __syncwarp();
+    } else {
+        // ---- rows
+        const int wg = warp >> 2, row = (warp & 3) * 32 + lane;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        uint32_t cs[3] = {0, 0, 0}, cpv = 0, ktile = 0;   // S of the pairs' tile, the two of single tiles
+        const float scale = fmaxf(fabsf(a.scale_log2), 1e-30f);       // a masked score times it is no NaN
+        const uint32_t flip = a.scale_log2 < 0 ? 0x80008000u : 0u;    // a negative scale: of the rows
+        bool ok = true;
+        for (Piece x; ok && walk.next(x);) {
+            const int n = max(x.n, 0);
+            const bool pair = NT == 2 && x.rows > 128;
+            const int t = pair ? wg : 0;
+            if (wg && !pair) {                        // the other group's piece alone
+                ktile += n;
+                continue;
+            }
+            const int R = x.row0 + t * 128 + row, last = x.row0 + x.rows - 1;
+            const bool mine = R <= last, any = x.row0 + t * 128 + (warp & 3) * 32 <= last;
+            const int Rc = min(R, last), tok = (int)a.group.div(Rc), h = x.head * (int)a.group.d + Rc - tok * (int)a.group.d;
+            const int p = x.r.past + tok;
+            const int p_first = x.r.past + (int)a.group.div(min(x.row0 + t * 128, last)),
+                      p_top = x.r.past + (int)a.group.div(min(x.row0 + t * 128 + 127, last));
+            float m = -INFINITY, l = 0.0f;
+            if (n) {
+                // Q: the warp's own 32 rows, eight pieces in flight; past the tile's, zeros
+                const uint32_t qs = pf_smem(q_sm + t * At<D>::q_tile);
+                constexpr int PR = D / 8, RPI = 32 / PR;              // pieces of a row, rows at once
+#pragma unroll
+                for (int r0 = 0; r0 < 32; r0 += 8 * RPI) {
+                    uint4 w[8];
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const int r = (warp & 3) * 32 + r0 + e * RPI + lane / PR, Q = x.row0 + t * 128 + r, qt = (int)a.group.div(Q);
+                        w[e] = make_uint4(0, 0, 0, 0);
+                        if (Q <= last)
+                            w[e] = *(const uint4*)(a.q + (int64_t)(x.r.begin + qt) * a.q_token +
+                                                   (int64_t)(x.head * (int)a.group.d + Q - qt * (int)a.group.d) * a.q_head + (lane % PR) * 16);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const int r = (warp & 3) * 32 + r0 + e * RPI + lane / PR, c = lane % PR;
+                        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(qs + (c >> 3) * (128 * 128) + r * 128 + (((c ^ r) & 7) << 4)),
+                                     "r"(w[e].x ^ flip), "r"(w[e].y ^ flip), "r"(w[e].z ^ flip), "r"(w[e].w ^ flip) : "memory");
+                    }
+                }
+                at_fence_async();
+                __syncwarp();
+                if (lane == 0) pf_bar_arrive(&H.q_full[t]);
+            }
+            for (int j = 0; j < n; j++) {
+                const int s = pair ? t : 2 + (j & 1);
+                uint32_t& count = pair ? cs[0] : j & 1 ? cs[2] : cs[1];
+                if (!at_wait_warp(&H.s_full[s], count & 1, &H.abort)) { ok = false; break; }
+                count++;
+                if (any) {
+                    pf_fence_after();
+                    const uint32_t s_at = tmem + 256 + (s & 1) * 128 + lanes;
+                    int v[128];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) pf_tmem_ld32(s_at + 32 * e, *(int(*)[32])(v + 32 * e));
+                    pf_tmem_wait_ld();
+                    const int key0 = x.tiles.tile(x.i0 + j) * AT_KEYS;
+                    const uint4 there = *(const uint4*)H.there[(ktile + j) & 7];
+                    const bool all = (there.x & there.y & there.z & there.w) == 0xffffffffu && key0 + AT_KEYS - 1 <= p_first &&
+                                     (a.window <= 0 || p_top - key0 < a.window || key0 + AT_KEYS <= a.sinks);
+                    if (!all) {
+                        const uint32_t tw[4] = {there.x, there.y, there.z, there.w};
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const int k0 = key0 + 32 * e;
+                            uint32_t see = bits_below(p + 1 - k0) & tw[e];
+                            if (a.window > 0) see &= ~bits_below(p - a.window + 1 - k0) | bits_below(a.sinks - k0);
+#pragma unroll
+                            for (int i = 0; i < 32; i++) v[32 * e + i] = see >> i & 1 ? v[32 * e + i] : (int)0xff800000u;   // -infinity
+                        }
+                    }
+                    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int i = 0; i < 128; i++) top[i & 3] = fmaxf(top[i & 3], __int_as_float(v[i]));
+                    const float grown = fmaxf(fmaxf(m, fmaxf(top[0], top[1])), fmaxf(top[2], top[3]));
+                    if (j == 0) m = grown;
+                    const bool far = (grown - m) * scale > AT_GROWTH;
+                    if (__any_sync(0xffffffffu, far)) {
+                        // O follows, once the product before has been added
+                        if (!at_wait_warp(&H.pv_done[t], (cpv + j - 1) & 1, &H.abort)) { ok = false; break; }
+                        pf_fence_after();
+                        const float by = far ? (m == -INFINITY ? 0.0f : exp2_of((m - grown) * scale)) : 1.0f;
+                        if (far) m = grown;
+                        l *= by;
+                        const uint32_t o_at = tmem + t * D + lanes;
+#pragma unroll 1
+                        for (int c = 0; c < D; c += 32) {
+                            int o[32];
+                            pf_tmem_ld32(o_at + c, o);
+                            pf_tmem_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 32; i++) o[i] = __float_as_int(__int_as_float(o[i]) * by);
+                            at_tmem_st32(o_at + c, (const uint32_t*)o);
+                        }
+                        at_tmem_wait_st();
+                    }
+                    const float minus = m == -INFINITY ? 0.0f : -m * scale;
+                    const f32x2 sc = pk(scale, scale), mi = pk(minus, minus);
+                    f32x2 sum[2] = {0, 0};
+                    uint32_t w[32];
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+#pragma unroll
+                        for (int i = 0; i < 32; i++) {
+                            const f32x2 z = fma2(pk(__int_as_float(v[64 * e + 2 * i]), __int_as_float(v[64 * e + 2 * i + 1])), sc, mi);
+                            const float y0 = exp2_of(lo_of(z)), y1 = exp2_of(hi_of(z));
+                            sum[i & 1] = add2(sum[i & 1], pk(y0, y1));
+                            // the weights rounded to the cache's type for the second product (relative error
+                            // 2^-9 or 2^-12 each); l sums them unrounded
+                            w[i] = pack2<T>(y0, y1);
+                        }
+                        at_tmem_st32(s_at + 32 * e, w);
+                    }
+                    sum[0] = add2(sum[0], sum[1]);
+                    l += lo_of(sum[0]) + hi_of(sum[0]);
+                    at_tmem_wait_st();
+                }
+                pf_fence_before();
+                __syncwarp();
+                if (lane == 0) pf_bar_arrive(&H.p_full[s]);
+            }
+            if (!ok) { give_up(AT_SITE_ROWS); break; }
+            ktile += n;
+            if (n) {
+                if (!at_wait_warp(&H.pv_done[t], (cpv + n - 1) & 1, &H.abort)) { give_up(AT_SITE_ROWS); ok = false; break; }
+                cpv += n;
+                pf_fence_after();
+            }
+            if (!any) continue;
+            // ---- O out, 32 values of a row at a time
+            const bool cut = x.parts > 1;
+            const float by = cut ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+            uint8_t* out = a.out + (int64_t)(x.r.begin + tok) * a.out_token + (int64_t)h * a.out_head;
+            const int64_t place = (int64_t)x.slot(x.part) * TR + t * 128 + row;
+            float* part = a.part_o + place * D;
+            float odd = l * 0.0f;                     // NaN as soon as something is not finite
+#pragma unroll 1
+            for (int c = 0; c < D; c += 32) {
+                int o[32];
+                if (n) {
+                    pf_tmem_ld32(tmem + t * D + lanes + c, o);
+                    pf_tmem_wait_ld();
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; i++) o[i] = 0;
+                }
+                float y[32];
+#pragma unroll
+                for (int i = 0; i < 32; i++) {
+                    y[i] = __int_as_float(o[i]) * by;
+                    odd = fmaf(__int_as_float(o[i]), 0.0f, odd);
+                }
+                if (mine && cut) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4) __stcg((float4*)(part + c + i), make_float4(y[i], y[i + 1], y[i + 2], y[i + 3]));
+                } else if (mine) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 8)
+                        *(uint4*)(out + (c + i) * 2) = make_uint4(pack2<T>(y[i], y[i + 1]), pack2<T>(y[i + 2], y[i + 3]),
+                                                                  pack2<T>(y[i + 4], y[i + 5]), pack2<T>(y[i + 6], y[i + 7]));
+                }
+                __syncwarp();
+            }
+            if (cut && mine) __stcg(a.part_ml + place, make_float2(m * scale, l));
+            for (uint32_t bad = __ballot_sync(0xffffffffu, mine && odd != 0.0f); bad; bad &= bad - 1) {
+                __syncwarp();
+                const int of = __ffs(bad) - 1, r = t * 128 + (warp & 3) * 32 + of;
+                float o[D / 32], cm, cl;
+                careful_row<D, T>(a, x, r, AT_KEYS, o, cm, cl);
+                const int64_t out_of = __shfl_sync(0xffffffffu, (int64_t)(out - a.out), of);
+                const int64_t at = (int64_t)x.slot(x.part) * TR + r;
+                const float inv = cl == 0.0f ? 0.0f : 1.0f / cl;
+                for (int e = 0; e < D / 32; e++) {
+                    if (cut) __stcg(a.part_o + at * D + lane + 32 * e, o[e]);
+                    else ((T*)(a.out + out_of))[lane + 32 * e] = from_f32<T>(o[e] * inv);
+                }
+                if (cut && lane == 0) __stcg(a.part_ml + at, make_float2(cm, cl));
+            }
+            if (!cut) continue;
+            // the warp that is last with these 32 rows joins their pieces, in the pieces' order
+            __threadfence();
+            __syncwarp();
+            int last_one = 0;
+            int32_t* arrived = a.arrived + x.c0 * 8 + t * 4 + (warp & 3);
+            if (lane == 0) {
+                last_one = atomicAdd(arrived, 1) == x.parts - 1;
+                if (last_one) *arrived = 0;
+            }
+            if (!__shfl_sync(0xffffffffu, last_one, 0)) continue;
+            __threadfence();
+            const int r0 = t * 128 + (warp & 3) * 32;
+            float M = -INFINITY, L = 0.0f;            // of the row of this lane
+            for (int i = 0; i < x.parts; i++) M = fmaxf(M, __ldcg(a.part_ml + (int64_t)x.slot(i) * TR + r0 + lane).x);
+            auto weight = [](float2 ml, float top) {  // a NaN piece has a sum that is one, whatever its maximum
+                return ml.x == -INFINITY ? (ml.y == 0.0f ? 0.0f : 1.0f) : exp2_of(ml.x - top);
+            };
+            for (int i = 0; i < x.parts; i++) {
+                const float2 ml = __ldcg(a.part_ml + (int64_t)x.slot(i) * TR + r0 + lane);
+                L += ml.y * weight(ml, M);
+            }
+            const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+            constexpr int V = D / 32;                 // values a lane, neighbours
+            const int rows = min(32, x.rows - r0);
+#pragma unroll 4
+            for (int r = 0; r < rows; r++) {
+                const float top = __shfl_sync(0xffffffffu, M, r), f = __shfl_sync(0xffffffffu, inv, r);
+                const int64_t out_of = __shfl_sync(0xffffffffu, (int64_t)(out - a.out), r);
+                float y[V] = {};
+                for (int i = 0; i < x.parts; i++) {
+                    const int64_t at = (int64_t)x.slot(i) * TR + r0 + r;
+                    const float2 ml = __ldcg(a.part_ml + at);
+                    float z[V];
+                    const float* from = a.part_o + at * D + lane * V;
+                    if constexpr (V == 2) { const float2 u = __ldcg((const float2*)from); z[0] = u.x; z[1] = u.y; }
+                    else
+#pragma unroll
+                        for (int e = 0; e < V; e += 4) {
+                            const float4 u = __ldcg((const float4*)(from + e));
+                            z[e] = u.x; z[e + 1] = u.y; z[e + 2] = u.z; z[e + 3] = u.w;
+                        }
+                    const float w = weight(ml, top);
+#pragma unroll
+                    for (int e = 0; e < V; e++)
+                        if (w != 0.0f) y[e] += z[e] * w;
+                }
+                uint32_t* to = (uint32_t*)(a.out + out_of) + lane * (V / 2);
+#pragma unroll
+                for (int e = 0; e < V; e += 2) to[e / 2] = pack2<T>(y[e] * f, y[e + 1] * f);
+            }
+        }
+    }
+    pf_fence_before();
+    __syncthreads();
+    pf_fence_after();
+    if (warp == AT_MMA_WARP) {
+        __syncwarp();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+}
+
+template <int D, class T> static cudaError_t tc(const AttendCall& a, int sm_count, cudaStream_t stream) {
+    static_assert(At<D>::fixed + share_smem(kCacheSeqs, AT_THREADS) <= 227 * 1024, "the block must fit in shared memory");
+    static std::atomic<uint64_t> attr_set{0};
+    if (cudaError_t e = ensure_dynamic_smem(attend_tc_kernel<D, T>, (int)(At<D>::fixed + share_smem(kCacheSeqs, AT_THREADS)), attr_set)) return e;
+    count_launch();
+    return launch_with(false, stream, attend_tc_kernel<D, T>, dim3(sm_count), dim3(AT_THREADS),
+                       (size_t)At<D>::fixed + share_smem(a.n_seq, AT_THREADS), a);
+}
+cudaError_t launch_attend_tc(const AttendCall& a, int head_dim, int ggml_type, int sm_count, cudaStream_t stream) {
+    const bool f16 = ggml_type == BIVMOE_F16;
+    switch (head_dim) {
+        case 64: return f16 ? tc<64, __half>(a, sm_count, stream) : tc<64, __nv_bfloat16>(a, sm_count, stream);
+        case 128: return f16 ? tc<128, __half>(a, sm_count, stream) : tc<128, __nv_bfloat16>(a, sm_count, stream);
+        default: return f16 ? tc<256, __half>(a, sm_count, stream) : tc<256, __nv_bfloat16>(a, sm_count, stream);
+    }
+}
+
+}  // namespace bivmoe

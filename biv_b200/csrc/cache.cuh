@@ -1,6 +1,6 @@
 // The paged key/value cache: what its kernels share.  Arguments as the kernels take them, the
-// addresses of keys in the pages, which keys a row sees, how a batch of requests is cut into items of
-// work on the device, and the careful row.
+// addresses of keys in the pages, which keys a row sees, how the work of a batch is shared out on the
+// device, and the careful row.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -56,11 +56,10 @@ struct AttendCall {
     FastDiv page, group;             // group: query heads to a kv head
     int heads_kv, window, sinks;
     float scale_log2;                // scale * log2(e): the softmax is taken in powers of two
-    float* part_o;                   // [parts][rows][head_dim], not yet divided by the sum
-    float2* part_ml;                 // [parts][rows]: running maximum and sum
-    int32_t* arrived;                // [parts]: how many parts of a tile are there; zero between calls
+    float* part_o;                   // [2 blocks][rows][head_dim], not yet divided by the sum
+    float2* part_ml;                 // [2 blocks][rows]: running maximum and sum
+    int32_t* arrived;                // [blocks][..]: how many pieces of a tile are there; zero between calls
     int32_t* status;
-    int parts, target;               // room for parts; into how many equal pieces the work is cut at most
 };
 
 // ---- requests ------------------------------------------------------------------------------------
@@ -99,16 +98,6 @@ template <int KT> __device__ __forceinline__ TileList tiles_of(const AttendCall&
     t.n = t.ns + last - t.from + 1;
     return t;
 }
-// an upper bound of tiles_of().n over the row tiles of a request
-template <int KT> __device__ __forceinline__ int most_tiles(const AttendCall& a, const Request& r, int tile_rows) {
-    const int tokens = (int)a.group.div(r.rows), p1 = r.past + tokens - 1;
-    if (p1 < 0) return 0;
-    const int all = p1 / KT + 1;
-    if (a.window <= 0) return all;
-    const int span = min(tokens, tile_rows / (int)a.group.d + 2);
-    const int64_t some = (int64_t)(min(a.sinks, p1 + 1) + KT - 1) / KT + ((int64_t)a.window + span) / KT + 2;
-    return some < all ? (int)some : all;
-}
 __device__ __forceinline__ bool sees(const AttendCall& a, int p, int j) {
     return j <= p && (a.window <= 0 || p - j < a.window || j < a.sinks);
 }
@@ -121,111 +110,175 @@ __device__ __forceinline__ int page_of(const AttendCall& a, const int32_t* row, 
     return page >= 0 && page < a.k.n_pages ? page : -1;
 }
 
-// ---- items of work -------------------------------------------------------------------------------
-// An item is a tile of TR rows of a request's kv head (row r: token r / group, query head r % group:
-// the heads that share keys share the tile) against at most `len` of the key tiles that the tile sees.
-// `len` is the same in the whole call: the work in key tiles, W, over `target` pieces, so that the
-// parts that have to be joined number at most 2 W / len <= 2 target whatever the lengths are.  Every
-// block finds the items by itself from the lengths: it needs no list in memory and no launch before.
-struct Items {
-    int len, total;
-    const int* first_item;           // shared, [n_seq + 1]
-    const int* first_part;           // shared, [n_seq + 1]; requests whose tiles are cut only
+// ---- shares of the work ----------------------------------------------------------------------------
+// A tile is TR rows of a request's kv head (row r: token r / group, query head r % group: the heads that
+// share keys share the tile); its work is the key tiles it sees, one unit each (a tile that sees none:
+// one, for its zeros).  The units of all tiles stand in one line, requests, kv heads, tiles, key tiles
+// in this order, and each of `g` blocks takes an equal share of the line, wherever that cuts a tile:
+// the blocks end together whatever the lengths are, and a block has at most two pieces of tiles
+// that others share, so that the room for pieces is two to a block.  Every block finds its share by
+// itself from the lengths: no list in memory, no launch before.
+struct Share {
+    int64_t total, lo, hi;           // units of the call, of this block
+    int g;
+    const int64_t* before;           // shared, [n_seq + 1]: units of the requests before
+    // the block that has unit u: the last c with total * c / g <= u
+    __device__ __forceinline__ int owner(int64_t u) const { return (int)(((u + 1) * g - 1) / total); }
 };
+template <int KT, int TR> __device__ __forceinline__ TileList tile_list(const AttendCall& a, const Request& r, int t) {
+    return tiles_of<KT>(a, r.past + (int)a.group.div(t * TR), r.past + (int)a.group.div(min((t + 1) * TR, r.rows) - 1));
+}
+template <int KT, int TR> __device__ __forceinline__ int tile_units(const AttendCall& a, const Request& r, int t) {
+    return max(tile_list<KT, TR>(a, r, t).n, 1);
+}
+constexpr size_t share_smem(int n_seq, int threads) { return (((size_t)n_seq + 1 + threads / 32) * 8 + 15) / 16 * 16; }
+constexpr int kAlone = 4;            // tiles of a request that one thread counts
+// least: units that are worth a block
 template <int KT, int TR, int THREADS>
-__device__ __forceinline__ Items find_items(const AttendCall& a, int least, int* sh /* 2 (n_seq + 1) + THREADS / 16 + 4 */) {
+__device__ __forceinline__ Share find_share(const AttendCall& a, int least, int64_t* sh /* share_smem */) {
     constexpr int WARPS = THREADS / 32;
-    int* first_item = sh;
-    int* first_part = sh + a.n_seq + 1;
-    int* warps = sh + 2 * (a.n_seq + 1);
-    float* works = (float*)(warps + 2 * WARPS);
+    int64_t* before = sh;
+    int64_t* sums = sh + a.n_seq + 1;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int each = (a.n_seq + THREADS - 1) / THREADS, b0 = tid * each, b1 = min(b0 + each, a.n_seq);
-    // W as a float: it is only what `len` is chosen by, and every block sums it in the same order
-    float w = 0.0f;
-    for (int b = b0; b < b1; b++) {
-        const Request r = request_of(a, b);
-        const int nt = (r.rows + TR - 1) / TR, c = nt ? most_tiles<KT>(a, r, TR) : 0;
-        first_item[b] = nt;
-        first_part[b] = c;
-        w += (float)nt * (float)c;
+    int64_t carry = 0;
+    for (int b0 = 0; b0 < a.n_seq; b0 += THREADS) {
+        const int b = b0 + tid;
+        Request r{0, 0, 0};
+        if (b < a.n_seq) r = request_of(a, b);
+        const int nt = (r.rows + TR - 1) / TR;
+        int64_t units = 0;
+        if (nt <= kAlone)
+            for (int t = 0; t < nt; t++) units += tile_units<KT, TR>(a, r, t);
+        for (uint32_t many = __ballot_sync(0xffffffffu, nt > kAlone); many; many &= many - 1) {
+            const int of = __ffs(many) - 1;   // a long one: counted by the warp
+            const Request q{__shfl_sync(0xffffffffu, r.begin, of), __shfl_sync(0xffffffffu, r.rows, of), __shfl_sync(0xffffffffu, r.past, of)};
+            int64_t some = 0;
+            for (int t = lane; t < (q.rows + TR - 1) / TR; t += 32) some += tile_units<KT, TR>(a, q, t);
+            for (int d = 16; d; d >>= 1) some += __shfl_xor_sync(0xffffffffu, some, d);
+            if (lane == of) units = some;
+        }
+        units *= a.heads_kv;
+        int64_t x = units;
+        for (int d = 1; d < 32; d <<= 1) {
+            const int64_t y = __shfl_up_sync(0xffffffffu, x, d);
+            if (lane >= d) x += y;
+        }
+        __syncthreads();
+        if (lane == 31) sums[warp] = x;
+        __syncthreads();
+        int64_t base = carry;
+        for (int i = 0; i < WARPS; i++) {
+            if (i < warp) base += sums[i];
+            carry += sums[i];
+        }
+        if (b < a.n_seq) before[b] = base + x - units;
     }
-    for (int d = 16; d; d >>= 1) w += __shfl_xor_sync(0xffffffffu, w, d);
-    if (lane == 0) works[warp] = w;
+    if (tid == 0) before[a.n_seq] = carry;
     __syncthreads();
-    w = 0.0f;
-    for (int i = 0; i < WARPS; i++) w += works[i];
-    Items it;
-    // one more than the quotient: the float's rounding may not make more pieces than there is room for
-    it.len = max(least, (int)fminf(w * (float)a.heads_kv / (float)a.target * 1.0001f, 1e9f) + 1);
-    int items = 0, parts = 0;
-    for (int b = b0; b < b1; b++) {
-        const int nt = first_item[b], s = (first_part[b] + it.len - 1) / it.len;
-        first_item[b] = items;
-        first_part[b] = parts;
-        items += nt * a.heads_kv * max(s, 1);
-        if (s > 1) parts += nt * a.heads_kv * s;
+    Share s;
+    s.total = carry;
+    s.before = before;
+    const int64_t worth = (carry + least - 1) / least;
+    s.g = (int)(worth < gridDim.x ? worth : gridDim.x);
+    s.lo = s.hi = 0;
+    if ((int)blockIdx.x < s.g) {
+        s.lo = carry * blockIdx.x / s.g;
+        s.hi = carry * (blockIdx.x + 1) / s.g;
     }
-    int xi = items, xp = parts;
-    for (int d = 1; d < 32; d <<= 1) {
-        const int yi = __shfl_up_sync(0xffffffffu, xi, d), yp = __shfl_up_sync(0xffffffffu, xp, d);
-        if (lane >= d) { xi += yi; xp += yp; }
-    }
-    if (lane == 31) { warps[2 * warp] = xi; warps[2 * warp + 1] = xp; }
-    __syncthreads();
-    int bi = xi - items, bp = xp - parts;
-    it.total = 0;
-    for (int i = 0; i < WARPS; i++) {
-        if (i < warp) { bi += warps[2 * i]; bp += warps[2 * i + 1]; }
-        it.total += warps[2 * i];
-    }
-    for (int b = b0; b < b1; b++) { first_item[b] += bi; first_part[b] += bp; }
-    if (tid == 0) first_item[a.n_seq] = it.total;
-    it.first_item = first_item;
-    it.first_part = first_part;
-    __syncthreads();
-    return it;
+    return s;
 }
-constexpr size_t items_smem(int n_seq, int threads) {
-    return ((2 * ((size_t)n_seq + 1) + 3 * (threads / 32) + 4) * 4 + 15) / 16 * 16;
-}
-struct Item {
+struct Piece {
     int b, head, row0, rows;         // request, kv head, the tile's first row and how many of its rows there are
     Request r;
     TileList tiles;
-    int i0, i1;                      // of the tile list
-    int split, splits, part;         // which piece of how many; the first piece's place among the parts
+    int i0, n;                       // first of the tile list, and how many
+    int part, parts;                 // which piece of how many
+    int c0;                          // the block that has the first one
+    // where a piece's unfinished sums stand: a block is the first of at most one cut tile, and has
+    // at most one piece of a tile that began before it
+    __device__ __forceinline__ int slot(int p) const { return p == 0 ? 2 * c0 + 1 : 2 * (c0 + p); }
 };
-// Long tiles first: within a request the last rows see the most.
-template <int KT, int TR> __device__ __forceinline__ Item item_at(const AttendCall& a, const Items& it, int index) {
-    int lo = 0, hi = a.n_seq;        // the request: the last one that begins at or before the item
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (it.first_item[mid] <= index) lo = mid; else hi = mid;
+// The pieces of a block's share, one after another: every warp goes through them by itself.
+template <int KT, int TR> struct Walk {
+    const AttendCall& a;
+    const Share& s;
+    int64_t at;                      // the next unit
+    int b, head, t, nt, off;         // where it lies
+    Request r;
+    __device__ __forceinline__ Walk(const AttendCall& call, const Share& share) : a(call), s(share), at(share.lo) {
+        if (at >= s.hi) return;
+        int lo = 0, hi = a.n_seq;    // the request: the last one that begins at or before the unit
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (s.before[mid] <= at) lo = mid; else hi = mid;
+        }
+        open(lo);
+        const int64_t rest = at - s.before[b], each = (s.before[b + 1] - s.before[b]) / a.heads_kv;
+        head = (int)(rest / each);
+        int64_t in = rest - head * each;
+        const int lane = threadIdx.x & 31;
+        for (t = 0; nt > 1 && t < nt;) {   // the tile: 32 of them at a time
+            const int mine = t + lane < nt ? tile_units<KT, TR>(a, r, t + lane) : 0;
+            int64_t x = mine;
+            for (int d = 1; d < 32; d <<= 1) {
+                const int64_t y = __shfl_up_sync(0xffffffffu, x, d);
+                if (lane >= d) x += y;
+            }
+            const uint32_t beyond = __ballot_sync(0xffffffffu, x > in);
+            if (beyond) {
+                const int of = __ffs(beyond) - 1;
+                in -= __shfl_sync(0xffffffffu, x - mine, of);
+                t += of;
+                break;
+            }
+            in -= __shfl_sync(0xffffffffu, x, 31);
+            t += 32;
+        }
+        off = (int)in;
     }
-    Item x;
-    x.b = lo;
-    x.r = request_of(a, lo);
-    const int nt = (x.r.rows + TR - 1) / TR;
-    const int most = max((most_tiles<KT>(a, x.r, TR) + it.len - 1) / it.len, 1);
-    int rest = index - it.first_item[lo];
-    x.split = rest % most;
-    rest /= most;
-    x.head = rest % a.heads_kv;
-    const int t = nt - 1 - rest / a.heads_kv;
-    x.row0 = t * TR;
-    x.rows = min(TR, x.r.rows - x.row0);
-    const int p0 = x.r.past + (int)a.group.div(x.row0), p1 = x.r.past + (int)a.group.div(x.row0 + x.rows - 1);
-    x.tiles = tiles_of<KT>(a, p0, p1);
-    x.i0 = x.split * it.len;
-    x.i1 = min(x.i0 + it.len, x.tiles.n);
-    x.splits = (x.tiles.n + it.len - 1) / it.len;
-    x.part = it.first_part[lo] + (t * a.heads_kv + x.head) * most;
-    return x;
-}
-// what a piece beyond the tile's own number of pieces has to do: nothing; the first one of a tile
-// that sees nothing writes its zeros
-__device__ __forceinline__ bool item_void(const Item& x) { return x.split > 0 && x.i0 >= x.i1; }
+    __device__ __forceinline__ void open(int request) {
+        b = request;
+        r = request_of(a, b);
+        nt = (r.rows + TR - 1) / TR;
+    }
+    __device__ __forceinline__ bool next(Piece& x) {
+        if (at >= s.hi) return false;
+        x.b = b;
+        x.head = head;
+        x.r = r;
+        x.row0 = t * TR;
+        x.rows = min(TR, r.rows - x.row0);
+        x.tiles = tile_list<KT, TR>(a, r, t);
+        const int units = max(x.tiles.n, 1), take = (int)min((int64_t)(units - off), s.hi - at);
+        x.i0 = off;
+        x.n = min(off + take, x.tiles.n) - off;
+        x.part = 0;
+        x.parts = 1;
+        x.c0 = (int)blockIdx.x;
+        if (take < units) {
+            x.c0 = s.owner(at - off);
+            x.parts = s.owner(at - off + units - 1) - x.c0 + 1;
+            x.part = (int)blockIdx.x - x.c0;
+        }
+        at += take;
+        off += take;
+        if (off == units) {
+            off = 0;
+            if (++t == nt) {
+                t = 0;
+                if (++head == a.heads_kv) {
+                    head = 0;
+                    if (at < s.hi) {
+                        int next = b + 1;
+                        while (s.before[next + 1] == s.before[next]) next++;   // those without rows
+                        open(next);
+                    }
+                }
+            }
+        }
+        return true;
+    }
+};
 
 // ---- types ---------------------------------------------------------------------------------------
 __device__ __forceinline__ float to_f32(float v) { return v; }
@@ -257,7 +310,7 @@ __device__ __forceinline__ float exp2_of(float x) {
 // from the keys that they see alone; a row that does see such values has its NaN after the first of
 // them.  Lane l holds the values l, l + 32, ... of o.
 template <int D, class T>
-__device__ __noinline__ void careful_row(const AttendCall& a, const Item& x, int row, int kt, float (&o)[D / 32], float& m, float& l) {
+__device__ __noinline__ void careful_row(const AttendCall& a, const Piece& x, int row, int kt, float (&o)[D / 32], float& m, float& l) {
     const int lane = threadIdx.x & 31, R = x.row0 + row;
     const int tok = (int)a.group.div(R), h = x.head * (int)a.group.d + R - tok * (int)a.group.d, p = x.r.past + tok;
     const T* q = (const T*)(a.q + (int64_t)(x.r.begin + tok) * a.q_token + (int64_t)h * a.q_head);
@@ -266,7 +319,7 @@ __device__ __noinline__ void careful_row(const AttendCall& a, const Item& x, int
     for (int i = 0; i < D / 32; i++) { qv[i] = to_f32(q[lane + 32 * i]); o[i] = 0.0f; }
     m = -INFINITY;
     l = 0.0f;
-    for (int i = x.i0; i < x.i1; i++) {
+    for (int i = x.i0; i < x.i0 + x.n; i++) {
         const int j0 = x.tiles.tile(i) * kt;
         for (int j = j0; j < j0 + kt && j <= p; j++) {
             int at;
@@ -291,12 +344,13 @@ __device__ __noinline__ void careful_row(const AttendCall& a, const Item& x, int
     }
 }
 
-size_t attend_few_smem(int head_dim, int n_seq);
 cudaError_t launch_attend_few(const AttendCall& a, int head_dim, int ggml_type, int sm_count, cudaStream_t stream);
+cudaError_t launch_attend_tc(const AttendCall& a, int head_dim, int ggml_type, int sm_count, cudaStream_t stream);
 cudaError_t launch_extend(const bivmoe_extend_args& a, int page_size, int sm_count, cudaStream_t stream);
 cudaError_t launch_store(const bivmoe_store_args& a, const RopePlan& rope, int ggml_type, int heads, int heads_kv, int head_dim,
                          int page_size, int sm_count, cudaStream_t stream);
-// the rows, and the pieces of work, that the workspace is sized for
-constexpr int kFewRows = 16;
+// what the workspace is sized for: rows of a tile, blocks to a multiprocessor
+constexpr int kFewRows = 16, kFewBlocks = 2;
+constexpr int tc_rows(int head_dim) { return head_dim == 256 ? 128 : 256; }
 
 }  // namespace bivmoe

@@ -41,9 +41,6 @@ static int cuda_fail(cudaError_t e, const char* what) {
     return fail(e == cudaErrorMemoryAllocation ? BIVMOE_ERR_OOM : BIVMOE_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
 }
 
-// pieces of work of a call, at most: eight to a multiprocessor
-static int pieces(const bivmoe_cache* c) { return 8 * c->sm_count; }
-
 extern "C" void bivmoe_cache_destroy(bivmoe_cache* c) {
     if (!c) return;
     DeviceScope on_device(c->d.device);
@@ -104,22 +101,24 @@ extern "C" int bivmoe_cache_create(const bivmoe_cache_desc* d, bivmoe_cache** ou
     int cur = -1;
     cudaError_t e = cudaGetDevice(&cur);
     if (e == cudaSuccess && cur != d->device) e = cudaSetDevice(d->device);   // reports an invalid ordinal
-    cudaDeviceProp prop;
-    if (e == cudaSuccess) e = cudaGetDeviceProperties(&prop, d->device);
+    int major = 0, sms = 0;
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, d->device);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, d->device);
     if (e != cudaSuccess) return cuda_fail(e, "bivmoe_cache_create");
-    if (prop.major != 10)
-        return fail(BIVMOE_ERR_UNSUPPORTED, "device %d is sm_%d%d; this library is built for sm_100a only", d->device, prop.major, prop.minor);
+    if (major != 10)
+        return fail(BIVMOE_ERR_UNSUPPORTED, "device %d is of compute capability %d.x; this library is built for sm_100a only", d->device, major);
     bivmoe_cache* c = new (std::nothrow) bivmoe_cache();
     if (!c) return fail(BIVMOE_ERR_OOM, "host allocation failed");
     c->d = *d;
-    c->sm_count = prop.multiProcessorCount;
-    // parts: at most two to a piece of work (cache.cuh)
-    const size_t parts = 2 * (size_t)pieces(c), rows = kFewRows;
+    c->sm_count = sms;
+    // pieces: at most two to a block (cache.cuh)
+    const size_t few = 2 * (size_t)kFewBlocks * c->sm_count * kFewRows, tc = 2 * (size_t)c->sm_count * tc_rows(d->head_dim),
+                 rows = few > tc ? few : tc, counts = 8 * (size_t)c->sm_count;
     size_t off = 0;
     auto take = [&off](size_t bytes) { const size_t at = off; off += (bytes + 255) & ~(size_t)255; return at; };
-    const size_t o = take(parts * rows * d->head_dim * 4), ml = take(parts * rows * sizeof(float2)), tt = take(turns.size() * 8 + 8),
-                 ax = take(axis.size() * 4 + 4), arr = take(parts * 4), st = take(16);
-    c->arrived_bytes = parts * 4;
+    const size_t o = take(rows * d->head_dim * 4), ml = take(rows * sizeof(float2)), tt = take(turns.size() * 8 + 8),
+                 ax = take(axis.size() * 4 + 4), arr = take(counts * 4), st = take(16);
+    c->arrived_bytes = counts * 4;
     e = dev_alloc((void**)&c->mem, off);
     if (e == cudaSuccess) e = cudaMemset(c->mem + arr, 0, off - arr);
     if (e == cudaSuccess && d->n_rot) e = cudaMemcpy(c->mem + tt, turns.data(), turns.size() * 8, cudaMemcpyHostToDevice);
@@ -264,12 +263,16 @@ extern "C" int bivmoe_cache_attend(bivmoe_cache* c, const bivmoe_attend_args* a,
     k.window = a->window; k.sinks = a->sinks;
     k.scale_log2 = a->scale * 1.4426950408889634f;
     k.part_o = c->part_o; k.part_ml = c->part_ml; k.arrived = c->arrived; k.status = c->status;
-    k.parts = 2 * pieces(c);
-    k.target = pieces(c);
     const cudaStream_t s = (cudaStream_t)stream;
     bool captured = false;
     cudaError_t e = take_turn(c, s, &captured);
-    if (e == cudaSuccess) e = launch_attend_few(k, c->d.head_dim, c->d.ggml_type, c->sm_count, s);
+    // tiles of 16 rows where no request has more rows to a kv head; max_new is the caller's word, which
+    // decides the speed alone: both kernels take any number of rows
+    const int most = a->max_new > 0 && a->max_new < a->n_tokens ? a->max_new : a->n_tokens;
+    const bool few = most <= kFewRows / (int)k.group.d;
+    if (e == cudaSuccess)
+        e = few ? launch_attend_few(k, c->d.head_dim, c->d.ggml_type, c->sm_count, s)
+                : launch_attend_tc(k, c->d.head_dim, c->d.ggml_type, c->sm_count, s);
     if (e == cudaSuccess) e = end_turn(c, s, captured);
     return e == cudaSuccess ? BIVMOE_OK : cuda_fail(e, "bivmoe_cache_attend");
 }
