@@ -2,7 +2,7 @@
 //
 //   S = Q K^T (128 rows x 128 keys),  P = 2^(scale S - m),  O += P V,  o = O / sum P
 //
-// One block per SM takes its share of the work (cache.cuh) and has three kinds of warps:
+// One block per SM takes its share of the work (cache.cuh) and has four kinds of warps:
 //
 //   warps 0-7    two groups of 128 threads, a thread to a row: S from tensor memory, its maximum, the
 //                powers, P as 16-bit values back into tensor memory over S; at a piece's start the
@@ -10,7 +10,8 @@
 //   warp 8       one lane issues the MMAs.  K and V stand in shared memory in rows of 64 values
 //                (128-byte swizzle): K is read along the values (K-major), V along the keys (MN-major),
 //                so that neither is turned; P is read from tensor memory.
-//   warps 9-11   copy K and V from the pages, 128 keys x 64 values (16 KB) a slot, in a ring of eight:
+//   warp 9       finds where a tile's keys lie, ahead of the copies.
+//   warps 12-15  copy K and V from the pages, 128 keys x 64 values (16 KB) a slot, in a ring of eight:
 //                cp.async in 16-byte pieces, since a tile's keys lie in pages of any size.
 //
 // Heads of up to 128 values: two tiles of 128 rows at once, a group each, so that one group's powers
@@ -30,17 +31,21 @@
 namespace bivmoe {
 
 constexpr int AT_KEYS = 128, AT_SLOT = AT_KEYS * 128, AT_SLOTS = 8;
-constexpr int AT_THREADS = 384, AT_COPY_WARPS = 3, AT_MMA_WARP = 8;
-constexpr int AT_HEAD = 1024;
+constexpr int AT_THREADS = 512, AT_MMA_WARP = 8, AT_PAGE_WARP = 9, AT_COPY_WARP = 12, AT_COPY_WARPS = 4;
+constexpr int AT_ROW_REGS = 192, AT_OTHER_REGS = 64;
+static_assert(AT_ROW_REGS * 256 + AT_OTHER_REGS * 256 <= 512 * 128, "setmaxnreg would wait for registers that nobody gives");
+constexpr int AT_HEAD = 1024, AT_PAGES = 8;    // key tiles whose addresses stand ready
 constexpr float AT_GROWTH = 8.0f;     // powers of two
-enum { AT_SITE_COPY = 31, AT_SITE_MMA, AT_SITE_ROWS };
+enum { AT_SITE_COPY = 31, AT_SITE_MMA, AT_SITE_ROWS, AT_SITE_PAGES };
 
+// where a tile's keys and values lie, from the head's first page on; -1 where there is none
+struct AtPlaces { int64_t k[AT_KEYS], v[AT_KEYS]; };
 template <int D> struct At {
     static constexpr int tiles = D == 256 ? 1 : 2;           // of 128 rows
     static constexpr int rows = 128 * tiles;
     static constexpr int chunks = D / 64;                    // slots of a tile of K, or of V
     static constexpr int q_tile = 128 * D * 2;
-    static constexpr int fixed = AT_HEAD + tiles * q_tile + AT_SLOTS * AT_SLOT;
+    static constexpr int fixed = AT_HEAD + tiles * q_tile + AT_SLOTS * AT_SLOT + (int)sizeof(AtPlaces) * AT_PAGES;
 };
 
 struct AtHead {
@@ -48,12 +53,18 @@ struct AtHead {
     // [0], [1]: of the two tiles of a pair; [2], [3]: of the two S of a single tile.  Apart, because the
     // second group passes single tiles by: a parity tells a phase from the next one only.
     uint64_t s_full[4], p_full[4], q_full[2], pv_done[2], drained;
-    alignas(16) uint32_t there[8][4];   // read 16 bytes at once: which keys of a K tile lie in pages that there are
+    uint64_t page_full[AT_PAGES], page_empty[AT_PAGES];
+    // Which keys of a tile lie in pages that there are, or are seen by no row; read 16 bytes at once.  The
+    // addresses are at most eight tiles ahead of the copies, these at most five ahead of the rows.
+    alignas(16) uint32_t there[16][4];
     uint32_t tmem;
     int abort;
 };
 static_assert(sizeof(AtHead) <= AT_HEAD && offsetof(AtHead, there) % 16 == 0, "");
 
+// Each role's registers are dealt out in its own branch: where branches meet, the compiler reckons with
+// the fewest.
+__device__ __forceinline__ void at_fewer_regs() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(AT_OTHER_REGS)); }
 __device__ __forceinline__ bool at_wait(uint64_t* bar, uint32_t parity, const int* abort) {
     return bounded_wait<256>(PfWait<false, false>{bar, parity, abort});
 }
@@ -103,6 +114,13 @@ __device__ __forceinline__ uint64_t at_desc_v(uint32_t smem_addr) {
     return (uint64_t)((smem_addr & 0x3FFFFu) >> 4) | ((uint64_t)(AT_SLOT >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) |
            (2ull << 61);
 }
+// 16-byte piece `c` of row `r` of 128 rows in tiles of 64 values, 128-byte swizzle
+__device__ __forceinline__ uint32_t at_piece(uint32_t tile, int r, int c) {
+    return tile + (c >> 3) * (128 * 128) + r * 128 + (((c ^ r) & 7) << 4);
+}
+__device__ __forceinline__ void sts128(uint32_t a, uint4 v) {
+    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
 __device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
 
 // place q of the 2 n tiles of K and V in the order the products take them
@@ -121,16 +139,23 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(AttendCall a) 
     constexpr int NT = At<D>::tiles, TR = At<D>::rows, CH = At<D>::chunks;
     uint8_t* q_sm = sm + AT_HEAD;
     uint8_t* ring = q_sm + NT * At<D>::q_tile;
+    AtPlaces* places = (AtPlaces*)(ring + AT_SLOTS * AT_SLOT);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const Share share = find_share<AT_KEYS, TR, AT_THREADS>(a, 1, (int64_t*)(sm + At<D>::fixed));
-    if (share.lo >= share.hi) return;
+    // the share is looked at once a piece: it stands in shared memory, the rows' registers are full
+    __shared__ Share share;
+    {
+        const Share found = find_share<AT_KEYS, TR, AT_THREADS>(a, 1, (int64_t*)(sm + At<D>::fixed));
+        if (found.lo >= found.hi) return;
+        if (tid == 0) share = found;
+    }
     if (tid == 0) {
-        for (int i = 0; i < AT_SLOTS; i++) { pf_bar_init(&H.full[i], 33); pf_bar_init(&H.empty[i], 1); }
+        for (int i = 0; i < AT_SLOTS; i++) { pf_bar_init(&H.full[i], 32); pf_bar_init(&H.empty[i], 1); }
         for (int i = 0; i < 2; i++) {
             pf_bar_init(&H.q_full[i], 4);
             pf_bar_init(&H.pv_done[i], 1);
         }
         for (int i = 0; i < 4; i++) { pf_bar_init(&H.s_full[i], 1); pf_bar_init(&H.p_full[i], 4); }
+        for (int i = 0; i < AT_PAGES; i++) { pf_bar_init(&H.page_full[i], 1); pf_bar_init(&H.page_empty[i], 2 * CH); }
         pf_bar_init(&H.drained, 1);
         H.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -151,59 +176,79 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(AttendCall a) 
     };
     Walk<AT_KEYS, TR> walk(a, share);
 
-    if (warp > AT_MMA_WARP) {
-        // ---- copies
-        uint32_t base = 0, ktile = 0;             // slots, K tiles of the pieces before
+    if (warp == AT_PAGE_WARP) {
+        at_fewer_regs();
+        // ---- addresses: four keys a lane, once for K and V and all their slots
+        uint32_t ktile = 0;                       // key tiles of the pieces before
         bool ok = true;
         for (Piece x; ok && walk.next(x);) {
-            const int n = max(x.n, 0);
-            const bool pair = NT == 2 && x.rows > 128;
+            const int n = max(x.n, 0), p_top = x.r.past + (int)a.group.div(x.row0 + x.rows - 1);
             const int32_t* table = a.table + (int64_t)x.b * a.table_stride;
-            const int p_top = x.r.past + (int)a.group.div(x.row0 + x.rows - 1);
-            const int total = 2 * n * CH;
-            // this warp's slots: every third of the block's
-            for (int i = (int)((3 - base % 3 + (warp - AT_MMA_WARP - 1)) % 3); i < total; i += AT_COPY_WARPS) {
+            for (int j = 0; j < n; j++, ktile++) {
+                const int e = ktile % AT_PAGES, key0 = x.tiles.tile(x.i0 + j) * AT_KEYS;
+                int page[4], at[4];
+                uint32_t known[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int key = key0 + 32 * i + lane;
+                    page[i] = key <= p_top ? page_of(a, table, key, at[i]) : -1;
+                    known[i] = __ballot_sync(0xffffffffu, page[i] >= 0 || key > p_top);
+                }
+                if (!bounded_wait_together<256>(PfWait<true, true>{&H.page_empty[e], ((ktile / AT_PAGES) & 1) ^ 1, &H.abort})) {
+                    give_up(AT_SITE_PAGES);
+                    ok = false;
+                    break;
+                }
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    places[e].k[32 * i + lane] = page[i] >= 0 ? page[i] * a.k.page + at[i] * a.k.token : -1;
+                    places[e].v[32 * i + lane] = page[i] >= 0 ? page[i] * a.v.page + at[i] * a.v.token : -1;
+                }
+                if (lane == 0) *(uint4*)H.there[ktile & 15] = make_uint4(known[0], known[1], known[2], known[3]);
+                __syncwarp();
+                if (lane == 0) pf_bar_arrive(&H.page_full[e]);
+            }
+        }
+    } else if (warp >= AT_COPY_WARP) {
+        at_fewer_regs();
+        // ---- copies
+        uint32_t base = 0, ktile = 0;             // slots, key tiles of the pieces before
+        bool ok = true;
+        for (Piece x; ok && walk.next(x);) {
+            const int n = max(x.n, 0), total = 2 * n * CH;
+            const bool pair = NT == 2 && x.rows > 128;
+            // this warp's slots: every fourth of the block's
+            for (int i = (int)((warp - AT_COPY_WARP - base) & 3); i < total; i += AT_COPY_WARPS) {
                 const uint32_t gs = base + i, slot = gs % AT_SLOTS;
                 const AtTurn turn = at_turn(i / CH, n, pair);
-                const int c = i % CH, key0 = x.tiles.tile(x.i0 + turn.j) * AT_KEYS;
-                const Pool& pool = turn.v ? a.v : a.k;
-                const uint8_t* from = pool.data + x.head * pool.head + c * 128;
-                int64_t off[4];
-                uint32_t there[4], known[4];
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const int j = key0 + 32 * e + lane;
-                    int at = 0;
-                    const int page = j <= p_top ? page_of(a, table, j, at) : -1;
-                    off[e] = page >= 0 ? page * pool.page + at * pool.token : 0;
-                    there[e] = __ballot_sync(0xffffffffu, page >= 0);
-                    known[e] = __ballot_sync(0xffffffffu, page >= 0 || j > p_top);   // what no row sees need not be masked again
-                }
-                if (!bounded_wait_together<256>(PfWait<true, true>{&H.empty[slot], ((gs / AT_SLOTS) & 1) ^ 1, &H.abort})) {
+                const int c = i % CH;
+                const uint32_t kt = ktile + turn.j;
+                if (!bounded_wait_together<256>(PfWait<true, true>{&H.page_full[kt % AT_PAGES], (kt / AT_PAGES) & 1, &H.abort}) ||
+                    !bounded_wait_together<256>(PfWait<true, true>{&H.empty[slot], ((gs / AT_SLOTS) & 1) ^ 1, &H.abort})) {
                     give_up(AT_SITE_COPY);
                     ok = false;
                     break;
                 }
+                const AtPlaces& pl = places[kt % AT_PAGES];
+                const int64_t* place = turn.v ? pl.v : pl.k;
+                const uint8_t* from = (turn.v ? a.v.data + x.head * a.v.head : a.k.data + x.head * a.k.head) + c * 128 + ((lane & 7) << 4);
                 const uint32_t dst = pf_smem(ring + slot * AT_SLOT) + ((lane & 7) << 4);
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-#pragma unroll
-                    for (int s = 0; s < 8; s++) {
-                        // lanes 8 g to 8 g + 7: the eight pieces of row r
-                        const int r = 32 * e + 4 * s + (lane >> 3);
-                        const int64_t o = __shfl_sync(0xffffffffu, off[e], 4 * s + (lane >> 3));
-                        at_cp16((dst + r * 128) ^ ((r & 7) << 4), from + o + ((lane & 7) << 4), there[e] >> (4 * s + (lane >> 3)) & 1);
-                    }
+#pragma unroll 8
+                for (int s = 0; s < AT_KEYS / 4; s++) {
+                    const int r = 4 * s + (lane >> 3);        // lanes 8 g to 8 g + 7: the eight pieces of a row
+                    const int64_t o = place[r];
+                    at_cp16((dst + r * 128) ^ ((r & 7) << 4), from + max(o, (int64_t)0), o >= 0);
+                }
                 at_cp_arrive(&H.full[slot]);
-                if (!turn.v && c == 0 && lane < 4) H.there[(ktile + turn.j) & 7][lane] = lane == 0 ? known[0] : lane == 1 ? known[1] : lane == 2 ? known[2] : known[3];
                 __syncwarp();
-                if (lane == 0) pf_bar_arrive(&H.full[slot]);
+                if (lane == 0) pf_bar_arrive(&H.page_empty[kt % AT_PAGES]);
             }
             base += total;
             ktile += n;
         }
         asm volatile("cp.async.wait_all;" ::: "memory");   // nothing is in flight when the block ends
     } else if (warp == AT_MMA_WARP) {
+        at_fewer_regs();
         // ---- products
         uint32_t base = 0, pieces[2] = {0, 0};    // slots, Q tiles of the pieces before
         uint32_t used[3] = {0, 0, 0};             // S: of each tile of the pairs; the two of single tiles
@@ -306,13 +351,13 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(AttendCall a) 
         __syncwarp();
         pf_bar_wait(&H.drained, 0);
         __syncwarp();
-    } else {
+    } else if (warp < 8) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(AT_ROW_REGS));
         // ---- rows
         const int wg = warp >> 2, row = (warp & 3) * 32 + lane;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         uint32_t cs[3] = {0, 0, 0}, cpv = 0, ktile = 0;   // S of the pairs' tile, the two of single tiles
         const float scale = fmaxf(fabsf(a.scale_log2), 1e-30f);       // a masked score times it is no NaN
-        const uint32_t flip = a.scale_log2 < 0 ? 0x80008000u : 0u;    // a negative scale: of the rows
         bool ok = true;
         for (Piece x; ok && walk.next(x);) {
             const int n = max(x.n, 0);
@@ -329,28 +374,18 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(AttendCall a) 
             const int p_first = x.r.past + (int)a.group.div(min(x.row0 + t * 128, last)),
                       p_top = x.r.past + (int)a.group.div(min(x.row0 + t * 128 + 127, last));
             float m = -INFINITY, l = 0.0f;
+            const uint32_t qs = pf_smem(q_sm + t * At<D>::q_tile);
+            constexpr int PR = D / 8, RPI = 32 / PR;              // pieces of a row, rows of a warp's access
             if (n) {
-                // Q: the warp's own 32 rows, eight pieces in flight; past the tile's, zeros
-                const uint32_t qs = pf_smem(q_sm + t * At<D>::q_tile);
-                constexpr int PR = D / 8, RPI = 32 / PR;              // pieces of a row, rows at once
-#pragma unroll
-                for (int r0 = 0; r0 < 32; r0 += 8 * RPI) {
-                    uint4 w[8];
-#pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        const int r = (warp & 3) * 32 + r0 + e * RPI + lane / PR, Q = x.row0 + t * 128 + r, qt = (int)a.group.div(Q);
-                        w[e] = make_uint4(0, 0, 0, 0);
-                        if (Q <= last)
-                            w[e] = *(const uint4*)(a.q + (int64_t)(x.r.begin + qt) * a.q_token +
-                                                   (int64_t)(x.head * (int)a.group.d + Q - qt * (int)a.group.d) * a.q_head + (lane % PR) * 16);
-                    }
-#pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        const int r = (warp & 3) * 32 + r0 + e * RPI + lane / PR, c = lane % PR;
-                        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(qs + (c >> 3) * (128 * 128) + r * 128 + (((c ^ r) & 7) << 4)),
-                                     "r"(w[e].x ^ flip), "r"(w[e].y ^ flip), "r"(w[e].z ^ flip), "r"(w[e].w ^ flip) : "memory");
-                    }
+                // Q: the warp's own 32 rows; past the tile's, zeros
+#pragma unroll 8
+                for (int i = 0; i < 32 / RPI; i++) {
+                    const int r = (warp & 3) * 32 + i * RPI + lane / PR, Q = min(x.row0 + t * 128 + r, last), qt = (int)a.group.div(Q);
+                    at_cp16(at_piece(qs, r, lane % PR),
+                            a.q + (int64_t)(x.r.begin + qt) * a.q_token + (int64_t)(x.head * (int)a.group.d + Q - qt * (int)a.group.d) * a.q_head +
+                                (lane % PR) * 16, x.row0 + t * 128 + r <= last);
                 }
+                asm volatile("cp.async.wait_all;" ::: "memory");
                 at_fence_async();
                 __syncwarp();
                 if (lane == 0) pf_bar_arrive(&H.q_full[t]);
@@ -368,9 +403,12 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(AttendCall a) 
                     for (int e = 0; e < 4; e++) pf_tmem_ld32(s_at + 32 * e, *(int(*)[32])(v + 32 * e));
                     pf_tmem_wait_ld();
                     const int key0 = x.tiles.tile(x.i0 + j) * AT_KEYS;
-                    const uint4 there = *(const uint4*)H.there[(ktile + j) & 7];
+                    const uint4 there = *(const uint4*)H.there[(ktile + j) & 15];
                     const bool all = (there.x & there.y & there.z & there.w) == 0xffffffffu && key0 + AT_KEYS - 1 <= p_first &&
                                      (a.window <= 0 || p_top - key0 < a.window || key0 + AT_KEYS <= a.sinks);
+                    if (a.scale_log2 < 0.0f)
+#pragma unroll
+                        for (int i = 0; i < 128; i++) v[i] ^= (int)0x80000000u;
                     if (!all) {
                         const uint32_t tw[4] = {there.x, there.y, there.z, there.w};
 #pragma unroll
@@ -428,6 +466,10 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(AttendCall a) 
                     l += lo_of(sum[0]) + hi_of(sum[0]);
                     at_tmem_wait_st();
                 }
+                // Every product's end is waited for, and before the next one can begin: a parity tells a phase
+                // from the one before or after it only.  (Single tiles: the product before is followed by the
+                // next scores, so that the tensor cores do not wait for this.)
+                if (j && !at_wait_warp(&H.pv_done[t], (cpv + j - 1) & 1, &H.abort)) { ok = false; break; }
                 pf_fence_before();
                 __syncwarp();
                 if (lane == 0) pf_bar_arrive(&H.p_full[s]);
@@ -440,48 +482,65 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(AttendCall a) 
                 pf_fence_after();
             }
             if (!any) continue;
-            // ---- O out, 32 values of a row at a time
+            // ---- O out, through the shared memory of the warp's rows of Q, so that rows are written whole
             const bool cut = x.parts > 1;
             const float by = cut ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
-            uint8_t* out = a.out + (int64_t)(x.r.begin + tok) * a.out_token + (int64_t)h * a.out_head;
-            const int64_t place = (int64_t)x.slot(x.part) * TR + t * 128 + row;
-            float* part = a.part_o + place * D;
+            const int64_t out_at = (int64_t)(x.r.begin + tok) * a.out_token + (int64_t)h * a.out_head;
+            const int r0 = t * 128 + (warp & 3) * 32, rows = min(32, x.rows - r0);     // the warp's, of the tile
+            const int64_t place0 = (int64_t)x.slot(x.part) * TR + r0;
             float odd = l * 0.0f;                     // NaN as soon as something is not finite
+            __syncwarp();
+            // unfinished sums go out in f32, in two halves of the row, results in one
 #pragma unroll 1
-            for (int c = 0; c < D; c += 32) {
-                int o[32];
-                if (n) {
-                    pf_tmem_ld32(tmem + t * D + lanes + c, o);
-                    pf_tmem_wait_ld();
-                } else {
+            for (int half = 0; half < (cut ? 2 : 1); half++) {
+                const int c0 = half * (D / 2), c1 = cut ? c0 + D / 2 : D;
+#pragma unroll 1
+                for (int c = c0; c < c1; c += 32) {
+                    int o[32];
+                    if (n) {
+                        pf_tmem_ld32(tmem + t * D + lanes + c, o);
+                        pf_tmem_wait_ld();
+                    } else {
 #pragma unroll
-                    for (int i = 0; i < 32; i++) o[i] = 0;
+                        for (int i = 0; i < 32; i++) o[i] = 0;
+                    }
+                    float y[32];
+#pragma unroll
+                    for (int i = 0; i < 32; i++) {
+                        y[i] = __int_as_float(o[i]) * by;
+                        odd = fmaf(__int_as_float(o[i]), 0.0f, odd);
+                    }
+                    if (cut) {
+#pragma unroll
+                        for (int i = 0; i < 8; i++)
+                            sts128(at_piece(qs, row, (c - c0) / 4 + i), make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]));
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            sts128(at_piece(qs, row, c / 8 + i), make_uint4(pack2<T>(y[8 * i], y[8 * i + 1]), pack2<T>(y[8 * i + 2], y[8 * i + 3]),
+                                                                            pack2<T>(y[8 * i + 4], y[8 * i + 5]), pack2<T>(y[8 * i + 6], y[8 * i + 7])));
+                    }
                 }
-                float y[32];
-#pragma unroll
-                for (int i = 0; i < 32; i++) {
-                    y[i] = __int_as_float(o[i]) * by;
-                    odd = fmaf(__int_as_float(o[i]), 0.0f, odd);
-                }
-                if (mine && cut) {
-#pragma unroll
-                    for (int i = 0; i < 32; i += 4) __stcg((float4*)(part + c + i), make_float4(y[i], y[i + 1], y[i + 2], y[i + 3]));
-                } else if (mine) {
-#pragma unroll
-                    for (int i = 0; i < 32; i += 8)
-                        *(uint4*)(out + (c + i) * 2) = make_uint4(pack2<T>(y[i], y[i + 1]), pack2<T>(y[i + 2], y[i + 3]),
-                                                                  pack2<T>(y[i + 4], y[i + 5]), pack2<T>(y[i + 6], y[i + 7]));
+                __syncwarp();
+#pragma unroll 4
+                for (int i = 0; i < 32 / RPI; i++) {
+                    const int r = i * RPI + lane / PR, c = lane % PR;
+                    const int64_t to = __shfl_sync(0xffffffffu, out_at, r);
+                    const uint4 w = lds128(at_piece(qs, (warp & 3) * 32 + r, c));
+                    if (r < rows) {
+                        if (cut) __stcg((uint4*)(a.part_o + (place0 + r) * D + c0 + 4 * c), w);
+                        else *(uint4*)(a.out + to + 16 * c) = w;
+                    }
                 }
                 __syncwarp();
             }
-            if (cut && mine) __stcg(a.part_ml + place, make_float2(m * scale, l));
+            if (cut && mine) __stcg(a.part_ml + place0 + lane, make_float2(m * scale, l));
             for (uint32_t bad = __ballot_sync(0xffffffffu, mine && odd != 0.0f); bad; bad &= bad - 1) {
                 __syncwarp();
-                const int of = __ffs(bad) - 1, r = t * 128 + (warp & 3) * 32 + of;
+                const int of = __ffs(bad) - 1, r = r0 + of;
                 float o[D / 32], cm, cl;
                 careful_row<D, T>(a, x, r, AT_KEYS, o, cm, cl);
-                const int64_t out_of = __shfl_sync(0xffffffffu, (int64_t)(out - a.out), of);
-                const int64_t at = (int64_t)x.slot(x.part) * TR + r;
+                const int64_t out_of = __shfl_sync(0xffffffffu, out_at, of), at = place0 + of;
                 const float inv = cl == 0.0f ? 0.0f : 1.0f / cl;
                 for (int e = 0; e < D / 32; e++) {
                     if (cut) __stcg(a.part_o + at * D + lane + 32 * e, o[e]);
@@ -501,7 +560,6 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(AttendCall a) 
             }
             if (!__shfl_sync(0xffffffffu, last_one, 0)) continue;
             __threadfence();
-            const int r0 = t * 128 + (warp & 3) * 32;
             float M = -INFINITY, L = 0.0f;            // of the row of this lane
             for (int i = 0; i < x.parts; i++) M = fmaxf(M, __ldcg(a.part_ml + (int64_t)x.slot(i) * TR + r0 + lane).x);
             auto weight = [](float2 ml, float top) {  // a NaN piece has a sum that is one, whatever its maximum
@@ -512,35 +570,40 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(AttendCall a) 
                 L += ml.y * weight(ml, M);
             }
             const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-            constexpr int V = D / 32;                 // values a lane, neighbours
-            const int rows = min(32, x.rows - r0);
-#pragma unroll 4
-            for (int r = 0; r < rows; r++) {
-                const float top = __shfl_sync(0xffffffffu, M, r), f = __shfl_sync(0xffffffffu, inv, r);
-                const int64_t out_of = __shfl_sync(0xffffffffu, (int64_t)(out - a.out), r);
-                float y[V] = {};
+            constexpr int V = D / 32, AT_ONCE = D == 256 ? 4 : 8;       // values a lane, neighbours; rows in flight
+            for (int r = 0; r < rows; r += AT_ONCE) {
+                float y[AT_ONCE][V] = {};
                 for (int i = 0; i < x.parts; i++) {
-                    const int64_t at = (int64_t)x.slot(i) * TR + r0 + r;
-                    const float2 ml = __ldcg(a.part_ml + at);
-                    float z[V];
-                    const float* from = a.part_o + at * D + lane * V;
-                    if constexpr (V == 2) { const float2 u = __ldcg((const float2*)from); z[0] = u.x; z[1] = u.y; }
-                    else
+                    const float2 ml = __ldcg(a.part_ml + (int64_t)x.slot(i) * TR + r0 + lane);
+                    const float mine_w = weight(ml, M);
+                    const float* from = a.part_o + ((int64_t)x.slot(i) * TR + r0 + r) * D + lane * V;
+                    float z[AT_ONCE][V];
 #pragma unroll
-                        for (int e = 0; e < V; e += 4) {
-                            const float4 u = __ldcg((const float4*)(from + e));
-                            z[e] = u.x; z[e + 1] = u.y; z[e + 2] = u.z; z[e + 3] = u.w;
-                        }
-                    const float w = weight(ml, top);
+                    for (int u = 0; u < AT_ONCE; u++) {                 // rows past the tile's: whatever stands there
+                        if constexpr (V == 2) *(float2*)z[u] = __ldcg((const float2*)(from + u * D));
+                        else
 #pragma unroll
-                    for (int e = 0; e < V; e++)
-                        if (w != 0.0f) y[e] += z[e] * w;
+                            for (int e = 0; e < V; e += 4) *(float4*)(z[u] + e) = __ldcg((const float4*)(from + u * D + e));
+                    }
+#pragma unroll
+                    for (int u = 0; u < AT_ONCE; u++) {
+                        const float w = __shfl_sync(0xffffffffu, mine_w, r + u);
+#pragma unroll
+                        for (int e = 0; e < V; e++) y[u][e] = w != 0.0f ? y[u][e] + z[u][e] * w : y[u][e];
+                    }
                 }
-                uint32_t* to = (uint32_t*)(a.out + out_of) + lane * (V / 2);
 #pragma unroll
-                for (int e = 0; e < V; e += 2) to[e / 2] = pack2<T>(y[e] * f, y[e + 1] * f);
+                for (int u = 0; u < AT_ONCE; u++) {
+                    const float f = __shfl_sync(0xffffffffu, inv, r + u);
+                    const int64_t to = __shfl_sync(0xffffffffu, out_at, r + u);
+                    if (r + u >= rows) continue;
+#pragma unroll
+                    for (int e = 0; e < V; e += 2) ((uint32_t*)(a.out + to) + lane * (V / 2))[e / 2] = pack2<T>(y[u][e] * f, y[u][e + 1] * f);
+                }
             }
         }
+    } else {
+        at_fewer_regs();
     }
     pf_fence_before();
     __syncthreads();
