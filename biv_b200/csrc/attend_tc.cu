@@ -11,8 +11,9 @@
 //                (128-byte swizzle): K is read along the values (K-major), V along the keys (MN-major),
 //                so that neither is turned; P is read from tensor memory.
 //   warp 9       finds where a tile's keys lie, ahead of the copies.
-//   warps 12-15  copy K and V from the pages, 128 keys x 64 values (16 KB) a slot, in a ring of eight:
-//                cp.async in 16-byte pieces, since a tile's keys lie in pages of any size.
+//   warps 12-15  bring K and V from the pages, 128 keys x 64 values (16 KB) a slot, in a ring of eight: by
+//                the copy engine, a box for each page's part, where pages are of 16 tokens and more and
+//                the tile ends before the rows' last key; else cp.async in 16-byte pieces.
 //
 // Heads of up to 128 values: two tiles of 128 rows at once, a group each, so that one group's powers
 // run while the other's products do.  Heads of 256 values, whose O alone takes half of tensor memory,
@@ -21,6 +22,8 @@
 // m is not the running maximum itself but one that follows it when it has grown by more than 2^8:
 // O is then scaled in tensor memory, which happens a few times at a piece's start and rarely after (P
 // is at most 2^8, its sum and O are held in f32).
+#include <cuda.h>
+#include <cudaTypedefs.h>
 #include <stddef.h>
 
 #include "cache.cuh"
@@ -38,8 +41,14 @@ constexpr int AT_HEAD = 1024, AT_PAGES = 8;    // key tiles whose addresses stan
 constexpr float AT_GROWTH = 8.0f;     // powers of two
 enum { AT_SITE_COPY = 31, AT_SITE_MMA, AT_SITE_ROWS, AT_SITE_PAGES };
 
-// where a tile's keys and values lie, from the head's first page on; -1 where there is none
-struct AtPlaces { int64_t k[AT_KEYS], v[AT_KEYS]; };
+// Where a tile's keys and values lie: bytes from the head's first page on, -1 where there is none; or the
+// boxes that the copy engine fetches, the pool's number of pages for one that is not there (it writes zeros).
+struct AtPlaces {
+    union {
+        struct { int64_t k[AT_KEYS], v[AT_KEYS]; };
+        struct { int page[16], row[16]; };
+    };
+};
 template <int D> struct At {
     static constexpr int tiles = D == 256 ? 1 : 2;           // of 128 rows
     static constexpr int rows = 128 * tiles;
@@ -48,15 +57,21 @@ template <int D> struct At {
     static constexpr int fixed = AT_HEAD + tiles * q_tile + AT_SLOTS * AT_SLOT + (int)sizeof(AtPlaces) * AT_PAGES;
 };
 
+// the pools for the copy engine: boxes of `rows` tokens x 64 values; rows 0: none
+struct AtMaps {
+    CUtensorMap k, v;
+    int rows;
+};
 struct AtHead {
     uint64_t full[AT_SLOTS], empty[AT_SLOTS];
     // [0], [1]: of the two tiles of a pair; [2], [3]: of the two S of a single tile.  Apart, because the
     // second group passes single tiles by: a parity tells a phase from the next one only.
-    uint64_t s_full[4], p_full[4], q_full[2], pv_done[2], drained;
+    uint64_t s_full[4], p_half[4], p_full[4], q_full[2], pv_done[2], drained;
     uint64_t page_full[AT_PAGES], page_empty[AT_PAGES];
     // Which keys of a tile lie in pages that there are, or are seen by no row; read 16 bytes at once.  The
     // addresses are at most eight tiles ahead of the copies, these at most five ahead of the rows.
     alignas(16) uint32_t there[16][4];
+    int boxes[AT_PAGES];              // of a key tile that the copy engine fetches, or 0
     uint32_t tmem;
     int abort;
 };
@@ -77,6 +92,11 @@ __device__ __forceinline__ void at_cp16(uint32_t dst, const void* src, bool ther
 // the thread's arrival, once its copies so far have landed
 __device__ __forceinline__ void at_cp_arrive(uint64_t* bar) {
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(pf_smem(bar)) : "memory");
+}
+// 64 values of `rows` tokens of a page's head, zeros where there is no such page
+__device__ __forceinline__ void at_box(uint32_t dst, const CUtensorMap* map, int value, int token, int head, int page, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::
+                     "r"(dst), "l"(map), "r"(value), "r"(token), "r"(head), "r"(page), "r"(pf_smem(bar)) : "memory");
 }
 // what threads have written to shared memory, or have seen written, before what the tensor cores read
 __device__ __forceinline__ void at_fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
@@ -121,6 +141,11 @@ __device__ __forceinline__ uint32_t at_piece(uint32_t tile, int r, int c) {
 __device__ __forceinline__ void sts128(uint32_t a, uint4 v) {
     asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
 __device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
 
 // place q of the 2 n tiles of K and V in the order the products take them
@@ -133,7 +158,7 @@ __device__ __forceinline__ AtTurn at_turn(int q, int n, bool pair) {
 }
 
 template <int D, class T>
-__global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(AttendCall a) {
+__global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(const __grid_constant__ AttendCall a, const __grid_constant__ AtMaps maps) {
     extern __shared__ __align__(1024) uint8_t sm[];
     AtHead& H = *(AtHead*)sm;
     constexpr int NT = At<D>::tiles, TR = At<D>::rows, CH = At<D>::chunks;
@@ -154,7 +179,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(AttendCall a) 
             pf_bar_init(&H.q_full[i], 4);
             pf_bar_init(&H.pv_done[i], 1);
         }
-        for (int i = 0; i < 4; i++) { pf_bar_init(&H.s_full[i], 1); pf_bar_init(&H.p_full[i], 4); }
+        for (int i = 0; i < 4; i++) { pf_bar_init(&H.s_full[i], 1); pf_bar_init(&H.p_half[i], 4); pf_bar_init(&H.p_full[i], 4); }
         for (int i = 0; i < AT_PAGES; i++) { pf_bar_init(&H.page_full[i], 1); pf_bar_init(&H.page_empty[i], 2 * CH); }
         pf_bar_init(&H.drained, 1);
         H.abort = 0;
@@ -186,24 +211,39 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(AttendCall a) 
             const int32_t* table = a.table + (int64_t)x.b * a.table_stride;
             for (int j = 0; j < n; j++, ktile++) {
                 const int e = ktile % AT_PAGES, key0 = x.tiles.tile(x.i0 + j) * AT_KEYS;
+                // The copy engine fetches tiles that end before the rows' last key: what lies behind that one in
+                // its page belongs to nobody, may be anything, and has to be zeros here.
+                const bool boxes = maps.rows && key0 + AT_KEYS - 1 <= p_top;
                 int page[4], at[4];
                 uint32_t known[4];
+                if (boxes) {
+                    const int n_box = AT_KEYS / maps.rows;
+                    page[0] = lane < n_box ? page_of(a, table, key0 + lane * maps.rows, at[0]) : -1;
+                    const uint32_t there = __ballot_sync(0xffffffffu, page[0] >= 0);
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int key = key0 + 32 * i + lane;
-                    page[i] = key <= p_top ? page_of(a, table, key, at[i]) : -1;
-                    known[i] = __ballot_sync(0xffffffffu, page[i] >= 0 || key > p_top);
+                    for (int i = 0; i < 4; i++) known[i] = __ballot_sync(0xffffffffu, there >> ((32 * i + lane) / maps.rows) & 1);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int key = key0 + 32 * i + lane;
+                        page[i] = key <= p_top ? page_of(a, table, key, at[i]) : -1;
+                        known[i] = __ballot_sync(0xffffffffu, page[i] >= 0 || key > p_top);
+                    }
                 }
                 if (!bounded_wait_together<256>(PfWait<true, true>{&H.page_empty[e], ((ktile / AT_PAGES) & 1) ^ 1, &H.abort})) {
                     give_up(AT_SITE_PAGES);
                     ok = false;
                     break;
                 }
+                if (boxes) {
+                    if (lane < 16) { places[e].page[lane] = page[0] >= 0 ? page[0] : (int)a.k.n_pages; places[e].row[lane] = at[0]; }
+                } else
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     places[e].k[32 * i + lane] = page[i] >= 0 ? page[i] * a.k.page + at[i] * a.k.token : -1;
                     places[e].v[32 * i + lane] = page[i] >= 0 ? page[i] * a.v.page + at[i] * a.v.token : -1;
                 }
+                if (lane == 0) H.boxes[e] = boxes ? AT_KEYS / maps.rows : 0;
                 if (lane == 0) *(uint4*)H.there[ktile & 15] = make_uint4(known[0], known[1], known[2], known[3]);
                 __syncwarp();
                 if (lane == 0) pf_bar_arrive(&H.page_full[e]);
@@ -230,14 +270,32 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(AttendCall a) 
                     break;
                 }
                 const AtPlaces& pl = places[kt % AT_PAGES];
+                if (const int n_box = H.boxes[kt % AT_PAGES]) {
+                    if (lane == 0) pf_bar_expect_tx(&H.full[slot], AT_SLOT);
+                    __syncwarp();
+                    if (lane < n_box)
+                        at_box(pf_smem(ring + slot * AT_SLOT) + lane * maps.rows * 128, turn.v ? &maps.v : &maps.k, c * 64, pl.row[lane],
+                               x.head, pl.page[lane], &H.full[slot]);
+                    if (lane) pf_bar_arrive(&H.full[slot]);
+                    __syncwarp();
+                    if (lane == 0) pf_bar_arrive(&H.page_empty[kt % AT_PAGES]);
+                    continue;
+                }
                 const int64_t* place = turn.v ? pl.v : pl.k;
                 const uint8_t* from = (turn.v ? a.v.data + x.head * a.v.head : a.k.data + x.head * a.k.head) + c * 128 + ((lane & 7) << 4);
                 const uint32_t dst = pf_smem(ring + slot * AT_SLOT) + ((lane & 7) << 4);
-#pragma unroll 8
-                for (int s = 0; s < AT_KEYS / 4; s++) {
-                    const int r = 4 * s + (lane >> 3);        // lanes 8 g to 8 g + 7: the eight pieces of a row
-                    const int64_t o = place[r];
-                    at_cp16((dst + r * 128) ^ ((r & 7) << 4), from + max(o, (int64_t)0), o >= 0);
+                // lanes 8 g to 8 g + 7: the eight pieces of a row; eight addresses at a time, so that their loads'
+                // latency passes once for eight copies
+#pragma unroll
+                for (int s0 = 0; s0 < AT_KEYS / 4; s0 += 8) {
+                    int64_t o[8];
+#pragma unroll
+                    for (int s = 0; s < 8; s++) o[s] = place[4 * (s0 + s) + (lane >> 3)];
+#pragma unroll
+                    for (int s = 0; s < 8; s++) {
+                        const int r = 4 * (s0 + s) + (lane >> 3);
+                        at_cp16((dst + r * 128) ^ ((r & 7) << 4), from + max(o[s], (int64_t)0), o[s] >= 0);
+                    }
                 }
                 at_cp_arrive(&H.full[slot]);
                 __syncwarp();
@@ -282,16 +340,23 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(AttendCall a) 
                     }
                     pf_commit(&H.s_full[s]);
                 };
-                auto values = [&](int q, int t, int s, bool first) {   // O_t += P_s V
-                    const uint32_t va = pf_smem(ring + slot_of(q, 0) * AT_SLOT);
-#pragma unroll
-                    for (int k = 0; k < AT_KEYS / 16; k++)
-                        at_mma_ts(o_at + t * D, s_at + (s & 1) * 128 + 8 * k, at_desc_v(va + 2048 * k), at_idesc<T>(D, true), !first || k);
-                    pf_commit(&H.pv_done[t]);
-                };
-                auto powers = [&](int s) {
-                    wait(&H.p_full[s], cp[s]++ & 1);
+                // O_t += P_s V: the first 64 keys' weights are there before the others are made
+                auto values = [&](int q, int t, int s, bool first) {
+                    const uint32_t va = pf_smem(ring + slot_of(q, 0) * AT_SLOT), parity = cp[s]++ & 1;
+                    wait(&H.p_half[s], parity);
+                    for (int c = 0; c < CH; c++) landed(q, c);
                     pf_fence_after();
+                    if (!ok) return;
+#pragma unroll
+                    for (int k = 0; k < AT_KEYS / 16; k++) {
+                        if (k == AT_KEYS / 32) {
+                            wait(&H.p_full[s], parity);
+                            pf_fence_after();
+                            if (!ok) return;
+                        }
+                        at_mma_ts(o_at + t * D, s_at + (s & 1) * 128 + 8 * k, at_desc_v(va + 2048 * k), at_idesc<T>(D, true), !first || k);
+                    }
+                    pf_commit(&H.pv_done[t]);
                 };
                 wait(&H.q_full[0], pieces[0] & 1);
                 if (pair) wait(&H.q_full[1], pieces[1] & 1);
@@ -302,10 +367,8 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(AttendCall a) 
                     for (int j = 0; j < n && ok; j++) {
                         const bool more = j + 1 < n;
                         for (int t = 0; t < 2 && ok; t++) {
-                            powers(t);
-                            if (t == 0) for (int c = 0; c < CH; c++) landed(2 * j + 1, c);
-                            if (!ok) break;
                             values(2 * j + 1, t, t, j == 0);
+                            if (!ok) break;
                             if (t == 1) free(2 * j + 1);
                             if (more) {
                                 if (t == 0) for (int c = 0; c < CH; c++) landed(2 * j + 2, c);
@@ -326,11 +389,8 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(AttendCall a) 
                             scores(kq, 0, 2 + ((j + 1) & 1));
                             free(kq);
                         }
-                        powers(2 + (j & 1));
-                        for (int c = 0; c < CH; c++) landed(vq, c);
-                        if (!ok) break;
                         values(vq, 0, 2 + (j & 1), j == 0);
-                        free(vq);
+                        if (ok) free(vq);
                     }
                 }
                 if (!ok) {
@@ -395,6 +455,10 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(AttendCall a) 
                 uint32_t& count = pair ? cs[0] : j & 1 ? cs[2] : cs[1];
                 if (!at_wait_warp(&H.s_full[s], count & 1, &H.abort)) { ok = false; break; }
                 count++;
+                // Every product's end is waited for, and before the next one can begin: a parity tells a phase
+                // from the one before or after it only.  (Single tiles: the product before is followed by the
+                // next scores, so that the tensor cores do not wait for this.)
+                auto before = [&] { return !j || at_wait_warp(&H.pv_done[t], (cpv + j - 1) & 1, &H.abort); };
                 if (any) {
                     pf_fence_after();
                     const uint32_t s_at = tmem + 256 + (s & 1) * 128 + lanes;
@@ -420,15 +484,15 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(AttendCall a) 
                             for (int i = 0; i < 32; i++) v[32 * e + i] = see >> i & 1 ? v[32 * e + i] : (int)0xff800000u;   // -infinity
                         }
                     }
-                    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    float top[4] = {m, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int i = 0; i < 128; i++) top[i & 3] = fmaxf(top[i & 3], __int_as_float(v[i]));
-                    const float grown = fmaxf(fmaxf(m, fmaxf(top[0], top[1])), fmaxf(top[2], top[3]));
+                    for (int i = 0; i < 128; i += 2) top[i / 2 & 3] = max3(top[i / 2 & 3], __int_as_float(v[i]), __int_as_float(v[i + 1]));
+                    const float grown = fmaxf(max3(top[0], top[1], top[2]), top[3]);
                     if (j == 0) m = grown;
                     const bool far = (grown - m) * scale > AT_GROWTH;
                     if (__any_sync(0xffffffffu, far)) {
                         // O follows, once the product before has been added
-                        if (!at_wait_warp(&H.pv_done[t], (cpv + j - 1) & 1, &H.abort)) { ok = false; break; }
+                        if (!before()) { ok = false; break; }
                         pf_fence_after();
                         const float by = far ? (m == -INFINITY ? 0.0f : exp2_of((m - grown) * scale)) : 1.0f;
                         if (far) m = grown;
@@ -448,28 +512,36 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(AttendCall a) 
                     const float minus = m == -INFINITY ? 0.0f : -m * scale;
                     const f32x2 sc = pk(scale, scale), mi = pk(minus, minus);
                     f32x2 sum[2] = {0, 0};
-                    uint32_t w[32];
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
+                        uint32_t w[32];
 #pragma unroll
                         for (int i = 0; i < 32; i++) {
                             const f32x2 z = fma2(pk(__int_as_float(v[64 * e + 2 * i]), __int_as_float(v[64 * e + 2 * i + 1])), sc, mi);
-                            const float y0 = exp2_of(lo_of(z)), y1 = exp2_of(hi_of(z));
-                            sum[i & 1] = add2(sum[i & 1], pk(y0, y1));
+                            const f32x2 y = pk(exp2_of(lo_of(z)), exp2_of(hi_of(z)));
+                            sum[i & 1] = add2(sum[i & 1], y);
                             // the weights rounded to the cache's type for the second product (relative error
                             // 2^-9 or 2^-12 each); l sums them unrounded
-                            w[i] = pack2<T>(y0, y1);
+                            w[i] = pack2<T>(lo_of(y), hi_of(y));
                         }
                         at_tmem_st32(s_at + 32 * e, w);
+                        if (e == 0) {
+                            at_tmem_wait_st();
+                            if (!before()) { ok = false; break; }
+                            pf_fence_before();
+                            __syncwarp();
+                            if (lane == 0) pf_bar_arrive(&H.p_half[s]);
+                        }
                     }
+                    if (!ok) break;
                     sum[0] = add2(sum[0], sum[1]);
                     l += lo_of(sum[0]) + hi_of(sum[0]);
                     at_tmem_wait_st();
+                } else {
+                    if (!before()) { ok = false; break; }
+                    __syncwarp();
+                    if (lane == 0) pf_bar_arrive(&H.p_half[s]);
                 }
-                // Every product's end is waited for, and before the next one can begin: a parity tells a phase
-                // from the one before or after it only.  (Single tiles: the product before is followed by the
-                // next scores, so that the tensor cores do not wait for this.)
-                if (j && !at_wait_warp(&H.pv_done[t], (cpv + j - 1) & 1, &H.abort)) { ok = false; break; }
                 pf_fence_before();
                 __syncwarp();
                 if (lane == 0) pf_bar_arrive(&H.p_full[s]);
@@ -522,14 +594,19 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(AttendCall a) 
                     }
                 }
                 __syncwarp();
-#pragma unroll 4
-                for (int i = 0; i < 32 / RPI; i++) {
-                    const int r = i * RPI + lane / PR, c = lane % PR;
-                    const int64_t to = __shfl_sync(0xffffffffu, out_at, r);
-                    const uint4 w = lds128(at_piece(qs, (warp & 3) * 32 + r, c));
-                    if (r < rows) {
-                        if (cut) __stcg((uint4*)(a.part_o + (place0 + r) * D + c0 + 4 * c), w);
-                        else *(uint4*)(a.out + to + 16 * c) = w;
+#pragma unroll
+                for (int i0 = 0; i0 < 32 / RPI; i0 += 8) {
+                    uint4 w[8];
+#pragma unroll
+                    for (int i = 0; i < 8; i++) w[i] = lds128(at_piece(qs, (warp & 3) * 32 + (i0 + i) * RPI + lane / PR, lane % PR));
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const int r = (i0 + i) * RPI + lane / PR, c = lane % PR;
+                        const int64_t to = __shfl_sync(0xffffffffu, out_at, r);
+                        if (r < rows) {
+                            if (cut) __stcg((uint4*)(a.part_o + (place0 + r) * D + c0 + 4 * c), w[i]);
+                            else *(uint4*)(a.out + to + 16 * c) = w[i];
+                        }
                     }
                 }
                 __syncwarp();
@@ -614,13 +691,41 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(AttendCall a) 
     }
 }
 
+template <class T> constexpr bool at_is_half = false;
+template <> constexpr bool at_is_half<__half> = true;
+// Pages of fewer than 16 tokens go by cp.async: a tile would be sixteen boxes and more.
+constexpr int AT_LEAST_BOX = 16;
+// A pool as the copy engine takes it.  False where it cannot (a stride out of its range): cp.async can.
+static bool at_map(CUtensorMap* m, const Pool& p, const AttendCall& a, int dim, bool half, int rows) {
+    static const PFN_cuTensorMapEncodeTiled_v12000 encode = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult found = cudaDriverEntryPointSymbolNotFound;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &found) != cudaSuccess) cudaGetLastError();
+        return (PFN_cuTensorMapEncodeTiled_v12000)(found == cudaDriverEntryPointSuccess ? f : nullptr);
+    }();
+    if (!encode || p.n_pages < 1 || p.token <= 0 || p.head <= 0 || p.page <= 0) return false;
+    const cuuint64_t dims[4] = {(cuuint64_t)dim, a.page.d, (cuuint64_t)a.heads_kv, (cuuint64_t)p.n_pages};
+    const cuuint64_t strides[3] = {(cuuint64_t)p.token, (cuuint64_t)p.head, (cuuint64_t)p.page};
+    const cuuint32_t box[4] = {64, (cuuint32_t)rows, 1, 1}, step[4] = {1, 1, 1, 1};
+    return encode(m, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, p.data, dims, strides, box, step,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int D, class T> static cudaError_t tc(const AttendCall& a, int sm_count, cudaStream_t stream) {
     static_assert(At<D>::fixed + share_smem(kCacheSeqs, AT_THREADS) <= 227 * 1024, "the block must fit in shared memory");
     static std::atomic<uint64_t> attr_set{0};
     if (cudaError_t e = ensure_dynamic_smem(attend_tc_kernel<D, T>, (int)(At<D>::fixed + share_smem(kCacheSeqs, AT_THREADS)), attr_set)) return e;
+    AtMaps maps;
+    maps.rows = 0;
+    int rows = 128;                   // the largest power of two, up to a tile, that divides a page
+    while (a.page.d % rows) rows /= 2;
+    if (rows >= AT_LEAST_BOX && at_map(&maps.k, a.k, a, D, at_is_half<T>, rows) &&
+        at_map(&maps.v, a.v, a, D, at_is_half<T>, rows))
+        maps.rows = rows;
     count_launch();
     return launch_with(false, stream, attend_tc_kernel<D, T>, dim3(sm_count), dim3(AT_THREADS),
-                       (size_t)At<D>::fixed + share_smem(a.n_seq, AT_THREADS), a);
+                       (size_t)At<D>::fixed + share_smem(a.n_seq, AT_THREADS), a, maps);
 }
 cudaError_t launch_attend_tc(const AttendCall& a, int head_dim, int ggml_type, int sm_count, cudaStream_t stream) {
     const bool f16 = ggml_type == BIVMOE_F16;
