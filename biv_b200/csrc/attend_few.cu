@@ -17,7 +17,7 @@
 namespace bivmoe {
 
 constexpr int kFewWarps = 4, kFewThreads = 32 * kFewWarps, kFewStages = 3;
-constexpr int kFewLeast = 2;      // key tiles that are worth a block
+constexpr int kFewLeast = 2, kFewExtra = 3;   // key tiles that are worth a block; that a tile costs besides
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool there) {
     // nothing is read, and zeros are written, where there is nothing
@@ -68,11 +68,11 @@ __global__ void __launch_bounds__(kFewThreads, D == 256 ? 1 : 2) attend_few_kern
     uint8_t* ring_p = sm + warp * kFewStages * Few<D>::stage;
     const uint32_t ring = pf_smem(ring_p), qs = pf_smem(sm + Few<D>::ring);
     pdl_enter();
-    const Share share = find_share<KT, kFewRows, kFewThreads>(a, kFewLeast, (int64_t*)(sm + Few<D>::fixed));
+    const Share share = find_share<KT, kFewRows, kFewExtra, kFewThreads>(a, kFewLeast, (int64_t*)(sm + Few<D>::fixed));
     const int g = lane >> 2, quad = lane & 3;
     constexpr int CH = D / 8, RPI = 32 / CH;      // 16-byte pieces of a row, rows of a warp's copy
 
-    Walk<KT, kFewRows> walk(a, share);
+    Walk<KT, kFewRows, kFewExtra> walk(a, share);
     for (Piece x; walk.next(x);) {
         __syncthreads();                          // the piece before is done with the rings and the rows
         const int32_t* table = a.table + (int64_t)x.b * a.table_stride;

@@ -53,6 +53,7 @@ template <int D> struct At {
     static constexpr int tiles = D == 256 ? 1 : 2;           // of 128 rows
     static constexpr int rows = 128 * tiles;
     static constexpr int chunks = D / 64;                    // slots of a tile of K, or of V
+    static constexpr int extra = D == 256 ? 4 : 3;           // key tiles that a tile costs besides
     static constexpr int q_tile = 128 * D * 2;
     static constexpr int fixed = AT_HEAD + tiles * q_tile + AT_SLOTS * AT_SLOT + (int)sizeof(AtPlaces) * AT_PAGES;
 };
@@ -169,7 +170,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(const __grid_c
     // the share is looked at once a piece: it stands in shared memory, the rows' registers are full
     __shared__ Share share;
     {
-        const Share found = find_share<AT_KEYS, TR, AT_THREADS>(a, 1, (int64_t*)(sm + At<D>::fixed));
+        const Share found = find_share<AT_KEYS, TR, At<D>::extra, AT_THREADS>(a, 1, (int64_t*)(sm + At<D>::fixed));
         if (found.lo >= found.hi) return;
         if (tid == 0) share = found;
     }
@@ -199,7 +200,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(const __grid_c
             *(volatile int*)&H.abort = 1;
         }
     };
-    Walk<AT_KEYS, TR> walk(a, share);
+    Walk<AT_KEYS, TR, At<D>::extra> walk(a, share);
 
     if (warp == AT_PAGE_WARP) {
         at_fewer_regs();

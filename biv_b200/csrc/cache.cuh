@@ -113,7 +113,8 @@ __device__ __forceinline__ int page_of(const AttendCall& a, const int32_t* row, 
 // ---- shares of the work ----------------------------------------------------------------------------
 // A tile is TR rows of a request's kv head (row r: token r / group, query head r % group: the heads that
 // share keys share the tile); its work is the key tiles it sees, one unit each (a tile that sees none:
-// one, for its zeros).  The units of all tiles stand in one line, requests, kv heads, tiles, key tiles
+// one, for its zeros), and EXTRA units before them that stand for what a tile costs besides (its rows
+// in, its sums out).  The units of all tiles stand in one line, requests, kv heads, tiles, key tiles
 // in this order, and each of `g` blocks takes an equal share of the line, wherever that cuts a tile:
 // the blocks end together whatever the lengths are, and a block has at most two pieces of tiles
 // that others share, so that the room for pieces is two to a block.  Every block finds its share by
@@ -128,13 +129,13 @@ struct Share {
 template <int KT, int TR> __device__ __forceinline__ TileList tile_list(const AttendCall& a, const Request& r, int t) {
     return tiles_of<KT>(a, r.past + (int)a.group.div(t * TR), r.past + (int)a.group.div(min((t + 1) * TR, r.rows) - 1));
 }
-template <int KT, int TR> __device__ __forceinline__ int tile_units(const AttendCall& a, const Request& r, int t) {
-    return max(tile_list<KT, TR>(a, r, t).n, 1);
+template <int KT, int TR, int EXTRA> __device__ __forceinline__ int tile_units(const AttendCall& a, const Request& r, int t) {
+    return EXTRA + max(tile_list<KT, TR>(a, r, t).n, 1);
 }
 constexpr size_t share_smem(int n_seq, int threads) { return (((size_t)n_seq + 1 + threads / 32) * 8 + 15) / 16 * 16; }
 constexpr int kAlone = 4;            // tiles of a request that one thread counts
 // least: units that are worth a block
-template <int KT, int TR, int THREADS>
+template <int KT, int TR, int EXTRA, int THREADS>
 __device__ __forceinline__ Share find_share(const AttendCall& a, int least, int64_t* sh /* share_smem */) {
     constexpr int WARPS = THREADS / 32;
     int64_t* before = sh;
@@ -148,12 +149,12 @@ __device__ __forceinline__ Share find_share(const AttendCall& a, int least, int6
         const int nt = (r.rows + TR - 1) / TR;
         int64_t units = 0;
         if (nt <= kAlone)
-            for (int t = 0; t < nt; t++) units += tile_units<KT, TR>(a, r, t);
+            for (int t = 0; t < nt; t++) units += tile_units<KT, TR, EXTRA>(a, r, t);
         for (uint32_t many = __ballot_sync(0xffffffffu, nt > kAlone); many; many &= many - 1) {
             const int of = __ffs(many) - 1;   // a long one: counted by the warp
             const Request q{__shfl_sync(0xffffffffu, r.begin, of), __shfl_sync(0xffffffffu, r.rows, of), __shfl_sync(0xffffffffu, r.past, of)};
             int64_t some = 0;
-            for (int t = lane; t < (q.rows + TR - 1) / TR; t += 32) some += tile_units<KT, TR>(a, q, t);
+            for (int t = lane; t < (q.rows + TR - 1) / TR; t += 32) some += tile_units<KT, TR, EXTRA>(a, q, t);
             for (int d = 16; d; d >>= 1) some += __shfl_xor_sync(0xffffffffu, some, d);
             if (lane == of) units = some;
         }
@@ -199,7 +200,7 @@ struct Piece {
     __device__ __forceinline__ int slot(int p) const { return p == 0 ? 2 * c0 + 1 : 2 * (c0 + p); }
 };
 // The pieces of a block's share, one after another: every warp goes through them by itself.
-template <int KT, int TR> struct Walk {
+template <int KT, int TR, int EXTRA> struct Walk {
     const AttendCall& a;
     const Share& s;
     int64_t at;                      // the next unit
@@ -218,7 +219,7 @@ template <int KT, int TR> struct Walk {
         int64_t in = rest - head * each;
         const int lane = threadIdx.x & 31;
         for (t = 0; nt > 1 && t < nt;) {   // the tile: 32 of them at a time
-            const int mine = t + lane < nt ? tile_units<KT, TR>(a, r, t + lane) : 0;
+            const int mine = t + lane < nt ? tile_units<KT, TR, EXTRA>(a, r, t + lane) : 0;
             int64_t x = mine;
             for (int d = 1; d < 32; d <<= 1) {
                 const int64_t y = __shfl_up_sync(0xffffffffu, x, d);
@@ -241,42 +242,48 @@ template <int KT, int TR> struct Walk {
         r = request_of(a, b);
         nt = (r.rows + TR - 1) / TR;
     }
+    // The next piece; false at the share's end.  What the share has of a tile's EXTRA units alone is no piece.
     __device__ __forceinline__ bool next(Piece& x) {
-        if (at >= s.hi) return false;
-        x.b = b;
-        x.head = head;
-        x.r = r;
-        x.row0 = t * TR;
-        x.rows = min(TR, r.rows - x.row0);
-        x.tiles = tile_list<KT, TR>(a, r, t);
-        const int units = max(x.tiles.n, 1), take = (int)min((int64_t)(units - off), s.hi - at);
-        x.i0 = off;
-        x.n = min(off + take, x.tiles.n) - off;
-        x.part = 0;
-        x.parts = 1;
-        x.c0 = (int)blockIdx.x;
-        if (take < units) {
-            x.c0 = s.owner(at - off);
-            x.parts = s.owner(at - off + units - 1) - x.c0 + 1;
-            x.part = (int)blockIdx.x - x.c0;
-        }
-        at += take;
-        off += take;
-        if (off == units) {
-            off = 0;
-            if (++t == nt) {
-                t = 0;
-                if (++head == a.heads_kv) {
-                    head = 0;
-                    if (at < s.hi) {
-                        int next = b + 1;
-                        while (s.before[next + 1] == s.before[next]) next++;   // those without rows
-                        open(next);
+        for (;;) {
+            if (at >= s.hi) return false;
+            x.tiles = tile_list<KT, TR>(a, r, t);
+            const int units = EXTRA + max(x.tiles.n, 1), take = (int)min((int64_t)(units - off), s.hi - at), end = off + take;
+            const bool some = end > EXTRA;
+            if (some) {
+                x.b = b;
+                x.head = head;
+                x.r = r;
+                x.row0 = t * TR;
+                x.rows = min(TR, r.rows - x.row0);
+                x.i0 = max(off - EXTRA, 0);
+                x.n = min(end - EXTRA, x.tiles.n) - x.i0;
+                x.part = 0;
+                x.parts = 1;
+                x.c0 = (int)blockIdx.x;
+                if (off > EXTRA || end < units) {
+                    x.c0 = s.owner(at - off + EXTRA);
+                    x.parts = s.owner(at - off + units - 1) - x.c0 + 1;
+                    x.part = (int)blockIdx.x - x.c0;
+                }
+            }
+            at += take;
+            off = end;
+            if (off == units) {
+                off = 0;
+                if (++t == nt) {
+                    t = 0;
+                    if (++head == a.heads_kv) {
+                        head = 0;
+                        if (at < s.hi) {
+                            int next = b + 1;
+                            while (s.before[next + 1] == s.before[next]) next++;   // those without rows
+                            open(next);
+                        }
                     }
                 }
             }
+            if (some) return true;
         }
-        return true;
     }
 };
 
