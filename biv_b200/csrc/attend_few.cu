@@ -3,7 +3,7 @@
 //
 //   s_j = scale q . k_j,  m = max s_j,  l = sum 2^(s_j - m),  o = sum 2^(s_j - m) v_j / l   (s in powers of two)
 //
-// A block is four warps; of a tile of 64 keys (heads of 64 values: 128) a warp takes a quarter, in a ring of its own in shared memory
+// A block is four warps; of a tile of 64 keys a warp takes a quarter, in a ring of its own in shared memory
 // that its own cp.async copies fill, with its own running maximum, sum and o: the warps meet at the
 // piece's end only, where the four o are joined.  The work is shared out over blocks wherever that cuts a
 // long axis (cache.cuh); the block that is last to finish a tile joins its pieces, in their own order
@@ -35,35 +35,91 @@ __device__ __forceinline__ void ldm4t(uint32_t a, uint32_t (&r)[4]) {
 }
 template <class T> __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
 template <> __device__ __forceinline__ void mma16<__nv_bfloat16>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 template <> __device__ __forceinline__ void mma16<__half>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Keys of a warp's stage: what a stage costs beside its copies and products (pages, barriers, the running
-// maximum) is the same for 16 keys of 64 values and of 256.
 template <int D> struct Few {
-    static constexpr int keys = D == 64 ? 32 : 16, tile = keys * kFewWarps;
+    static constexpr int keys = 16, tile = keys * kFewWarps;
     static constexpr int half = keys * D * 2, stage = 2 * half;   // bytes: k, then v
     static constexpr int ring = kFewWarps * kFewStages * stage;
     static constexpr int fixed = ring + 16 * D * 2;               // and the 16 rows of q
+    static constexpr int part = D + 8;                            // floats from row to row where the warps' o meet: 8 rows apart, no bank twice
+    static_assert(16 * part * 4 <= kFewStages * stage, "");
 };
 
+// bytes from a head's first page on to a key's k and v
+struct alignas(16) Place { int64_t k, v; };
 // 16-byte piece `c` of row `r`: the low three bits of the piece's place are turned by the row, so that
 // eight rows' pieces c lie in different banks
 template <int D> __device__ __forceinline__ uint32_t few_at(int r, int c) {
     return (uint32_t)(r * (D * 2) + ((c ^ (r & 7)) << 4));
 }
 
+// The pieces of a tile, joined in their order by the block that was last.  The threads divide up the rows
+// that there are; four pieces are under way at a time.
+template <int D, class T> __device__ __forceinline__ void join(const AttendCall& a, const Piece& x) {
+    constexpr int CK = D / 32 < 4 ? D / 32 : 4;   // 16-byte pieces of a row that a thread has under way
+    const int per_row = min(kFewThreads / (x.rows > 8 ? 16 : x.rows > 4 ? 8 : 4), D / 4);
+    const int row = threadIdx.x / per_row, sub = threadIdx.x - row * per_row;
+    if (row >= x.rows) return;
+    const int R = x.row0 + row, tok = (int)a.group.div(R), h = x.head * (int)a.group.d + R - tok * (int)a.group.d;
+    auto weight = [](float2 ml, float top) {      // a NaN piece has a sum that is one, whatever its maximum
+        return ml.x == -INFINITY ? (ml.y == 0.0f ? 0.0f : 1.0f) : exp2_of(ml.x - top);
+    };
+    for (int c0 = sub * 4; c0 < D; c0 += CK * 4 * per_row) {
+        float M = -INFINITY, L = 0.0f;
+        float4 y[CK] = {};
+#pragma unroll 1
+        for (int s0 = 0; s0 < x.parts; s0 += 4) {
+            float2 ml[4];
+            float4 v[4][CK];
+#pragma unroll
+            for (int s = 0; s < 4; s++) {         // past the last piece: the last one again, of weight 0
+                const int64_t at = (int64_t)x.slot(min(s0 + s, x.parts - 1)) * kFewRows + row;
+                ml[s] = __ldcg(a.part_ml + at);
+#pragma unroll
+                for (int i = 0; i < CK; i++) v[s][i] = __ldcg((const float4*)(a.part_o + at * D + min(c0 + 4 * per_row * i, D - 4)));
+            }
+            float top = M;
+#pragma unroll
+            for (int s = 0; s < 4; s++) top = fmaxf(top, ml[s].x);
+            const float keep = weight(make_float2(M, 0.0f), top);
+            L *= keep;
+#pragma unroll
+            for (int i = 0; i < CK; i++) { y[i].x *= keep; y[i].y *= keep; y[i].z *= keep; y[i].w *= keep; }
+            M = top;
+#pragma unroll
+            for (int s = 0; s < 4; s++) {
+                const float w = s0 + s < x.parts ? weight(ml[s], M) : 0.0f;
+                if (w == 0.0f) continue;
+                L += ml[s].y * w;
+#pragma unroll
+                for (int i = 0; i < CK; i++) {
+                    y[i].x += v[s][i].x * w; y[i].y += v[s][i].y * w; y[i].z += v[s][i].z * w; y[i].w += v[s][i].w * w;
+                }
+            }
+        }
+        const float by = L == 0.0f ? 0.0f : 1.0f / L;
+        T* out = (T*)(a.out + (int64_t)(x.r.begin + tok) * a.out_token + (int64_t)h * a.out_head);
+#pragma unroll
+        for (int i = 0; i < CK; i++)
+            if (c0 + 4 * per_row * i < D)
+                *(uint2*)(out + c0 + 4 * per_row * i) = make_uint2(pack2<T>(y[i].x * by, y[i].y * by), pack2<T>(y[i].z * by, y[i].w * by));
+    }
+}
+
 template <int D, class T>
-__global__ void __launch_bounds__(kFewThreads, D == 256 ? 1 : 2) attend_few_kernel(AttendCall a) {
+__global__ void __launch_bounds__(kFewThreads, few_blocks(D)) attend_few_kernel(AttendCall a) {
     extern __shared__ __align__(1024) uint8_t sm[];
     constexpr int KW = Few<D>::keys, KT = Few<D>::tile;
     __shared__ float s_m[kFewWarps][16], s_l[kFewWarps][16];
     __shared__ int s_bad[16], s_last;
+    __shared__ Place s_place[kFewWarps][Few<D>::keys];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     uint8_t* ring_p = sm + warp * kFewStages * Few<D>::stage;
     const uint32_t ring = pf_smem(ring_p), qs = pf_smem(sm + Few<D>::ring);
@@ -85,62 +141,71 @@ __global__ void __launch_bounds__(kFewThreads, D == 256 ? 1 : 2) attend_few_kern
         cp_commit();
         const int n = x.n, p_first = x.r.past + (int)a.group.div(x.row0), p_top = x.r.past + (int)a.group.div(x.row0 + x.rows - 1);
         const uint8_t *k_base = a.k.data + x.head * a.k.head, *v_base = a.v.data + x.head * a.v.head;
-        // lane r: where key r of the warp's next stage lies
-        auto find = [&](int i, int64_t& ko, int64_t& vo, bool& ok) {
+        // lane r: where key r of the warp's stage i lies, or -1; keys that no row sees are not fetched
+        auto find = [&](int i) {
             const int j = x.tiles.tile(x.i0 + i) * KT + warp * KW + (lane & (KW - 1));
             int at = 0;
-            const int page = i < n && j <= p_top ? page_of(a, table, j, at) : -1;
-            ok = page >= 0;
-            ko = ok ? page * a.k.page + at * a.k.token : 0;
-            vo = ok ? page * a.v.page + at * a.v.token : 0;
+            const int page = i < n && seen(a, p_first, p_top, j) ? page_of(a, table, j, at) : -1;
+            return page >= 0 ? Place{page * a.k.page + at * a.k.token, page * a.v.page + at * a.v.token} : Place{-1, -1};
         };
-        uint32_t there[kFewStages];               // which of a stage's keys there are
-        int64_t ko, vo;
-        bool ok;
-        find(0, ko, vo, ok);
-        auto copy = [&](int i, int slot) {        // stage i, whose keys have been found; finds the next one's
-            const uint32_t mask = __ballot_sync(0xffffffffu, ok);   // KW 16: twice the same
-            const uint32_t dst = ring + slot * Few<D>::stage;
-            if (i < n) {
+        // the places of the first stages are asked for together: one trip to the table
+        Place ahead[kFewStages];
 #pragma unroll
-                for (int e = 0; e < KW / RPI; e++) {
-                    const int r = e * RPI + lane / CH, c = lane % CH;
-                    const int64_t kr = __shfl_sync(0xffffffffu, ko, r), vr = __shfl_sync(0xffffffffu, vo, r);
-                    cp16(dst + few_at<D>(r, c), k_base + kr + c * 16, mask >> r & 1);
-                    cp16(dst + Few<D>::half + few_at<D>(r, c), v_base + vr + c * 16, mask >> r & 1);
-                }
-            }
-            cp_commit();
-            find(i + 1, ko, vo, ok);
-            return mask;
-        };
-#pragma unroll
-        for (int i = 0; i < kFewStages - 1; i++) there[i] = copy(i, i);
-        cp_wait<kFewStages - 1>();                // the rows, which were asked for first
-        __syncthreads();
+        for (int i = 0; i < kFewStages; i++) ahead[i] = find(i);
         // D 256: a row's fragments take as many registers as half of o: read again at each use
         constexpr bool HOLD = D <= 128;
         uint32_t qf[HOLD ? D / 16 : 1][4];
-        if (HOLD)
-#pragma unroll
-            for (int k = 0; k < D / 16; k++) ldm4(qs + few_at<D>(lane & 15, 2 * k + (lane >> 4)), qf[k % (HOLD ? D / 16 : 1)]);
         int p[2];
 #pragma unroll
         for (int i = 0; i < 2; i++) p[i] = g + 8 * i < x.rows ? x.r.past + (int)a.group.div(x.row0 + g + 8 * i) : -1;
         float o[D / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < D / 8; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+        uint32_t there = 0, there1 = 0;           // which of a stage's keys there are: of this stage, the next
+        uint32_t into = ring, from = ring;        // the slot that is filled, the slot that is worked on
+        auto on = [&](uint32_t slot) { return slot == ring + (kFewStages - 1) * Few<D>::stage ? ring : slot + Few<D>::stage; };
+        // Two stages ahead, in one loop and with little unrolled: of a short call the larger part of the time
+        // is the fetch of instructions that run once (one token at 1000, heads of 256: 15.8 us with the loop
+        // unrolled by stages, stalled on instructions three times as long as they took to issue).
 #pragma unroll 1
-        for (int i0 = 0; i0 < n; i0 += kFewStages) {
-#pragma unroll
-            for (int u = 0; u < kFewStages; u++) {
-                const int i = i0 + u;
-                if (i >= n) break;
-                there[(u + kFewStages - 1) % kFewStages] = copy(i + kFewStages - 1, (u + kFewStages - 1) % kFewStages);
-                cp_wait<kFewStages - 1>();
+        for (int i = 1 - kFewStages; i < n; i++) {
+            const uint32_t there2 = __ballot_sync(0xffffffffu, ahead[0].k >= 0);   // twice the same 16
+            if (i + kFewStages - 1 < n) {
                 __syncwarp();
-                const uint32_t ks = ring + u * Few<D>::stage, vs = ks + Few<D>::half;
-                float s[KW / 8][4] = {};
+                if (lane < KW) s_place[warp][lane] = ahead[0];
+                __syncwarp();
+                constexpr int ROUND = KW / RPI < 8 ? KW / RPI : 8;      // places that are loaded before they are used
+#pragma unroll 1
+                for (int e0 = 0; e0 < KW / RPI; e0 += ROUND) {
+                    Place pl[ROUND];
+#pragma unroll
+                    for (int e = 0; e < ROUND; e++) pl[e] = s_place[warp][(e0 + e) * RPI + lane / CH];
+#pragma unroll
+                    for (int e = 0; e < ROUND; e++) {
+                        const int r = (e0 + e) * RPI + lane / CH, c = lane % CH;
+                        const bool is = pl[e].k >= 0;
+                        cp16(into + few_at<D>(r, c), k_base + (is ? pl[e].k : 0) + c * 16, is);
+                        cp16(into + Few<D>::half + few_at<D>(r, c), v_base + (is ? pl[e].v : 0) + c * 16, is);
+                    }
+                }
+            }
+            cp_commit();
+            into = on(into);
+#pragma unroll
+            for (int e = 0; e + 1 < kFewStages; e++) ahead[e] = ahead[e + 1];
+            ahead[kFewStages - 1] = find(i + 2 * kFewStages - 1);
+            if (i >= 0) {
+                cp_wait<kFewStages - 1>();
+                if (i == 0) {
+                    __syncthreads();              // the rows, which all warps brought
+                    if (HOLD)
+#pragma unroll
+                        for (int k = 0; k < D / 16; k++) ldm4(qs + few_at<D>(lane & 15, 2 * k + (lane >> 4)), qf[k % (HOLD ? D / 16 : 1)]);
+                }
+                __syncwarp();
+                const uint32_t ks = from, vs = ks + Few<D>::half;
+                // (two sums of every other 16 values each: half the chain of products that wait for one another)
+                float s[KW / 8][4] = {}, s_odd[KW / 8][4] = {};
 #pragma unroll
                 for (int k = 0; k < D / 16; k++) {
                     uint32_t again[4];
@@ -150,26 +215,26 @@ __global__ void __launch_bounds__(kFewThreads, D == 256 ? 1 : 2) attend_few_kern
                     for (int t = 0; t < KW / 16; t++) {
                         uint32_t b[4];
                         ldm4(ks + few_at<D>(16 * t + (lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1)), b);
-                        mma16<T>(s[2 * t], qk, b[0], b[1]);
-                        mma16<T>(s[2 * t + 1], qk, b[2], b[3]);
+                        mma16<T>(k & 1 ? s_odd[2 * t] : s[2 * t], qk, b[0], b[1]);
+                        mma16<T>(k & 1 ? s_odd[2 * t + 1] : s[2 * t + 1], qk, b[2], b[3]);
                     }
                 }
                 const int j0 = x.tiles.tile(x.i0 + i) * KT + warp * KW;
                 // most stages lie where all rows see all keys: no comparison by key
-                const bool all = there[u] == 0xffffffffu && j0 + KW - 1 <= p_first &&
+                const bool all = there == 0xffffffffu && j0 + KW - 1 <= p_first &&
                                  (a.window <= 0 || p_top - j0 < a.window || j0 + KW <= a.sinks);
                 float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
                 for (int t = 0; t < KW / 8; t++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) s[t][e] *= a.scale_log2;
+                    for (int e = 0; e < 4; e++) s[t][e] = (s[t][e] + s_odd[t][e]) * a.scale_log2;
                 if (!all)
 #pragma unroll
                     for (int t = 0; t < KW / 8; t++)
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
                             const int r = t * 8 + quad * 2 + (e & 1);
-                            if (!(there[u] >> r & 1) || !sees(a, p[e >> 1], j0 + r)) s[t][e] = -INFINITY;
+                            if (!(there >> r & 1) || !sees(a, p[e >> 1], j0 + r)) s[t][e] = -INFINITY;
                         }
 #pragma unroll
                 for (int t = 0; t < KW / 8; t++)
@@ -213,7 +278,10 @@ __global__ void __launch_bounds__(kFewThreads, D == 256 ? 1 : 2) attend_few_kern
                     }
                 }
                 __syncwarp();
+                from = on(from);
             }
+            there = there1;
+            there1 = there2;
         }
         cp_wait<0>();
         // the four warps' o, maxima and sums through shared memory: [16][D] f32 in the warp's own ring
@@ -228,7 +296,7 @@ __global__ void __launch_bounds__(kFewThreads, D == 256 ? 1 : 2) attend_few_kern
 #pragma unroll
         for (int c = 0; c < D / 8; c++)
 #pragma unroll
-            for (int e = 0; e < 2; e++) *(float2*)(om + (g + 8 * e) * D + 8 * c + 2 * quad) = make_float2(o[c][2 * e], o[c][2 * e + 1]);
+            for (int e = 0; e < 2; e++) *(float2*)(om + (g + 8 * e) * Few<D>::part + 8 * c + 2 * quad) = make_float2(o[c][2 * e], o[c][2 * e + 1]);
         if (tid < 16) s_bad[tid] = 0;
         __syncthreads();
         // eight threads to a row, 4 values at a time
@@ -246,7 +314,7 @@ __global__ void __launch_bounds__(kFewThreads, D == 256 ? 1 : 2) attend_few_kern
             float4 v = make_float4(0, 0, 0, 0);
 #pragma unroll
             for (int w = 0; w < kFewWarps; w++) {
-                const float4 z = *(const float4*)(sm + w * kFewStages * Few<D>::stage + (row * D + sub * 4 + 32 * i) * 4);
+                const float4 z = *(const float4*)(sm + w * kFewStages * Few<D>::stage + (row * Few<D>::part + sub * 4 + 32 * i) * 4);
                 if (f[w] != 0.0f) { v.x += z.x * f[w]; v.y += z.y * f[w]; v.z += z.z * f[w]; v.w += z.w * f[w]; }
             }
             y[i] = v;
@@ -269,42 +337,25 @@ __global__ void __launch_bounds__(kFewThreads, D == 256 ? 1 : 2) attend_few_kern
                 for (int i = 0; i < D / 32; i++) y[i] = *(const float4*)(sm + (row * D + sub * 4 + 32 * i) * 4);
             }
         }
-        bool write = true;
         if (x.parts > 1) {
             const int mine = x.slot(x.part);
             float* po = a.part_o + ((int64_t)mine * kFewRows + row) * D + sub * 4;
             for (int i = 0; i < D / 32; i++) __stcg((float4*)(po + 32 * i), y[i]);
             if (sub == 0) __stcg(a.part_ml + (int64_t)mine * kFewRows + row, make_float2(M, L));
-            __threadfence();
             __syncthreads();
             if (tid == 0) {
-                s_last = atomicAdd(a.arrived + x.c0, 1) == x.parts - 1;
+                // releases what the block has written (it met at the barrier), acquires what the others have
+                int before;
+                asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(before) : "l"(a.arrived + x.c0) : "memory");
+                s_last = before == x.parts - 1;
                 if (s_last) a.arrived[x.c0] = 0;
             }
             __syncthreads();
-            write = s_last;
-            if (write) {
-                __threadfence();
-                M = -INFINITY;
-                L = 0.0f;
-                for (int s = 0; s < x.parts; s++) M = fmaxf(M, __ldcg(a.part_ml + (int64_t)x.slot(s) * kFewRows + row).x);
-#pragma unroll
-                for (int i = 0; i < D / 32; i++) y[i] = make_float4(0, 0, 0, 0);
-                for (int s = 0; s < x.parts; s++) {
-                    const float2 ml = __ldcg(a.part_ml + (int64_t)x.slot(s) * kFewRows + row);
-                    // a NaN part has a finite maximum, or none, and a sum that is one
-                    const float e = ml.x == -INFINITY && ml.y == 0.0f ? 0.0f : ml.x == -INFINITY ? 1.0f : exp2_of(ml.x - M);
-                    const float* z = a.part_o + ((int64_t)x.slot(s) * kFewRows + row) * D + sub * 4;
-                    L += ml.y * e;
-#pragma unroll
-                    for (int i = 0; i < D / 32; i++) {
-                        const float4 v = __ldcg((const float4*)(z + 32 * i));
-                        if (e != 0.0f) { y[i].x += v.x * e; y[i].y += v.y * e; y[i].z += v.z * e; y[i].w += v.w * e; }
-                    }
-                }
-            }
+            if (!s_last) continue;
+            join<D, T>(a, x);
+            continue;
         }
-        if (write && row < x.rows) {
+        if (row < x.rows) {
             const int R = x.row0 + row, tok = (int)a.group.div(R), h = x.head * (int)a.group.d + R - tok * (int)a.group.d;
             T* out = (T*)(a.out + (int64_t)(x.r.begin + tok) * a.out_token + (int64_t)h * a.out_head) + sub * 4;
             const float by = L == 0.0f ? 0.0f : 1.0f / L;
@@ -319,7 +370,7 @@ template <int D, class T> static cudaError_t few(const AttendCall& a, int sm_cou
     static std::atomic<uint64_t> attr_set{0};
     if (cudaError_t e = ensure_dynamic_smem(attend_few_kernel<D, T>, (int)(Few<D>::fixed + share_smem(kCacheSeqs, kFewThreads)), attr_set)) return e;
     count_launch();
-    return launch_with(false, stream, attend_few_kernel<D, T>, dim3(sm_count * (D == 256 ? 1 : kFewBlocks)), dim3(kFewThreads), smem, a);
+    return launch_with(false, stream, attend_few_kernel<D, T>, dim3(sm_count * few_blocks(D)), dim3(kFewThreads), smem, a);
 }
 template <int D> static cudaError_t few_as(const AttendCall& a, int ggml_type, int sm_count, cudaStream_t stream) {
     return ggml_type == BIVMOE_F16 ? few<D, __half>(a, sm_count, stream) : few<D, __nv_bfloat16>(a, sm_count, stream);

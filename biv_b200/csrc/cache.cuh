@@ -98,6 +98,10 @@ template <int KT> __device__ __forceinline__ TileList tiles_of(const AttendCall&
     t.n = t.ns + last - t.from + 1;
     return t;
 }
+// whether some row from p0 to p1 sees key j
+__device__ __forceinline__ bool seen(const AttendCall& a, int p0, int p1, int j) {
+    return j <= p1 && (a.window <= 0 || j > p0 - a.window || j < a.sinks);
+}
 __device__ __forceinline__ bool sees(const AttendCall& a, int p, int j) {
     return j <= p && (a.window <= 0 || p - j < a.window || j < a.sinks);
 }
@@ -119,12 +123,18 @@ __device__ __forceinline__ int page_of(const AttendCall& a, const int32_t* row, 
 // the blocks end together whatever the lengths are, and a block has at most two pieces of tiles
 // that others share, so that the room for pieces is two to a block.  Every block finds its share by
 // itself from the lengths: no list in memory, no launch before.
+// a / b for a >= 0, b > 0; most are short
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+    return (a | b) >> 31 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
+}
 struct Share {
-    int64_t total, lo, hi;           // units of the call, of this block
-    int g;
+    int64_t lo, hi;                  // this block's units
+    int64_t each, longer;            // units of a block; those of the first blocks, which have one more
     const int64_t* before;           // shared, [n_seq + 1]: units of the requests before
-    // the block that has unit u: the last c with total * c / g <= u
-    __device__ __forceinline__ int owner(int64_t u) const { return (int)(((u + 1) * g - 1) / total); }
+    // the block that has unit u
+    __device__ __forceinline__ int owner(int64_t u) const {
+        return u < longer ? (int)quotient(u, each + 1) : (int)(quotient(longer, each + 1) + quotient(u - longer, each));
+    }
 };
 template <int KT, int TR> __device__ __forceinline__ TileList tile_list(const AttendCall& a, const Request& r, int t) {
     return tiles_of<KT>(a, r.past + (int)a.group.div(t * TR), r.past + (int)a.group.div(min((t + 1) * TR, r.rows) - 1));
@@ -177,14 +187,16 @@ __device__ __forceinline__ Share find_share(const AttendCall& a, int least, int6
     if (tid == 0) before[a.n_seq] = carry;
     __syncthreads();
     Share s;
-    s.total = carry;
     s.before = before;
-    const int64_t worth = (carry + least - 1) / least;
-    s.g = (int)(worth < gridDim.x ? worth : gridDim.x);
-    s.lo = s.hi = 0;
-    if ((int)blockIdx.x < s.g) {
-        s.lo = carry * blockIdx.x / s.g;
-        s.hi = carry * (blockIdx.x + 1) / s.g;
+    const int64_t worth = quotient(carry + least - 1, least);
+    const int g = (int)(worth < gridDim.x ? worth : gridDim.x);
+    s.lo = s.hi = s.each = s.longer = 0;
+    if ((int)blockIdx.x < g) {
+        s.each = quotient(carry, g);
+        const int more = (int)(carry - s.each * g), c = (int)blockIdx.x;
+        s.longer = more * (s.each + 1);
+        s.lo = s.each * c + min(c, more);
+        s.hi = s.lo + s.each + (c < more);
     }
     return s;
 }
@@ -214,8 +226,8 @@ template <int KT, int TR, int EXTRA> struct Walk {
             if (s.before[mid] <= at) lo = mid; else hi = mid;
         }
         open(lo);
-        const int64_t rest = at - s.before[b], each = (s.before[b + 1] - s.before[b]) / a.heads_kv;
-        head = (int)(rest / each);
+        const int64_t rest = at - s.before[b], each = quotient(s.before[b + 1] - s.before[b], a.heads_kv);
+        head = (int)quotient(rest, each);
         int64_t in = rest - head * each;
         const int lane = threadIdx.x & 31;
         for (t = 0; nt > 1 && t < nt;) {   // the tile: 32 of them at a time
@@ -357,7 +369,8 @@ cudaError_t launch_extend(const bivmoe_extend_args& a, int page_size, int sm_cou
 cudaError_t launch_store(const bivmoe_store_args& a, const RopePlan& rope, int ggml_type, int heads, int heads_kv, int head_dim,
                          int page_size, int sm_count, cudaStream_t stream);
 // what the workspace is sized for: rows of a tile, blocks to a multiprocessor
-constexpr int kFewRows = 16, kFewBlocks = 2;
+constexpr int kFewRows = 16;
+constexpr int few_blocks(int head_dim) { return head_dim == 256 ? 1 : head_dim == 128 ? 2 : 3; }
 constexpr int tc_rows(int head_dim) { return head_dim == 256 ? 128 : 256; }
 
 }  // namespace bivmoe

@@ -112,7 +112,7 @@ extern "C" int bivmoe_cache_create(const bivmoe_cache_desc* d, bivmoe_cache** ou
     c->d = *d;
     c->sm_count = sms;
     // pieces: at most two to a block (cache.cuh)
-    const size_t few = 2 * (size_t)kFewBlocks * c->sm_count * kFewRows, tc = 2 * (size_t)c->sm_count * tc_rows(d->head_dim),
+    const size_t few = 2 * (size_t)few_blocks(d->head_dim) * c->sm_count * kFewRows, tc = 2 * (size_t)c->sm_count * tc_rows(d->head_dim),
                  rows = few > tc ? few : tc, counts = 8 * (size_t)c->sm_count;
     size_t off = 0;
     auto take = [&off](size_t bytes) { const size_t at = off; off += (bytes + 255) & ~(size_t)255; return at; };
