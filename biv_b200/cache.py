@@ -15,20 +15,19 @@ the current torch stream, waits for nothing and can be captured into a graph.
 from __future__ import annotations
 
 import ctypes as C
-import math
-import struct
 from typing import NamedTuple, Optional, Sequence
 
 import torch
 
 from . import capi
 
-# bivmoe_extend_args, bivmoe_store_args and bivmoe_attend_args field by field (native order, C's alignment)
-_ROWS, _POOL = "Pqqii", "Pqqqq"
-_EXTEND = struct.Struct("6Pq4i6P").pack_into
-_STORE = struct.Struct(_ROWS * 4 + _POOL * 2 + "2Pq2i").pack_into
-_ATTEND = struct.Struct(_ROWS * 2 + _POOL * 2 + "Pq4i2Pf3i").pack_into
-_GGML = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
+try:
+    from . import _cache_calls
+except ImportError as e:
+    raise ImportError("biv_b200/_cache_calls.so is missing or was built for another torch: build it with `python -c "
+                      "'import __graft_entry__ as g; g.build()'` (or `make -C biv_b200/csrc`); there is no fallback") from e
+
+_GGML = {torch.float16: 1, torch.bfloat16: 30}
 
 
 class Rope:
@@ -78,25 +77,16 @@ class PagedCache:
         self._h = h
         self.n_head, self.n_head_kv, self.head_dim, self.page_size = n_head, n_head_kv, head_dim, page_size
         self.max_seqs, self.max_tokens, self.dtype, self.rope, self.device = max_seqs, max_tokens, dtype, rope, device
-        self._set_up(torch.device("cuda", device))
-
-    def _set_up(self, dev):
-        self._dev = dev
+        # the calls go through a small extension module (checks, outputs, argument structs), by these addresses
         L = capi.lib()
-        self._calls = L.bivmoe_cache_extend, L.bivmoe_cache_store, L.bivmoe_cache_attend
-        self._scale = 1.0 / math.sqrt(self.head_dim)
-        # A call's arguments are packed anew for every launch, into a buffer of the struct's size; a step
-        # of small kernels is bound by the host, so one pack and few attribute look-ups.
-        self._bufs = [C.create_string_buffer(C.sizeof(t)) for t in (capi.ExtendArgs, capi.StoreArgs, capi.AttendArgs)]
-        self._refs = [C.cast(b, C.POINTER(t)) for b, t in zip(self._bufs, (capi.ExtendArgs, capi.StoreArgs, capi.AttendArgs))]
-        self._ggml = _GGML[self.dtype]
-        self._pool_shape = (self.page_size, self.n_head_kv, self.head_dim)
-        self._axes = len(self.rope.sections) if self.rope is not None else 0
+        at = [C.cast(f, C.c_void_p).value for f in (L.bivmoe_cache_extend, L.bivmoe_cache_store, L.bivmoe_cache_attend)]
+        self._geometry = _cache_calls.make(h.value, *at, device, n_head, n_head_kv, head_dim, page_size, _GGML[dtype],
+                                           len(rope.sections) if rope is not None else 0)
 
     def close(self):
         if self._h is not None:
             capi.lib().bivmoe_cache_destroy(self._h)
-            self._h = None
+            self._h = self._geometry = None
 
     def __del__(self):
         try:
@@ -104,52 +94,10 @@ class PagedCache:
         except Exception:
             pass
 
-    def _call(self, i, pack, *values):
-        pack(self._bufs[i], 0, *values)
-        code = self._calls[i](self._h, self._refs[i], torch.cuda.current_stream(self._dev).cuda_stream)
-        if code:
-            capi.check(code)
-
-    def _ints(self, t, what, n, dtype=torch.int32):
-        if t.dtype is not dtype or t.device != self._dev or not t.is_contiguous() or t.numel() < n:
-            raise ValueError(f"{what}: {n} contiguous {dtype} on {self._dev} are wanted")
-        return t.data_ptr()
-
     def pools(self, n_pages: int):
         """A layer's k and v pools."""
         shape = (n_pages, self.page_size, self.n_head_kv, self.head_dim)
-        return tuple(torch.empty(shape, dtype=self.dtype, device=self._dev) for _ in range(2))
-
-    def _table(self, t, n_seq):
-        """address, stride, width"""
-        if t.dtype is not torch.int32 or t.device != self._dev or t.dim() != 2:
-            raise ValueError("table: [n_seq, pages] int32 is wanted")
-        rows, width = t.shape
-        stride, one = t.stride()
-        if rows < n_seq or (width > 1 and one != 1):
-            raise ValueError("table: [n_seq, pages] with neighbouring pages is wanted")
-        return t.data_ptr(), stride, width
-
-    def _pool(self, t, name):
-        """address, strides of a page, a token and a head, pages: a ``bivmoe_pool``"""
-        shape, stride = t.shape, t.stride()
-        if t.dtype is not self.dtype or t.device != self._dev or shape[1:] != self._pool_shape or stride[3] != 1:
-            raise ValueError(f"{name}: [pages, {self.page_size}, {self.n_head_kv}, {self.head_dim}] of {self.dtype} is wanted")
-        return t.data_ptr(), stride[0], stride[1], stride[2], shape[0]
-
-    def _rows(self, t, what, heads, n):
-        """address, strides of a token and a head"""
-        stride = t.stride()
-        if t.shape != (n, heads, self.head_dim) or stride[2] != 1 or t.device != self._dev:
-            raise ValueError(f"{what}: [tokens, {heads}, {self.head_dim}] rows on {self._dev} are wanted")
-        return t.data_ptr(), stride[0], stride[1]
-
-    def _out(self, out, q):
-        if out is None:
-            return torch.empty_like(q, dtype=self.dtype)
-        if out.dtype is not self.dtype:
-            raise ValueError(f"out: {self.dtype} is wanted")
-        return out
+        return tuple(torch.empty(shape, dtype=self.dtype, device=f"cuda:{self.device}") for _ in range(2))
 
     def extend(self, past, added, free_pages, free_count, table, n_tokens: int, held=None, out: Optional[Step] = None) -> Step:
         """Pages for ``added[b]`` new tokens of each request b, which has ``past[b]`` (int32 device
@@ -158,41 +106,19 @@ class PagedCache:
         more than the requests add (a padded batch) have slot -1.  ``held``: pages each request holds
         already, where that is not what ``past`` needs (drafted tokens that were taken back); ``out``:
         a step to write into."""
-        n_seq = past.numel()
-        if out is None:
-            room = torch.empty(3 * n_seq + 3 + n_tokens, dtype=torch.int32, device=self._dev)
-            length, first, left, kept, positions = room.split((n_seq, n_seq + 1, 2, n_seq, n_tokens))
-            out = Step(length, first, torch.empty(n_tokens, dtype=torch.int64, device=self._dev), positions, left, kept)
-            wrote = [t.data_ptr() for t in (length, first, positions, left, kept, out.slots)]
-        else:
-            wrote = [self._ints(out.length, "length", n_seq), self._ints(out.first, "first", n_seq + 1),
-                     self._ints(out.positions, "positions", n_tokens), self._ints(out.left, "left", 2),
-                     self._ints(out.held, "held", n_seq), self._ints(out.slots, "slots", n_tokens, torch.int64)]
-        self._call(0, _EXTEND, self._ints(past, "past", n_seq), self._ints(added, "added", n_seq),
-                   0 if held is None else self._ints(held, "held", n_seq), self._ints(free_pages, "free_pages", 0),
-                   self._ints(free_count, "free_count", 1), *self._table(table, n_seq), free_pages.numel(), n_seq, n_tokens, *wrote)
-        return out
+        r = _cache_calls.extend(self._geometry, past, added, held, free_pages, free_count, table, n_tokens, out)
+        if r.__class__ is int:
+            capi.check(r)
+        return r if out is not None else Step._make(r)
 
     def store(self, q, k, v, k_pool, v_pool, slots, positions=None, out=None):
         """q and k [n, heads, head_dim] (float32, float16 or bfloat16; any strides of the first two)
         turned by ``positions`` ([n], or [axes, n]), k and v into the pages at ``slots``; returns the
         turned q in the cache's type."""
-        n, ty = q.shape[0], _GGML.get(q.dtype)
-        if ty is None or k.dtype is not q.dtype or v.dtype is not q.dtype:
-            raise ValueError("q, k and v: rows of one type, float32, float16 or bfloat16, are wanted")
-        out = self._out(out, q)
-        where, stride = 0, 0
-        if self._axes:
-            if positions is None or positions.dtype is not torch.int32 or positions.device != self._dev or \
-                    positions.numel() != self._axes * n or (n > 1 and positions.stride(-1) != 1):
-                raise ValueError(f"positions: [{self._axes}, n] int32 are wanted" if self._axes > 1 else "positions: [n] int32 are wanted")
-            where, stride = positions.data_ptr(), positions.stride(0) if positions.dim() > 1 else n
-        kv = self.n_head_kv
-        self._call(1, _STORE, *self._rows(q, "q", self.n_head, n), ty, 0, *self._rows(k, "k", kv, n), ty, 0,
-                   *self._rows(v, "v", kv, n), ty, 0, *self._rows(out, "out", self.n_head, n), self._ggml, 0,
-                   *self._pool(k_pool, "k_pool"), *self._pool(v_pool, "v_pool"),
-                   self._ints(slots, "slots", n, torch.int64), where, stride, n, 0)
-        return out
+        r = _cache_calls.store(self._geometry, q, k, v, k_pool, v_pool, slots, positions, out)
+        if r.__class__ is int:
+            capi.check(r)
+        return r
 
     def attend(self, q, k_pool, v_pool, table, first, length, max_new: int = 0, scale: Optional[float] = None,
                window: int = 0, sinks: int = 0, out=None):
@@ -200,17 +126,12 @@ class PagedCache:
         the last tokens of its length[b] tokens.  A token at position p sees p and what is before it;
         with ``window`` the last ``window`` positions up to its own and the first ``sinks``.  ``max_new``:
         the most new rows of a request, where the caller knows it."""
-        n, n_seq = q.shape[0], length.numel()
-        if q.dtype is not self.dtype:
-            raise ValueError(f"q: {self.dtype} is wanted")
-        out = self._out(out, q)
-        self._call(2, _ATTEND, *self._rows(q, "q", self.n_head, n), self._ggml, 0, *self._rows(out, "out", self.n_head, n), self._ggml, 0,
-                   *self._pool(k_pool, "k_pool"), *self._pool(v_pool, "v_pool"), *self._table(table, n_seq), n_seq, n, max_new,
-                   self._ints(first, "first", n_seq + 1), self._ints(length, "length", n_seq),
-                   self._scale if scale is None else scale, window, sinks, 0)
-        return out
+        r = _cache_calls.attend(self._geometry, q, k_pool, v_pool, table, first, length, max_new, scale, window, sinks, out)
+        if r.__class__ is int:
+            capi.check(r)
+        return r
 
     def status(self):
         """Waits for the current stream and raises if a kernel of this cache gave up on a bounded wait
         since the last report."""
-        capi.check(capi.lib().bivmoe_cache_status(self._h, torch.cuda.current_stream(self._dev).cuda_stream))
+        capi.check(capi.lib().bivmoe_cache_status(self._h, torch.cuda.current_stream(self.device).cuda_stream))

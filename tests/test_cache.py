@@ -36,12 +36,6 @@ def test_argument_structs_have_the_header_s_sizes(tmp_path):
     subprocess.run(["gcc", "-std=c99", "-Wall", "-Werror", "-I", os.path.join(ROOT, "include"), str(src), "-o", exe], check=True)
     got = [int(v) for v in subprocess.run([exe], check=True, capture_output=True, text=True).stdout.split()]
     assert got == [C.sizeof(t) for t in (capi.CacheDesc, capi.ExtendArgs, capi.StoreArgs, capi.AttendArgs)]
-    from biv_b200 import cache as K
-    for pack, t in ((K._EXTEND, capi.ExtendArgs), (K._STORE, capi.StoreArgs), (K._ATTEND, capi.AttendArgs)):
-        fields = [f for f, _ in t._fields_]        # what is packed is the struct, field by field
-        a = t()
-        pack.__self__.pack_into(a, 0, *range(1, len(fields) + 1))
-        assert pack.__self__.size == C.sizeof(t) and [getattr(a, f) for f in fields] == list(range(1, len(fields) + 1))
 
 
 def test_null_arguments_are_refused():
