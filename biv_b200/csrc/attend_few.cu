@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(D)) attend_few_kernel(
     const int g = lane >> 2, quad = lane & 3;
     constexpr int CH = D / 8, RPI = 32 / CH;      // 16-byte pieces of a row, rows of a warp's copy
 
-    Walk<KT, kFewRows, kFewExtra> walk(a, share);
+    Walk<KT, kFewRows, kFewExtra, kFewExtra> walk(a, share);
     for (Piece x; walk.next(x);) {
         __syncthreads();                          // the piece before is done with the rings and the rows
         const int32_t* table = a.table + (int64_t)x.b * a.table_stride;

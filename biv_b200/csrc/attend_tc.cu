@@ -54,6 +54,7 @@ template <int D> struct At {
     static constexpr int rows = 128 * tiles;
     static constexpr int chunks = D / 64;                    // slots of a tile of K, or of V
     static constexpr int extra = D == 256 ? 4 : 3;           // key tiles that a tile costs besides
+    static constexpr int snap = D == 256 ? 6 : 5;            // key tiles that are not worth a cut
     static constexpr int q_tile = 128 * D * 2;
     static constexpr int fixed = AT_HEAD + tiles * q_tile + AT_SLOTS * AT_SLOT + (int)sizeof(AtPlaces) * AT_PAGES;
 };
@@ -81,11 +82,20 @@ static_assert(sizeof(AtHead) <= AT_HEAD && offsetof(AtHead, there) % 16 == 0, ""
 // Each role's registers are dealt out in its own branch: where branches meet, the compiler reckons with
 // the fewest.
 __device__ __forceinline__ void at_fewer_regs() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(AT_OTHER_REGS)); }
+// Every role's waits look at the clock, once in 64 tries that found nothing: a role that ends early does not
+// leave the others without one that gives up.
 __device__ __forceinline__ bool at_wait(uint64_t* bar, uint32_t parity, const int* abort) {
-    return bounded_wait<256>(PfWait<false, false>{bar, parity, abort});
+    return bounded_wait<64>(PfWait<true, false>{bar, parity, abort});
 }
 __device__ __forceinline__ bool at_wait_warp(uint64_t* bar, uint32_t parity, const int* abort) {
-    return bounded_wait_together<256>(PfWait<false, false>{bar, parity, abort});
+    return bounded_wait_together<64>(PfWait<true, false>{bar, parity, abort});
+}
+// One lane's arrival for its warp, which is together again after it: what follows may be an instruction that
+// a whole warp has to execute at once (tcgen05.ld, .st), and a branch that one lane takes does not by
+// itself end together.
+__device__ __forceinline__ void at_arrive(uint64_t* bar) {
+    if ((threadIdx.x & 31) == 0) pf_bar_arrive(bar);
+    __syncwarp();
 }
 __device__ __forceinline__ void at_cp16(uint32_t dst, const void* src, bool there) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
@@ -200,7 +210,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(const __grid_c
             *(volatile int*)&H.abort = 1;
         }
     };
-    Walk<AT_KEYS, TR, At<D>::extra> walk(a, share);
+    Walk<AT_KEYS, TR, At<D>::extra, At<D>::snap> walk(a, share);
 
     if (warp == AT_PAGE_WARP) {
         at_fewer_regs();
@@ -231,7 +241,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(const __grid_c
                         known[i] = __ballot_sync(0xffffffffu, page[i] >= 0 || key > p_top);
                     }
                 }
-                if (!bounded_wait_together<256>(PfWait<true, true>{&H.page_empty[e], ((ktile / AT_PAGES) & 1) ^ 1, &H.abort})) {
+                if (!bounded_wait_together<64>(PfWait<true, true>{&H.page_empty[e], ((ktile / AT_PAGES) & 1) ^ 1, &H.abort})) {
                     give_up(AT_SITE_PAGES);
                     ok = false;
                     break;
@@ -247,7 +257,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(const __grid_c
                 if (lane == 0) H.boxes[e] = boxes ? AT_KEYS / maps.rows : 0;
                 if (lane == 0) *(uint4*)H.there[ktile & 15] = make_uint4(known[0], known[1], known[2], known[3]);
                 __syncwarp();
-                if (lane == 0) pf_bar_arrive(&H.page_full[e]);
+                at_arrive(&H.page_full[e]);
             }
         }
     } else if (warp >= AT_COPY_WARP) {
@@ -264,8 +274,8 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(const __grid_c
                 const AtTurn turn = at_turn(i / CH, n, pair);
                 const int c = i % CH;
                 const uint32_t kt = ktile + turn.j;
-                if (!bounded_wait_together<256>(PfWait<true, true>{&H.page_full[kt % AT_PAGES], (kt / AT_PAGES) & 1, &H.abort}) ||
-                    !bounded_wait_together<256>(PfWait<true, true>{&H.empty[slot], ((gs / AT_SLOTS) & 1) ^ 1, &H.abort})) {
+                if (!bounded_wait_together<64>(PfWait<true, true>{&H.page_full[kt % AT_PAGES], (kt / AT_PAGES) & 1, &H.abort}) ||
+                    !bounded_wait_together<64>(PfWait<true, true>{&H.empty[slot], ((gs / AT_SLOTS) & 1) ^ 1, &H.abort})) {
                     give_up(AT_SITE_COPY);
                     ok = false;
                     break;
@@ -279,7 +289,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(const __grid_c
                                x.head, pl.page[lane], &H.full[slot]);
                     if (lane) pf_bar_arrive(&H.full[slot]);
                     __syncwarp();
-                    if (lane == 0) pf_bar_arrive(&H.page_empty[kt % AT_PAGES]);
+                    at_arrive(&H.page_empty[kt % AT_PAGES]);
                     continue;
                 }
                 const int64_t* place = turn.v ? pl.v : pl.k;
@@ -300,7 +310,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(const __grid_c
                 }
                 at_cp_arrive(&H.full[slot]);
                 __syncwarp();
-                if (lane == 0) pf_bar_arrive(&H.page_empty[kt % AT_PAGES]);
+                at_arrive(&H.page_empty[kt % AT_PAGES]);
             }
             base += total;
             ktile += n;
@@ -449,7 +459,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(const __grid_c
                 asm volatile("cp.async.wait_all;" ::: "memory");
                 at_fence_async();
                 __syncwarp();
-                if (lane == 0) pf_bar_arrive(&H.q_full[t]);
+                at_arrive(&H.q_full[t]);
             }
             for (int j = 0; j < n; j++) {
                 const int s = pair ? t : 2 + (j & 1);
@@ -531,7 +541,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(const __grid_c
                             if (!before()) { ok = false; break; }
                             pf_fence_before();
                             __syncwarp();
-                            if (lane == 0) pf_bar_arrive(&H.p_half[s]);
+                            at_arrive(&H.p_half[s]);
                         }
                     }
                     if (!ok) break;
@@ -541,11 +551,11 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(const __grid_c
                 } else {
                     if (!before()) { ok = false; break; }
                     __syncwarp();
-                    if (lane == 0) pf_bar_arrive(&H.p_half[s]);
+                    at_arrive(&H.p_half[s]);
                 }
                 pf_fence_before();
                 __syncwarp();
-                if (lane == 0) pf_bar_arrive(&H.p_full[s]);
+                at_arrive(&H.p_full[s]);
             }
             if (!ok) { give_up(AT_SITE_ROWS); break; }
             ktile += n;

@@ -212,11 +212,14 @@ struct Piece {
     __device__ __forceinline__ int slot(int p) const { return p == 0 ? 2 * c0 + 1 : 2 * (c0 + p); }
 };
 // The pieces of a block's share, one after another: every warp goes through them by itself.
-template <int KT, int TR, int EXTRA> struct Walk {
+// A share's end that lies at most SNAP units behind a tile's beginning, or before its end, is moved there:
+// a tile that is cut costs its unfinished sums' way out and in (SNAP >= EXTRA: no piece is without keys).
+template <int KT, int TR, int EXTRA, int SNAP> struct Walk {
+    static_assert(SNAP >= EXTRA, "");
     const AttendCall& a;
     const Share& s;
     int64_t at;                      // the next unit
-    int b, head, t, nt, off;         // where it lies
+    int b, head, t, nt, off;         // where it lies: of which tile, and how far in
     Request r;
     __device__ __forceinline__ Walk(const AttendCall& call, const Share& share) : a(call), s(share), at(share.lo) {
         if (at >= s.hi) return;
@@ -248,54 +251,66 @@ template <int KT, int TR, int EXTRA> struct Walk {
             t += 32;
         }
         off = (int)in;
+        const int units = tile_units<KT, TR, EXTRA>(a, r, t);
+        if (off <= SNAP) {
+            at -= off;
+            off = 0;
+        } else if (units - off <= SNAP) {
+            at += units - off;
+            step();
+        }
     }
     __device__ __forceinline__ void open(int request) {
         b = request;
         r = request_of(a, b);
         nt = (r.rows + TR - 1) / TR;
     }
-    // The next piece; false at the share's end.  What the share has of a tile's EXTRA units alone is no piece.
+    // to the beginning of the tile that follows, at `at`
+    __device__ __forceinline__ void step() {
+        off = 0;
+        if (++t < nt) return;
+        t = 0;
+        if (++head < a.heads_kv) return;
+        head = 0;
+        if (at >= s.before[a.n_seq]) return;
+        int next = b + 1;
+        while (s.before[next + 1] == s.before[next]) next++;   // those without rows
+        open(next);
+    }
+    // The next piece; false at the share's end.
     __device__ __forceinline__ bool next(Piece& x) {
-        for (;;) {
-            if (at >= s.hi) return false;
-            x.tiles = tile_list<KT, TR>(a, r, t);
-            const int units = EXTRA + max(x.tiles.n, 1), take = (int)min((int64_t)(units - off), s.hi - at), end = off + take;
-            const bool some = end > EXTRA;
-            if (some) {
-                x.b = b;
-                x.head = head;
-                x.r = r;
-                x.row0 = t * TR;
-                x.rows = min(TR, r.rows - x.row0);
-                x.i0 = max(off - EXTRA, 0);
-                x.n = min(end - EXTRA, x.tiles.n) - x.i0;
-                x.part = 0;
-                x.parts = 1;
-                x.c0 = (int)blockIdx.x;
-                if (off > EXTRA || end < units) {
-                    x.c0 = s.owner(at - off + EXTRA);
-                    x.parts = s.owner(at - off + units - 1) - x.c0 + 1;
-                    x.part = (int)blockIdx.x - x.c0;
-                }
+        if (at >= s.hi) return false;
+        x.tiles = tile_list<KT, TR>(a, r, t);
+        const int units = EXTRA + max(x.tiles.n, 1);
+        const int64_t u0 = at - off;
+        int end = units;
+        if (s.hi - u0 < units) {
+            const int e = (int)(s.hi - u0);
+            if (e <= SNAP) {
+                at = s.hi;
+                return false;
             }
-            at += take;
-            off = end;
-            if (off == units) {
-                off = 0;
-                if (++t == nt) {
-                    t = 0;
-                    if (++head == a.heads_kv) {
-                        head = 0;
-                        if (at < s.hi) {
-                            int next = b + 1;
-                            while (s.before[next + 1] == s.before[next]) next++;   // those without rows
-                            open(next);
-                        }
-                    }
-                }
-            }
-            if (some) return true;
+            if (units - e > SNAP) end = e;
         }
+        x.b = b;
+        x.head = head;
+        x.r = r;
+        x.row0 = t * TR;
+        x.rows = min(TR, r.rows - x.row0);
+        x.i0 = max(off - EXTRA, 0);
+        x.n = min(end - EXTRA, x.tiles.n) - x.i0;
+        x.part = 0;
+        x.parts = 1;
+        x.c0 = (int)blockIdx.x;
+        if (off > 0 || end < units) {
+            x.c0 = s.owner(u0 + SNAP);
+            x.parts = s.owner(u0 + units - SNAP - 1) - x.c0 + 1;
+            x.part = (int)blockIdx.x - x.c0;
+        }
+        at = u0 + end;
+        off = end;
+        if (end == units) step();
+        return true;
     }
 };
 
