@@ -17,7 +17,7 @@
 namespace bivmoe {
 
 constexpr int kFewWarps = 4, kFewThreads = 32 * kFewWarps, kFewStages = 3;
-constexpr int kFewLeast = 2, kFewExtra = 3;   // key tiles that are worth a block; that a tile costs besides
+constexpr int kFewLeast = 2, kFewExtra = 1;   // key tiles that are worth a block; that a tile costs besides
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool there) {
     // nothing is read, and zeros are written, where there is nothing

@@ -266,10 +266,18 @@ extern "C" int bivmoe_cache_attend(bivmoe_cache* c, const bivmoe_attend_args* a,
     const cudaStream_t s = (cudaStream_t)stream;
     bool captured = false;
     cudaError_t e = take_turn(c, s, &captured);
-    // tiles of 16 rows where no request has more rows to a kv head; max_new is the caller's word, which
-    // decides the speed alone: both kernels take any number of rows
+    // Which kernel, by the most rows a request has to a kv head (max_new is the caller's word and decides the
+    // speed alone: both kernels take any number).  Up to 16 rows a tile of the first reads the keys once; up to
+    // 32 it reads them twice, mostly from L2, and still ends sooner unless heads of 256 have many requests.
+    // us, tiles of 16 rows / tcgen05 (heads_kv 4, 4 and 2; requests x tokens):
+    //   rows  heads of    1 x 300      8 x 1000     32 x 4000     4 x 20000
+    //    32      64      9.9 / 13.1  13.5 / 21.1   58.4 / 67.1   41.5 / 56.8
+    //    32     128     10.4 / 15.4  15.9 / 23.9   90.2 / 82.2   62.7 / 70.7
+    //    32     256     11.6 / 17.8  18.3 / 27.6  100.9 / 80.5   69.7 / 113.7
+    //    48     128     10.7 / 15.2  18.2 / 23.5  138.5 / 81.3   83.3 / 71.4
     const int most = a->max_new > 0 && a->max_new < a->n_tokens ? a->max_new : a->n_tokens;
-    const bool few = most <= kFewRows / (int)k.group.d;
+    const int64_t rows = (int64_t)most * k.group.d;
+    const bool few = rows <= 16 || (rows <= 32 && (c->d.head_dim <= 128 || (int64_t)a->n_seq * k.heads_kv <= 32));
     if (e == cudaSuccess)
         e = few ? launch_attend_few(k, c->d.head_dim, c->d.ggml_type, c->sm_count, s)
                 : launch_attend_tc(k, c->d.head_dim, c->d.ggml_type, c->sm_count, s);
