@@ -174,6 +174,15 @@ extern "C" int bivmoe_cache_extend(bivmoe_cache* c, const bivmoe_extend_args* a,
                           (const void*)a->left, (const void*)a->held_out})
         if (!aligned(p, 4)) return fail(BIVMOE_ERR_ARGUMENT, "a list of int32 is not aligned");
     if (!aligned(a->slots, 8)) return fail(BIVMOE_ERR_ARGUMENT, "slots: not aligned");
+    // the blocks read the lists while the first of them writes its own
+    const struct { const void* p; int64_t n; } in[] = {{a->past, a->n_seq}, {a->added, a->n_seq}, {a->held, a->n_seq}, {a->free_count, 1},
+                                                       {a->free_pages, a->n_free}, {a->table, a->n_seq ? (a->n_seq - 1) * a->table_stride + a->table_width : 0}},
+        out[] = {{a->length, a->n_seq}, {a->first, a->n_seq + 1}, {a->left, 2}, {a->held_out, a->n_seq}, {a->positions, a->n_tokens},
+                 {a->slots, 2 * (int64_t)a->n_tokens}};
+    for (const auto& i : in)
+        for (const auto& o : out)
+            if (i.p && o.p && (uintptr_t)i.p < (uintptr_t)o.p + 4 * o.n && (uintptr_t)o.p < (uintptr_t)i.p + 4 * i.n)
+                return fail(BIVMOE_ERR_ARGUMENT, "a list that is written lies over one that is read");
     DeviceScope on_device(c->d.device);
     const cudaError_t e = launch_extend(*a, c->d.page_size, c->sm_count, (cudaStream_t)stream);
     return e == cudaSuccess ? BIVMOE_OK : cuda_fail(e, "bivmoe_cache_extend");

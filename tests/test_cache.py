@@ -132,6 +132,18 @@ def test_extend(seqs, page, most, spare, pad, use_held):
 
 
 @pytest.mark.gpu
+def test_extend_into_its_own_lists_is_refused():
+    c = cache(page=4, seqs=2, tokens=4)
+    table, past, count = torch.full((2, 2), -1, dtype=torch.int32, device=DEV), ints([0, 0]), ints([3])
+    s = c.extend(past, ints([1, 1]), ints([7, 8, 9]), count, table, 2)
+    cases = [(count, s._replace(length=past)), (count, s._replace(held=past)), (count, s._replace(first=table.view(-1))), (s.left[1:], s)]
+    for free_count, bad in cases:
+        with pytest.raises(capi.BivMoeError) as e:
+            c.extend(past, ints([1, 1]), ints([7, 8, 9]), free_count, table, 2, out=bad)
+        assert e.value.code == capi.ERR_ARGUMENT
+
+
+@pytest.mark.gpu
 def test_extend_of_lists_that_do_not_fit():
     c = cache(page=4, seqs=4, tokens=16)
     table = torch.full((3, 2), -1, dtype=torch.int32, device=DEV)
@@ -515,3 +527,113 @@ def test_no_rows_and_no_requests():
     k, v = c.pools(2)
     z = torch.zeros((0, 4, 64), dtype=BF16, device=DEV)
     assert c.store(z, z[:, :2], z[:, :2], k, v, torch.zeros(0, dtype=torch.int64, device=DEV)).shape == (0, 4, 64)
+
+
+# ---- the operators together ---------------------------------------------------------------------------
+def shares_by_hand(units, extra, snap, least, grid):
+    """The blocks' pieces of tiles of `units` each, as (tile, part, parts, first unit, end, place)."""
+    total = sum(units)
+    first = [0]
+    for u in units:
+        first.append(first[-1] + u)
+    g = min(-(-total // least), grid)
+    each, more = divmod(total, g)
+    longer = more * (each + 1)
+
+    def owner(u):
+        return u // (each + 1) if u < longer else longer // (each + 1) + (u - longer) // each
+
+    got = []
+    for c in range(g):
+        lo = each * c + min(c, more)
+        hi = lo + each + (c < more)
+        t = next(i for i in range(len(units)) if lo < first[i + 1])
+        at, off = lo, lo - first[t]
+        if off <= snap:
+            at, off = at - off, 0
+        elif units[t] - off <= snap:
+            at, off, t = at + units[t] - off, 0, t + 1
+        while at < hi:
+            u0, end = at - off, units[t]
+            if hi - u0 < units[t]:
+                if hi - u0 <= snap:
+                    break
+                if units[t] - (hi - u0) > snap:
+                    end = hi - u0
+            c0, part, parts, place = c, 0, 1, None
+            if off or end < units[t]:
+                c0 = owner(u0 + snap)
+                parts, part = owner(u0 + units[t] - snap - 1) - c0 + 1, c - c0
+                place = 2 * c0 + 1 if part == 0 else 2 * c
+            got.append((t, part, parts, off, end, place))
+            at, off = u0 + end, end
+            if end == units[t]:
+                t, off = t + 1, 0
+    return got
+
+
+def test_every_unit_is_in_one_piece_and_every_piece_has_a_place():
+    # the arithmetic of the blocks' shares, as the kernels do it (cache.cuh), over random batches
+    r = random.Random(5)
+    for _ in range(300):
+        snap = r.randint(1, 6)
+        extra = r.randint(0, snap)
+        units = [extra + 1 + (r.randint(0, 5) if r.random() < 0.6 else r.randint(0, 120)) for _ in range(r.randint(1, 40))]
+        got = shares_by_hand(units, extra, snap, r.randint(1, 4), r.randint(1, 150))
+        places = [p[5] for p in got if p[5] is not None]
+        assert len(set(places)) == len(places)
+        for t, u in enumerate(units):
+            mine = sorted(p for p in got if p[0] == t)
+            assert [p[1] for p in mine] == list(range(mine[0][2]))          # parts 0, 1, ... of the number they say
+            assert [p[3] for p in mine] == [0] + [p[4] for p in mine[:-1]] and mine[-1][4] == u
+            assert all(p[4] > extra for p in mine)                          # none without a key
+
+
+@pytest.mark.gpu
+def test_both_kernels_take_any_number_of_rows():
+    b = Batch([1, 4, 2], [500, 70, 3000], 8, 2, 128, BF16, 16)
+    c = cache(8, 2, 128, 16, 3, 512, BF16)
+    one, other = b.run(c, max_new=4), b.run(c, max_new=0)      # 16 rows a request; not known: 28
+    wide = Batch([9, 12, 40], [500, 70, 3000], 8, 2, 128, BF16, 16)
+    o = wide.want()
+    near(wide.run(c, max_new=8), o, BF16)                      # fewer than there are: the speed's matter alone
+    near(wide.run(c, max_new=40), o, BF16)
+    near(one, b.want(), BF16)
+    near(other, b.want(), BF16)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 2.0])
+@pytest.mark.parametrize("new", [[1, 2], [150, 40]])
+def test_attend_scales(scale, new):
+    b = Batch(new, [300, 20], 4, 2, 64, F16, 16)
+    near(b.run(cache(4, 2, 64, 16, 2, 512, F16), scale=scale), b.want(scale=scale), F16)
+
+
+@pytest.mark.gpu
+def test_a_prompt_in_chunks_and_token_by_token_is_the_prompt_at_once():
+    import sys
+    sys.path.insert(0, os.path.join(ROOT, "examples"))
+    import decoder
+    x = torch.randn((3 * 150, 512), generator=torch.Generator(device=DEV).manual_seed(3), device=DEV).view(3, 150, 512)
+
+    def outs(cuts):
+        d = decoder.Decoder(layers=1, requests=3, n_pages=96)
+        got = []
+        for lo, hi in zip(cuts, cuts[1:]):
+            n = hi - lo
+            s = d.cache.extend(d.past, ints([n] * 3), d.free, d.free_count, d.table, 3 * n)
+            got.append(d.layers[0].attention(x[:, lo:hi].reshape(-1, 512), s, d.table, n).view(3, n, 512))
+            d.past.copy_(s.length), d.free_count.copy_(s.left[:1])
+        d.close()
+        return torch.cat(got, 1)
+
+    whole, apart = outs([0, 150]), outs([0, 64, 65, 100] + list(range(101, 151)))
+    # the same keys and weights; the sums' order and the roundings of weights, o and the product's rows differ
+    assert float((whole - apart).norm() / whole.norm()) < 4 * UNIT[BF16]
+    d = decoder.Decoder(layers=2, requests=3, n_pages=96)
+    y = x[:, :40].reshape(-1, 512).contiguous()
+    d.step(y, ints([40] * 3), 40)
+    d.cache.status()
+    assert bool(y.isfinite().all()) and d.past.tolist() == [40] * 3
+    d.close()
