@@ -370,7 +370,7 @@ template <int D, class T> static cudaError_t few(const AttendCall& a, int sm_cou
     static std::atomic<uint64_t> attr_set{0};
     if (cudaError_t e = ensure_dynamic_smem(attend_few_kernel<D, T>, (int)(Few<D>::fixed + share_smem(kCacheSeqs, kFewThreads)), attr_set)) return e;
     count_launch();
-    return launch_with(false, stream, attend_few_kernel<D, T>, dim3(sm_count * few_blocks(D)), dim3(kFewThreads), smem, a);
+    return launch_with(pdl_mode() != 0, stream, attend_few_kernel<D, T>, dim3(sm_count * few_blocks(D)), dim3(kFewThreads), smem, a);
 }
 template <int D> static cudaError_t few_as(const AttendCall& a, int ggml_type, int sm_count, cudaStream_t stream) {
     return ggml_type == BIVMOE_F16 ? few<D, __half>(a, sm_count, stream) : few<D, __nv_bfloat16>(a, sm_count, stream);

@@ -177,6 +177,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(const __grid_c
     uint8_t* ring = q_sm + NT * At<D>::q_tile;
     AtPlaces* places = (AtPlaces*)(ring + AT_SLOTS * AT_SLOT);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    pdl_enter();
     // the share is looked at once a piece: it stands in shared memory, the rows' registers are full
     __shared__ Share share;
     {
@@ -735,7 +736,7 @@ template <int D, class T> static cudaError_t tc(const AttendCall& a, int sm_coun
         at_map(&maps.v, a.v, a, D, at_is_half<T>, rows))
         maps.rows = rows;
     count_launch();
-    return launch_with(false, stream, attend_tc_kernel<D, T>, dim3(sm_count), dim3(AT_THREADS),
+    return launch_with(pdl_mode() == 1, stream, attend_tc_kernel<D, T>, dim3(sm_count), dim3(AT_THREADS),
                        (size_t)At<D>::fixed + share_smem(a.n_seq, AT_THREADS), a, maps);
 }
 cudaError_t launch_attend_tc(const AttendCall& a, int head_dim, int ggml_type, int sm_count, cudaStream_t stream) {

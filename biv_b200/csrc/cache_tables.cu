@@ -33,6 +33,7 @@ __global__ void __launch_bounds__(kExtendThreads) extend_kernel(ExtendCall c) {
     __shared__ int s_first[kCacheSeqs + 1], s_page[kCacheSeqs + 1], s_past[kCacheSeqs], s_have[kCacheSeqs];
     __shared__ int s_sum[2 * kExtendThreads / 32];
     const bivmoe_extend_args& a = c.a;
+    pdl_enter();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = a.n_seq;
     const int count = max(min(*a.free_count, a.n_free), 0);
     int tokens = 0, pages = 0, add[kExtendEach], need[kExtendEach];
@@ -118,9 +119,8 @@ cudaError_t launch_extend(const bivmoe_extend_args& a, int page_size, int sm_cou
     ExtendCall c{a, FastDiv((uint32_t)page_size)};
     // a few rows a thread: more blocks only repeat the sums
     const int blocks = (int)min((int64_t)sm_count, ((int64_t)a.n_tokens + 2 * kExtendThreads - 1) / (2 * kExtendThreads) + 1);
-    extend_kernel<<<blocks, kExtendThreads, 0, stream>>>(c);
     count_launch();
-    return cudaGetLastError();
+    return launch_with(pdl_mode() != 0, stream, extend_kernel, dim3(blocks), dim3(kExtendThreads), 0, c);
 }
 
 // ---- store ---------------------------------------------------------------------------------------
@@ -175,6 +175,7 @@ template <class In, class T, bool ADJACENT, int D>
 __global__ void __launch_bounds__(32 * kStoreWarps, 8) store_kernel(const __grid_constant__ StoreCall c) {
     constexpr int COLUMNS = D / 16, ROWS = 32 / COLUMNS, OWN = 8 / ROWS;   // units of a head, heads at once, pairs a lane makes
     const bivmoe_store_args& a = c.a;
+    pdl_enter();
     const int lane = threadIdx.x & 31, job = blockIdx.x * kStoreWarps + (threadIdx.x >> 5);
     const int t = job / c.parts, part = job - t * c.parts;
     if (t >= a.n_tokens) return;
@@ -237,22 +238,21 @@ __global__ void __launch_bounds__(32 * kStoreWarps, 8) store_kernel(const __grid
     }
 }
 
-template <class In, class T, bool ADJACENT> static void store_of(const StoreCall& c, int dim, int blocks, cudaStream_t stream) {
-    switch (dim) {
-        case 64: store_kernel<In, T, ADJACENT, 64><<<blocks, 32 * kStoreWarps, 0, stream>>>(c); break;
-        case 128: store_kernel<In, T, ADJACENT, 128><<<blocks, 32 * kStoreWarps, 0, stream>>>(c); break;
-        default: store_kernel<In, T, ADJACENT, 256><<<blocks, 32 * kStoreWarps, 0, stream>>>(c);
-    }
+template <class In, class T, bool ADJACENT> static cudaError_t store_of(const StoreCall& c, int dim, int blocks, cudaStream_t stream) {
+    auto launch = [&](void (*kernel)(StoreCall)) {
+        return launch_with(pdl_mode() != 0, stream, kernel, dim3(blocks), dim3(32 * kStoreWarps), 0, c);
+    };
+    return dim == 64 ? launch(store_kernel<In, T, ADJACENT, 64>)
+                     : dim == 128 ? launch(store_kernel<In, T, ADJACENT, 128>) : launch(store_kernel<In, T, ADJACENT, 256>);
 }
-template <class In, class T> static void store_as(const StoreCall& c, int dim, int blocks, cudaStream_t stream) {
-    if (c.rope.adjacent) store_of<In, T, true>(c, dim, blocks, stream);
-    else store_of<In, T, false>(c, dim, blocks, stream);
+template <class In, class T> static cudaError_t store_as(const StoreCall& c, int dim, int blocks, cudaStream_t stream) {
+    return c.rope.adjacent ? store_of<In, T, true>(c, dim, blocks, stream) : store_of<In, T, false>(c, dim, blocks, stream);
 }
-template <class T> static void store_from(const StoreCall& c, int dim, int blocks, cudaStream_t stream) {
+template <class T> static cudaError_t store_from(const StoreCall& c, int dim, int blocks, cudaStream_t stream) {
     switch (c.a.q.ggml_type) {
-        case BIVMOE_F32: store_as<float, T>(c, dim, blocks, stream); break;
-        case BIVMOE_F16: store_as<__half, T>(c, dim, blocks, stream); break;
-        default: store_as<__nv_bfloat16, T>(c, dim, blocks, stream);
+        case BIVMOE_F32: return store_as<float, T>(c, dim, blocks, stream);
+        case BIVMOE_F16: return store_as<__half, T>(c, dim, blocks, stream);
+        default: return store_as<__nv_bfloat16, T>(c, dim, blocks, stream);
     }
 }
 
@@ -266,10 +266,8 @@ cudaError_t launch_store(const bivmoe_store_args& a, const RopePlan& rope, int g
     const int rounds = (heads + 2 * heads_kv + 512 / head_dim - 1) / (512 / head_dim);
     c.parts = max(1, min(rounds, 16 * sm_count / a.n_tokens));
     const int blocks = (int)(((int64_t)a.n_tokens * c.parts + kStoreWarps - 1) / kStoreWarps);
-    if (ggml_type == BIVMOE_F16) store_from<__half>(c, head_dim, blocks, stream);
-    else store_from<__nv_bfloat16>(c, head_dim, blocks, stream);
     count_launch();
-    return cudaGetLastError();
+    return ggml_type == BIVMOE_F16 ? store_from<__half>(c, head_dim, blocks, stream) : store_from<__nv_bfloat16>(c, head_dim, blocks, stream);
 }
 
 }  // namespace bivmoe

@@ -373,8 +373,9 @@ BIVMOE_API int bivmoe_ep_peer_wait_limit(bivmoe_layer* layer, uint64_t microseco
  * position past the table) are never followed: their keys are not visible, their rows not stored.
  * Pointers need the alignment of their type; pools, and attend's q and out, 16 bytes, strides that
  * are multiples of 8 values there.  Strides are in values; the head_dim values of a row's head are
- * neighbours.  Calls of one handle use one workspace: on several streams they are ordered one after
- * another by the handle (not while a stream is captured: there the caller orders them). */
+ * neighbours.  The attend calls of one handle use one workspace: on several streams the handle orders
+ * them one after another (not while a stream is captured: there the caller does), for which the stream
+ * of the last call has to exist still. */
 typedef struct bivmoe_cache bivmoe_cache;
 
 typedef struct bivmoe_cache_desc {
