@@ -541,7 +541,6 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(const __grid_c
                             at_tmem_wait_st();
                             if (!before()) { ok = false; break; }
                             pf_fence_before();
-                            __syncwarp();
                             at_arrive(&H.p_half[s]);
                         }
                     }
@@ -578,31 +577,33 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(const __grid_c
 #pragma unroll 1
             for (int half = 0; half < (cut ? 2 : 1); half++) {
                 const int c0 = half * (D / 2), c1 = cut ? c0 + D / 2 : D;
+                // (32 columns to a trip to tensor memory; with 64 and 128 the loop, which runs once a piece, has more
+                // instructions to fetch: ragged prompts 61.5 -> 69.3 us)
+                constexpr int WIDE = 32;
 #pragma unroll 1
-                for (int c = c0; c < c1; c += 32) {
-                    int o[32];
+                for (int c = c0; c < c1; c += WIDE) {
+                    int o[WIDE];
                     if (n) {
-                        pf_tmem_ld32(tmem + t * D + lanes + c, o);
+#pragma unroll
+                        for (int i = 0; i < WIDE; i += 32) pf_tmem_ld32(tmem + t * D + lanes + c + i, *(int(*)[32])(o + i));
                         pf_tmem_wait_ld();
                     } else {
 #pragma unroll
-                        for (int i = 0; i < 32; i++) o[i] = 0;
+                        for (int i = 0; i < WIDE; i++) o[i] = 0;
                     }
-                    float y[32];
+                    float bad[4] = {};
 #pragma unroll
-                    for (int i = 0; i < 32; i++) {
-                        y[i] = __int_as_float(o[i]) * by;
-                        odd = fmaf(__int_as_float(o[i]), 0.0f, odd);
-                    }
+                    for (int i = 0; i < WIDE; i++) bad[i & 3] = fmaf(__int_as_float(o[i]), 0.0f, bad[i & 3]);
+                    odd += (bad[0] + bad[1]) + (bad[2] + bad[3]);
                     if (cut) {
 #pragma unroll
-                        for (int i = 0; i < 8; i++)
+                        for (int i = 0; i < WIDE / 4; i++)
                             sts128(at_piece(qs, row, (c - c0) / 4 + i), make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]));
                     } else {
+                        auto two = [&](int i) { return pack2<T>(__int_as_float(o[i]) * by, __int_as_float(o[i + 1]) * by); };
 #pragma unroll
-                        for (int i = 0; i < 4; i++)
-                            sts128(at_piece(qs, row, c / 8 + i), make_uint4(pack2<T>(y[8 * i], y[8 * i + 1]), pack2<T>(y[8 * i + 2], y[8 * i + 3]),
-                                                                            pack2<T>(y[8 * i + 4], y[8 * i + 5]), pack2<T>(y[8 * i + 6], y[8 * i + 7])));
+                        for (int i = 0; i < WIDE / 8; i++)
+                            sts128(at_piece(qs, row, c / 8 + i), make_uint4(two(8 * i), two(8 * i + 2), two(8 * i + 4), two(8 * i + 6)));
                     }
                 }
                 __syncwarp();
@@ -649,36 +650,55 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(const __grid_c
             }
             if (!__shfl_sync(0xffffffffu, last_one, 0)) continue;
             __threadfence();
-            float M = -INFINITY, L = 0.0f;            // of the row of this lane
-            for (int i = 0; i < x.parts; i++) M = fmaxf(M, __ldcg(a.part_ml + (int64_t)x.slot(i) * TR + r0 + lane).x);
+            // of the row of this lane: maximum and sum over the pieces, four under way at a time
             auto weight = [](float2 ml, float top) {  // a NaN piece has a sum that is one, whatever its maximum
                 return ml.x == -INFINITY ? (ml.y == 0.0f ? 0.0f : 1.0f) : exp2_of(ml.x - top);
             };
-            for (int i = 0; i < x.parts; i++) {
-                const float2 ml = __ldcg(a.part_ml + (int64_t)x.slot(i) * TR + r0 + lane);
-                L += ml.y * weight(ml, M);
+            float2 ml[4];
+            auto four = [&](int i0) {
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    ml[i] = i0 + i < x.parts ? __ldcg(a.part_ml + (int64_t)x.slot(i0 + i) * TR + r0 + lane) : make_float2(-INFINITY, 0.0f);
+            };
+            float M = -INFINITY, L = 0.0f;
+#pragma unroll 1
+            for (int i0 = 0; i0 < x.parts; i0 += 4) {
+                four(i0);
+                const float top = fmaxf(max3(M, ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x));
+                L *= weight(make_float2(M, 0.0f), top);
+                M = top;
+#pragma unroll
+                for (int i = 0; i < 4; i++) L += ml[i].y * weight(ml[i], M);
             }
             const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-            constexpr int V = D / 32, AT_ONCE = D == 256 ? 4 : 8;       // values a lane, neighbours; rows in flight
+            constexpr int V = D / 32, AT_ONCE = D == 256 ? 4 : 8;       // values a lane, neighbours; rows under way, of four pieces each
+#pragma unroll 1
             for (int r = 0; r < rows; r += AT_ONCE) {
                 float y[AT_ONCE][V] = {};
-                for (int i = 0; i < x.parts; i++) {
-                    const float2 ml = __ldcg(a.part_ml + (int64_t)x.slot(i) * TR + r0 + lane);
-                    const float mine_w = weight(ml, M);
-                    const float* from = a.part_o + ((int64_t)x.slot(i) * TR + r0 + r) * D + lane * V;
-                    float z[AT_ONCE][V];
+#pragma unroll 1
+                for (int i0 = 0; i0 < x.parts; i0 += 4) {
+                    if (x.parts > 4) four(i0);
+                    float z[4][AT_ONCE][V];
 #pragma unroll
-                    for (int u = 0; u < AT_ONCE; u++) {                 // rows past the tile's: whatever stands there
-                        if constexpr (V == 2) *(float2*)z[u] = __ldcg((const float2*)(from + u * D));
-                        else
+                    for (int i = 0; i < 4; i++) {                       // pieces and rows past the last: the last, or what stands there, unused
+                        const float* from = a.part_o + ((int64_t)x.slot(min(i0 + i, x.parts - 1)) * TR + r0 + r) * D + lane * V;
 #pragma unroll
-                            for (int e = 0; e < V; e += 4) *(float4*)(z[u] + e) = __ldcg((const float4*)(from + u * D + e));
+                        for (int u = 0; u < AT_ONCE; u++) {
+                            if constexpr (V == 2) *(float2*)z[i][u] = __ldcg((const float2*)(from + u * D));
+                            else
+#pragma unroll
+                                for (int e = 0; e < V; e += 4) *(float4*)(z[i][u] + e) = __ldcg((const float4*)(from + u * D + e));
+                        }
                     }
 #pragma unroll
-                    for (int u = 0; u < AT_ONCE; u++) {
-                        const float w = __shfl_sync(0xffffffffu, mine_w, r + u);
+                    for (int i = 0; i < 4; i++) {
+                        const float mine_w = weight(ml[i], M);
 #pragma unroll
-                        for (int e = 0; e < V; e++) y[u][e] = w != 0.0f ? y[u][e] + z[u][e] * w : y[u][e];
+                        for (int u = 0; u < AT_ONCE; u++) {
+                            const float w = __shfl_sync(0xffffffffu, mine_w, r + u);
+#pragma unroll
+                            for (int e = 0; e < V; e++) y[u][e] = w != 0.0f ? y[u][e] + z[i][u][e] * w : y[u][e];
+                        }
                     }
                 }
 #pragma unroll
@@ -692,7 +712,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(const __grid_c
             }
         }
     } else {
-        at_fewer_regs();
+        at_fewer_regs();                          // (the rows' registers come from every other warp)
     }
     pf_fence_before();
     __syncthreads();
@@ -728,6 +748,13 @@ template <int D, class T> static cudaError_t tc(const AttendCall& a, int sm_coun
     static_assert(At<D>::fixed + share_smem(kCacheSeqs, AT_THREADS) <= 227 * 1024, "the block must fit in shared memory");
     static std::atomic<uint64_t> attr_set{0};
     if (cudaError_t e = ensure_dynamic_smem(attend_tc_kernel<D, T>, (int)(At<D>::fixed + share_smem(kCacheSeqs, AT_THREADS)), attr_set)) return e;
+    // setmaxnreg deals out the registers that the block was launched with: a build that launches with fewer
+    // would wait for the rest for ever
+    static const int regs = [] {
+        cudaFuncAttributes f;
+        return cudaFuncGetAttributes(&f, attend_tc_kernel<D, T>) == cudaSuccess ? f.numRegs : 0;
+    }();
+    if (regs * AT_THREADS < 256 * (AT_ROW_REGS + AT_OTHER_REGS)) return cudaErrorLaunchOutOfResources;
     AtMaps maps;
     maps.rows = 0;
     int rows = 128;                   // the largest power of two, up to a tile, that divides a page
