@@ -458,6 +458,13 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(const __grid_c
                                 (lane % PR) * 16, x.row0 + t * 128 + r <= last);
                 }
                 asm volatile("cp.async.wait_all;" ::: "memory");
+                if (a.scale_log2 < 0.0f)              // of a negative scale the sign goes to the rows
+#pragma unroll 1
+                    for (int i = 0; i < 32 / RPI; i++) {
+                        const uint32_t at = at_piece(qs, (warp & 3) * 32 + i * RPI + lane / PR, lane % PR);
+                        const uint4 w = lds128(at);   // (the lane's own copy)
+                        sts128(at, make_uint4(w.x ^ 0x80008000u, w.y ^ 0x80008000u, w.z ^ 0x80008000u, w.w ^ 0x80008000u));
+                    }
                 at_fence_async();
                 __syncwarp();
                 at_arrive(&H.q_full[t]);
@@ -482,9 +489,6 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(const __grid_c
                     const uint4 there = *(const uint4*)H.there[(ktile + j) & 15];
                     const bool all = (there.x & there.y & there.z & there.w) == 0xffffffffu && key0 + AT_KEYS - 1 <= p_first &&
                                      (a.window <= 0 || p_top - key0 < a.window || key0 + AT_KEYS <= a.sinks);
-                    if (a.scale_log2 < 0.0f)
-#pragma unroll
-                        for (int i = 0; i < 128; i++) v[i] ^= (int)0x80000000u;
                     if (!all) {
                         const uint32_t tw[4] = {there.x, there.y, there.z, there.w};
 #pragma unroll
@@ -606,8 +610,10 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(const __grid_c
                             sts128(at_piece(qs, row, c / 8 + i), make_uint4(two(8 * i), two(8 * i + 2), two(8 * i + 4), two(8 * i + 6)));
                     }
                 }
+                // (a row that is made again below is not written here: `out` may be where its q stands)
+                const uint32_t again = cut ? 0u : __ballot_sync(0xffffffffu, odd != 0.0f);
                 __syncwarp();
-#pragma unroll
+#pragma unroll 1
                 for (int i0 = 0; i0 < 32 / RPI; i0 += 8) {
                     uint4 w[8];
 #pragma unroll
@@ -616,7 +622,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(const __grid_c
                     for (int i = 0; i < 8; i++) {
                         const int r = (i0 + i) * RPI + lane / PR, c = lane % PR;
                         const int64_t to = __shfl_sync(0xffffffffu, out_at, r);
-                        if (r < rows) {
+                        if (r < rows && !(again >> r & 1)) {
                             if (cut) __stcg((uint4*)(a.part_o + (place0 + r) * D + c0 + 4 * c), w[i]);
                             else *(uint4*)(a.out + to + 16 * c) = w[i];
                         }

@@ -13,7 +13,8 @@ namespace bivmoe {
 
 constexpr int kCacheSeqs = 1024;            // requests of a call
 constexpr int kCacheTokens = 1 << 20;       // new tokens of a call
-constexpr int kCachePositions = 1 << 30;    // lengths beyond this are cut here: positions are 32-bit
+constexpr int kCachePositions = 1 << 29;    // lengths beyond this are cut here: sums of two positions and a window are 32-bit
+constexpr int kCachePages = 1 << 20;        // new pages of a request and call
 constexpr int kRopePairs = 128;             // half the widest head
 
 // n / d for 0 <= n < 2^31 by a product: mul = ceil(2^(31 + shift) / d) with 2^shift >= d is at most

@@ -272,7 +272,8 @@ extern "C" int bivmoe_cache_attend(bivmoe_cache* c, const bivmoe_attend_args* a,
     k.page = FastDiv((uint32_t)c->d.page_size);
     k.group = FastDiv((uint32_t)(c->d.n_head / c->d.n_head_kv));
     k.heads_kv = c->d.n_head_kv;
-    k.window = a->window; k.sinks = a->sinks;
+    k.window = a->window < kCachePositions ? a->window : 0;   // as wide as any length: none
+    k.sinks = a->sinks < kCachePositions ? a->sinks : kCachePositions;
     k.scale_log2 = a->scale * 1.4426950408889634f;
     k.part_o = c->part_o; k.part_ml = c->part_ml; k.arrived = c->arrived; k.status = c->status;
     const cudaStream_t s = (cudaStream_t)stream;

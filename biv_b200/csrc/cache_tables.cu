@@ -47,7 +47,7 @@ __global__ void __launch_bounds__(kExtendThreads) extend_kernel(ExtendCall c) {
             add[i] = max(min(a.added[b], kCacheTokens), 0);
             const int holds = (int)c.page.div(past + c.page.d - 1);
             const int have = a.held ? max(min(a.held[b], a.table_width), 0) : holds;
-            need[i] = max((int)c.page.div(past + add[i] + c.page.d - 1) - have, 0);
+            need[i] = min(max((int)c.page.div(past + add[i] + c.page.d - 1) - have, 0), kCachePages);
             s_past[b] = past;
             s_have[b] = have;
             tokens += add[i];
@@ -106,7 +106,8 @@ __global__ void __launch_bounds__(kExtendThreads) extend_kernel(ExtendCall c) {
             const int at = (int)c.page.div(p);
             if (at < a.table_width) {
                 const int i = s_page[b] + at - s_have[b];   // of the new pages
-                const int page = at < s_have[b] ? a.table[b * a.table_stride + at] : i < count ? a.free_pages[count - 1 - i] : -1;
+                const bool given = i < min(count, s_page[b + 1]);
+                const int page = at < s_have[b] ? a.table[b * a.table_stride + at] : given ? a.free_pages[count - 1 - i] : -1;
                 if (page >= 0) slot = (int64_t)page * c.page.d + (p - at * (int)c.page.d);
             }
         }

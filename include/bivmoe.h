@@ -416,7 +416,7 @@ BIVMOE_API void bivmoe_cache_destroy(bivmoe_cache* cache);
 
 /* Pages, slots and positions for `added[b]` new tokens of each request b, which has `past[b]`.
  * A request holds held[b] pages (held null: ceil(past / page_size)) and gets what it needs for
- * past + added from the end of the free list: the j-th new page of the call, in the requests' order,
+ * past + added (up to 2^20 pages) from the end of the free list: the j-th new page of the call, in the requests' order,
  * is free_pages[free_count - 1 - j], or -1 when there is none.  Written: the new entries of `table`;
  * length[b] = past + added; first[b], the first row of request b among the call's new tokens, and
  * first[n_seq], their number; for each of the n_tokens rows its slot (page * page_size + place; -1
@@ -453,7 +453,7 @@ BIVMOE_API int bivmoe_cache_store(bivmoe_cache* cache, const bivmoe_store_args* 
  * p - window < j and j < sinks.  A row that sees nothing is zeros; what lies in places it does not
  * see (infinities, NaN) does not reach it.  max_new: no request has more new rows (0: not known); it
  * decides the kernel.  Sums and softmax in f32; the weights are rounded to the cache's type for the
- * second product.  Rows past first[n_seq] are not written. */
+ * second product.  Rows past first[n_seq] are not written.  `out` may be q. */
 typedef struct bivmoe_attend_args {
     bivmoe_rows q, out;
     bivmoe_pool k_pool, v_pool;
@@ -467,7 +467,8 @@ typedef struct bivmoe_attend_args {
 BIVMOE_API int bivmoe_cache_attend(bivmoe_cache* cache, const bivmoe_attend_args* args, void* stream);
 
 /* Waits for the stream; BIVMOE_ERR_TIMEOUT if a bounded wait of one of the cache's kernels gave up
- * since the last report (the results of that call are not to be used). */
+ * since the last report: the results of that call, and of calls after it until this one, are not to be
+ * used. */
 BIVMOE_API int bivmoe_cache_status(bivmoe_cache* cache, void* stream);
 
 /* The int8 tensor-pipe peak of the layer's GPU in tera-operations per second (two per

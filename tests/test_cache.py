@@ -148,6 +148,9 @@ def test_extend_of_lists_that_do_not_fit():
     c = cache(page=4, seqs=4, tokens=16)
     table = torch.full((3, 2), -1, dtype=torch.int32, device=DEV)
     s = c.extend(ints([-5, 100, 2]), ints([-1, 3, 2]), ints([7, 8]), ints([99]), table, 8)
+    big = 2 ** 31 - 1
+    t = c.extend(ints([big, big, 5]), ints([big, 1, 1]), ints([7, 8]), ints([2]), table.clone(), 8, held=ints([0, 0, 2]))
+    assert t.slots.tolist() == [-1] * 8 and t.left.tolist()[0] == 0      # the first request takes what there is, past its table
     # request 1 has no place for its page in the table, and the free list holds two whatever the count says
     assert s.first.tolist() == [0, 0, 3, 5] and s.length.tolist() == [0, 103, 4]
     assert s.slots.tolist() == [-1] * 8      # request 2's page was never given (the table says -1)
@@ -486,6 +489,22 @@ def test_a_step_in_a_graph_follows_its_lists():
     apart = torch.stack(outs).transpose(0, 1).reshape(80, 4, 64)
     # two results within the bound of `near` of the same: weights of at most one on values of some units
     assert float((whole.float() - apart.float()).abs().max()) <= 4 * 2.0 ** -8 * float(v2[table2[table2 >= 0].long()].nan_to_num().abs().max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new", [[1, 3], [150, 40]])
+def test_out_may_be_q_and_windows_may_be_as_wide_as_an_int(new):
+    b = Batch(new, [300, 20], 4, 2, 64, BF16, 16)
+    b.v[int(b.table[0, 3]), 5, 1, 7] = float("inf")        # rows that are made again read their q again
+    c = cache(4, 2, 64, 16, 2, 512, BF16)
+    want = b.run(c)
+    assert bool(want.isinf().any())
+    for window, sinks in ((2 ** 31 - 1, 0), (2 ** 31 - 1, 2 ** 31 - 1), (1, 2 ** 31 - 1)):
+        assert torch.equal(b.run(c, window=window, sinks=sinks), want)
+    b.length[0] = new[0] - 1        # a first row before the beginning, beside a window that reaches back further than an int
+    near(b.run(c, window=2 ** 31 - 1)[new[0]:], tuple(x[new[0]:] for x in b.want()), BF16)
+    b.length[0] = new[0] + 300
+    assert b.run(c, out=b.q) is b.q and torch.equal(b.q, want)
 
 
 @pytest.mark.gpu
