@@ -475,20 +475,21 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(const __grid_c
                 if (!at_wait_warp(&H.s_full[s], count & 1, &H.abort)) { ok = false; break; }
                 count++;
                 // Every product's end is waited for, and before the next one can begin: a parity tells a phase
-                // from the one before or after it only.  (Single tiles: the product before is followed by the
-                // next scores, so that the tensor cores do not wait for this.)
-                auto before = [&] { return !j || at_wait_warp(&H.pv_done[t], (cpv + j - 1) & 1, &H.abort); };
+                // from the one before or after it only.  (Pairs: the scores follow it.  Single tiles: it is
+                // followed by the next scores, so that the tensor cores do not wait for this.)
+                auto before = [&] { return !j || pair || at_wait_warp(&H.pv_done[t], (cpv + j - 1) & 1, &H.abort); };
                 if (any) {
                     pf_fence_after();
                     const uint32_t s_at = tmem + 256 + (s & 1) * 128 + lanes;
                     int v[128];
 #pragma unroll
                     for (int e = 0; e < 4; e++) pf_tmem_ld32(s_at + 32 * e, *(int(*)[32])(v + 32 * e));
-                    pf_tmem_wait_ld();
+                    // (looked at while S is on its way)
                     const int key0 = x.tiles.tile(x.i0 + j) * AT_KEYS;
                     const uint4 there = *(const uint4*)H.there[(ktile + j) & 15];
                     const bool all = (there.x & there.y & there.z & there.w) == 0xffffffffu && key0 + AT_KEYS - 1 <= p_first &&
                                      (a.window <= 0 || p_top - key0 < a.window || key0 + AT_KEYS <= a.sinks);
+                    pf_tmem_wait_ld();
                     if (!all) {
                         const uint32_t tw[4] = {there.x, there.y, there.z, there.w};
 #pragma unroll
