@@ -332,9 +332,12 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(const __grid_c
                 uint32_t cp[4] = {used[0], used[0], used[1], used[2]};
                 auto wait = [&](uint64_t* bar, uint32_t parity) { return ok = ok && at_wait(bar, parity, &H.abort); };
                 auto slot_of = [&](int q, int c) { return (base + q * CH + c) % AT_SLOTS; };
-                auto landed = [&](int q, int c) {
-                    const uint32_t gs = base + q * CH + c;
-                    wait(&H.full[gs % AT_SLOTS], (gs / AT_SLOTS) & 1);
+                // a tile of K or V, all its slots
+                auto landed = [&](int q) {
+                    for (int c = 0; c < CH; c++) {
+                        const uint32_t gs = base + q * CH + c;
+                        wait(&H.full[gs % AT_SLOTS], (gs / AT_SLOTS) & 1);
+                    }
                     at_fence_async();
                 };
                 auto free = [&](int q) {
@@ -355,8 +358,8 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(const __grid_c
                 // O_t += P_s V: the first 64 keys' weights are there before the others are made
                 auto values = [&](int q, int t, int s, bool first) {
                     const uint32_t va = pf_smem(ring + slot_of(q, 0) * AT_SLOT), parity = cp[s]++ & 1;
+                    if (t == 0) landed(q);                // (the second tile's turn: it has)
                     wait(&H.p_half[s], parity);
-                    for (int c = 0; c < CH; c++) landed(q, c);
                     pf_fence_after();
                     if (!ok) return;
 #pragma unroll
@@ -374,7 +377,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(const __grid_c
                 if (pair) wait(&H.q_full[1], pieces[1] & 1);
                 at_fence_async();
                 if (pair) {
-                    for (int c = 0; c < CH; c++) landed(0, c);
+                    landed(0);
                     if (ok) { scores(0, 0, 0); scores(0, 1, 1); free(0); }
                     for (int j = 0; j < n && ok; j++) {
                         const bool more = j + 1 < n;
@@ -383,7 +386,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(const __grid_c
                             if (!ok) break;
                             if (t == 1) free(2 * j + 1);
                             if (more) {
-                                if (t == 0) for (int c = 0; c < CH; c++) landed(2 * j + 2, c);
+                                if (t == 0) landed(2 * j + 2);
                                 if (!ok) break;
                                 scores(2 * j + 2, t, t);
                                 if (t == 1) free(2 * j + 2);
@@ -391,12 +394,12 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(const __grid_c
                         }
                     }
                 } else {
-                    for (int c = 0; c < CH; c++) landed(0, c);
+                    landed(0);
                     if (ok) { scores(0, 0, 2); free(0); }
                     for (int j = 0; j < n && ok; j++) {
                         const int kq = 2 * j + 1, vq = j + 1 < n ? 2 * j + 2 : 2 * n - 1;
                         if (j + 1 < n) {
-                            for (int c = 0; c < CH; c++) landed(kq, c);
+                            landed(kq);
                             if (!ok) break;
                             scores(kq, 0, 2 + ((j + 1) & 1));
                             free(kq);
