@@ -19,6 +19,11 @@
 // run while the other's products do.  Heads of 256 values, whose O alone takes half of tensor memory,
 // and pieces of up to 128 rows: one tile with two S, the next product into one while the first group
 // works on the other.
+// Bound by neither pipe alone: with heads of 128 the tensor cores and the special-function unit (a power
+// for each score, 1024 clocks a tile of 128 x 128) are each busy 40 % of the time, and S's way out of tensor
+// memory and P's way in lengthen a tile's chain: 2048 tokens at 30000, 32 / 8 heads, 1.04 TFLOP, 1040 us
+// (1210 to 1250 under the power cap), 0.61 of the measured bf16 peak.  With heads of 256 a key tile is
+// 128 KB, longer on its way from L2 than in the products: a prompt of 4096, 16 / 2 heads, 182 us.
 // m is not the running maximum itself but one that follows it when it has grown by more than 2^8:
 // O is then scaled in tensor memory, which happens a few times at a piece's start and rarely after (P
 // is at most 2^8, its sum and O are held in f32).
@@ -53,8 +58,12 @@ template <int D> struct At {
     static constexpr int tiles = D == 256 ? 1 : 2;           // of 128 rows
     static constexpr int rows = 128 * tiles;
     static constexpr int chunks = D / 64;                    // slots of a tile of K, or of V
-    static constexpr int extra = D == 256 ? 4 : 3;           // key tiles that a tile costs besides
-    static constexpr int snap = D == 256 ? 6 : 5;            // key tiles that are not worth a cut
+    // Key tiles that a tile costs besides.  us with 0 / 4 / 6 / 9: a prompt of 4096, heads of 256, 404 / 170 / 174 /
+    // 207; with 0 / 2 / 4 / 6: ragged prompts, heads of 64, 79 / 60 / 62 / 66.
+    static constexpr int extra = D == 256 ? 4 : 3;
+    // Key tiles that are not worth a cut.  us with 4 or 3 / 6 or 5 / 9 or 8: 48 rows at 1000 in eight requests, heads of
+    // 256, 38.1 / 27.6 / 27.6; a windowed prompt, heads of 128, 289 / 259 / 247; ragged prompts 60 / 62 / 69.
+    static constexpr int snap = D == 256 ? 6 : 5;
     static constexpr int q_tile = 128 * D * 2;
     static constexpr int fixed = AT_HEAD + tiles * q_tile + AT_SLOTS * AT_SLOT + (int)sizeof(AtPlaces) * AT_PAGES;
 };

@@ -386,6 +386,7 @@ cudaError_t launch_store(const bivmoe_store_args& a, const RopePlan& rope, int g
                          int page_size, int sm_count, cudaStream_t stream);
 // what the workspace is sized for: rows of a tile, blocks to a multiprocessor
 constexpr int kFewRows = 16;
+// (heads of 64, a windowed step of 128 requests: two blocks 75.1, three 69.7, four of 128 registers 70.0 us)
 constexpr int few_blocks(int head_dim) { return head_dim == 256 ? 1 : head_dim == 128 ? 2 : 3; }
 constexpr int tc_rows(int head_dim) { return head_dim == 256 ? 128 : 256; }
 

@@ -112,7 +112,9 @@ extern "C" int bivmoe_cache_create(const bivmoe_cache_desc* d, bivmoe_cache** ou
     c->d = *d;
     c->sm_count = sms;
     // pieces: at most two to a block (cache.cuh)
-    const size_t few = 2 * (size_t)few_blocks(d->head_dim) * c->sm_count * kFewRows, tc = 2 * (size_t)c->sm_count * tc_rows(d->head_dim),
+    // (none of the tcgen05 kernel's where no call has more rows than the other one's tiles)
+    const size_t few = 2 * (size_t)few_blocks(d->head_dim) * c->sm_count * kFewRows,
+                 tc = (int64_t)d->max_tokens * (d->n_head / d->n_head_kv) > kFewRows ? 2 * (size_t)c->sm_count * tc_rows(d->head_dim) : 0,
                  rows = few > tc ? few : tc, counts = 8 * (size_t)c->sm_count;
     size_t off = 0;
     auto take = [&off](size_t bytes) { const size_t at = off; off += (bytes + 255) & ~(size_t)255; return at; };
@@ -289,7 +291,7 @@ extern "C" int bivmoe_cache_attend(bivmoe_cache* c, const bivmoe_attend_args* a,
     //    48     128     10.7 / 15.2  18.2 / 23.5  138.5 / 81.3   83.3 / 71.4
     const int most = a->max_new > 0 && a->max_new < a->n_tokens ? a->max_new : a->n_tokens;
     const int64_t rows = (int64_t)most * k.group.d;
-    const bool few = rows <= 16 || (rows <= 32 && (c->d.head_dim <= 128 || (int64_t)a->n_seq * k.heads_kv <= 32));
+    const bool few = rows <= kFewRows || (rows <= 32 && (c->d.head_dim <= 128 || (int64_t)a->n_seq * k.heads_kv <= 32));
     if (e == cudaSuccess)
         e = few ? launch_attend_few(k, c->d.head_dim, c->d.ggml_type, c->sm_count, s)
                 : launch_attend_tc(k, c->d.head_dim, c->d.ggml_type, c->sm_count, s);
