@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(D)) attend_few_kernel(
                     const float mn = fmaxf(m[e], top[e]);
                     keep[e] = mn == -INFINITY ? 1.0f : exp2_of(m[e] - mn);
                     m[e] = mn;
-                    top[e] = mn == -INFINITY ? 0.0f : mn;
+                    top[e] = mn == -INFINITY ? 0.0f : mn - weight_lift<T>();
                     l[e] *= keep[e];
                 }
 #pragma unroll
@@ -264,7 +264,7 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(D)) attend_few_kernel(
                         s[t][e] = exp2_of(s[t][e] - top[e >> 1]);
                         l[e >> 1] += s[t][e];
                     }
-                // the weights, at most 1, rounded to the cache's type for the second product (relative
+                // the weights, at most 2^lift, rounded to the cache's type for the second product (relative
                 // error 2^-9 or 2^-12 each); l sums them unrounded
                 uint32_t w[KW / 16][4];
 #pragma unroll
@@ -297,7 +297,7 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(D)) attend_few_kernel(
         for (int e = 0; e < 2; e++) {
             l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
             l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
-            if (quad == 0) { s_m[warp][g + 8 * e] = m[e]; s_l[warp][g + 8 * e] = l[e]; }
+            if (quad == 0) { s_m[warp][g + 8 * e] = m[e] - weight_lift<T>(); s_l[warp][g + 8 * e] = l[e]; }
         }
 #pragma unroll
         for (int c = 0; c < D / 8; c++)

@@ -339,6 +339,13 @@ __device__ __forceinline__ float exp2_of(float x) {
     return y;
 }
 
+// The powers of two by which the weights that go into the second product are lifted above one (up to
+// 2^15 in all): f16 keeps its 11 bits down to 2^-14 and nothing below 2^-25, and the many small weights beside one
+// large key count together.  The maximum that a piece is written with is lowered by as much, so that pieces join as they are.
+// bf16 has f32's exponents.
+template <class T> __device__ __forceinline__ constexpr float weight_lift() { return 0.0f; }
+template <> __device__ __forceinline__ constexpr float weight_lift<__half>() { return 15.0f; }
+
 // ---- the careful row -------------------------------------------------------------------------------
 // A weight of zero times an infinity or a NaN is a NaN, so in the tiled products a value that a row does
 // not see could reach it.  Rows that come out of them not finite are computed again like this, by a warp,

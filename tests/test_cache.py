@@ -336,6 +336,24 @@ def test_attend_scores_far_apart(dim, new, past):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("new, past", [([1] * 40, [3000] * 40), ([140] * 6, [2000] * 6)])
+def test_many_small_weights_beside_a_large_one(new, past, dim, dtype):
+    # four keys hold all but 2^-18.73 of a weight each and have values of zero: the result is what the others
+    # come to, weights that f16 has 6 bits for if the largest is 1
+    b = Batch(new, past, 8, 4, dim, dtype, 16, seed=17)
+    b.q.fill_(1.0)
+    b.k.fill_(0.0)
+    b.v.fill_(1.0)
+    for j in (0, 16, 32, 48):
+        at = b.table[:, j // 16].long()
+        b.k[at, 0] = 18.73 * math.log(2.0) / math.sqrt(dim)
+        b.v[at, 0] = 0.0
+    near(b.run(cache(8, 4, dim, 16, len(new), sum(new), dtype)), b.want(), dtype)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dim", [64, 128, 256])
 @pytest.mark.parametrize("new, past", [([3, 2], [100, 0]), ([300, 150], [20, 700])])
 def test_values_a_row_does_not_see_do_not_reach_it(dim, new, past):
