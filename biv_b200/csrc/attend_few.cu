@@ -85,7 +85,7 @@ template <int D, class T> __device__ __forceinline__ void join(const AttendCall&
             float2 ml[4];
             float4 v[4][CK];
 #pragma unroll
-            for (int s = 0; s < 4; s++) {         // past the last piece: the last one again, of weight 0
+            for (int s = 0; s < 4; s++) {         // past the last piece: the last one again, not added
                 const int64_t at = (int64_t)x.slot(min(s0 + s, x.parts - 1)) * kFewRows + row;
                 ml[s] = __ldcg(a.part_ml + at);
 #pragma unroll
@@ -101,8 +101,8 @@ template <int D, class T> __device__ __forceinline__ void join(const AttendCall&
             M = top;
 #pragma unroll
             for (int s = 0; s < 4; s++) {
-                const float w = s0 + s < x.parts ? weight(ml[s], M) : 0.0f;
-                if (w == 0.0f) continue;
+                if (s0 + s >= x.parts) continue;      // (a weight of zero counts: zero times a NaN)
+                const float w = weight(ml[s], M);
                 L += ml[s].y * w;
 #pragma unroll
                 for (int i = 0; i < CK; i++) {
@@ -321,7 +321,7 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(D)) attend_few_kernel(
 #pragma unroll
             for (int w = 0; w < kFewWarps; w++) {
                 const float4 z = *(const float4*)(sm + w * kFewStages * Few<D>::stage + (row * Few<D>::part + sub * 4 + 32 * i) * 4);
-                if (f[w] != 0.0f) { v.x += z.x * f[w]; v.y += z.y * f[w]; v.z += z.z * f[w]; v.w += z.w * f[w]; }
+                v.x += z.x * f[w]; v.y += z.y * f[w]; v.z += z.z * f[w]; v.w += z.w * f[w];
             }
             y[i] = v;
             const float z = (v.x - v.x) + (v.y - v.y) + (v.z - v.z) + (v.w - v.w);

@@ -717,7 +717,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(const __grid_c
                         for (int u = 0; u < AT_ONCE; u++) {
                             const float w = __shfl_sync(0xffffffffu, mine_w, r + u);
 #pragma unroll
-                            for (int e = 0; e < V; e++) y[u][e] = w != 0.0f ? y[u][e] + z[i][u][e] * w : y[u][e];
+                            for (int e = 0; e < V; e++) y[u][e] = i0 + i < x.parts ? y[u][e] + z[i][u][e] * w : y[u][e];
                         }
                     }
                 }

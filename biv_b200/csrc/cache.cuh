@@ -349,8 +349,10 @@ template <> __device__ __forceinline__ constexpr float weight_lift<__half>() { r
 // ---- the careful row -------------------------------------------------------------------------------
 // A weight of zero times an infinity or a NaN is a NaN, so in the tiled products a value that a row does
 // not see could reach it.  Rows that come out of them not finite are computed again like this, by a warp,
-// from the keys that they see alone; a row that does see such values has its NaN after the first of
-// them.  Lane l holds the values l, l + 32, ... of o.
+// from the keys that they see alone.  A value that a row does see reaches it whatever its weight, and a
+// piece of a weight that is zero in f32 takes part in the join for that: which keys share a piece is not
+// the row's matter.  A row that sees a score of NaN or infinity ends there, as a piece that every join
+// gives the weight 1 (maximum -infinity, sum NaN).  Lane l holds the values l, l + 32, ... of o.
 template <int D, class T>
 __device__ __noinline__ void careful_row(const AttendCall& a, const Piece& x, int row, int kt, float (&o)[D / 32], float& m, float& l) {
     const int lane = threadIdx.x & 31, R = x.row0 + row;
@@ -377,6 +379,7 @@ __device__ __noinline__ void careful_row(const AttendCall& a, const Piece& x, in
             if (s != s || mn == INFINITY) {       // the softmax of a NaN, or of infinity: NaN
                 for (int e = 0; e < D / 32; e++) o[e] = NAN;
                 l = NAN;
+                m = -INFINITY;
                 return;
             }
             m = mn;

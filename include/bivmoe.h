@@ -451,7 +451,9 @@ BIVMOE_API int bivmoe_cache_store(bivmoe_cache* cache, const bivmoe_store_args* 
  * first[b + 1] - 1 are the last tokens of request b, of length[b] tokens, which the pages of
  * table[b] hold.  A token at position p sees the positions j <= p; with window > 0 of these
  * p - window < j and j < sinks.  A row that sees nothing is zeros; what lies in places it does not
- * see (infinities, NaN) does not reach it.  max_new: no request has more new rows (0: not known); it
+ * see (infinities, NaN) does not reach it.  What it sees does, whatever its weight: a score of NaN or
+ * +infinity, or a value of NaN or infinity, leaves the row (the value's place in it) not finite.  A score of
+ * -infinity is a weight of zero, and a row of such scores alone zeros.  max_new: no request has more new rows (0: not known); it
  * decides the kernel.  Sums and softmax in f32; the weights are rounded to the cache's type for the
  * second product.  Rows past first[n_seq] are not written.  `out` may be q. */
 typedef struct bivmoe_attend_args {
