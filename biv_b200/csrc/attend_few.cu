@@ -331,6 +331,11 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(D)) attend_few_kernel(
         if (__syncthreads_or(!fine && row < x.rows)) {
             for (int r = warp; r < x.rows; r += kFewWarps) {
                 if (!s_bad[r]) continue;
+                if (!met_hidden<D, T>(a, x, r, KT)) {      // it stays as it is
+                    __syncwarp();
+                    if (lane == 0) s_bad[r] = 0;
+                    continue;
+                }
                 float c[D / 32], cm, cl;
                 careful_row<D, T>(a, x, r, KT, c, cm, cl);
                 for (int e = 0; e < D / 32; e++) ((float*)sm)[r * D + lane + 32 * e] = c[e];

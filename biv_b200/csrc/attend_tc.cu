@@ -85,6 +85,7 @@ struct AtHead {
     int boxes[AT_PAGES];              // of a key tile that the copy engine fetches, or 0
     uint32_t tmem;
     int abort;
+    int mending;                      // warps that make rows again, which may take as long as there are keys
 };
 static_assert(sizeof(AtHead) <= AT_HEAD && offsetof(AtHead, there) % 16 == 0, "");
 
@@ -92,12 +93,29 @@ static_assert(sizeof(AtHead) <= AT_HEAD && offsetof(AtHead, there) % 16 == 0, ""
 // the fewest.
 __device__ __forceinline__ void at_fewer_regs() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(AT_OTHER_REGS)); }
 // Every role's waits look at the clock, once in 64 tries that found nothing: a role that ends early does not
-// leave the others without one that gives up.
-__device__ __forceinline__ bool at_wait(uint64_t* bar, uint32_t parity, const int* abort) {
-    return bounded_wait<64>(PfWait<true, false>{bar, parity, abort});
+// leave the others without one that gives up.  The clock stands while rows are made again: that is bounded
+// by the keys they see, and could take longer than any other wait.  (A look is a call: written out at every
+// wait it made a prompt of 4096, heads of 256, 188 us instead of 181.)
+__device__ __noinline__ uint64_t at_look(const AtHead* h, uint32_t look, uint64_t t0) {   // where the clock began; 0: gives up
+    WaitClock clock{t0};
+    if (*(const volatile int*)&h->abort) return 0;
+    return clock.late(look, pf_now_ns(), *(const volatile int*)&h->mending != 0) ? 0 : clock.t0;
 }
-__device__ __forceinline__ bool at_wait_warp(uint64_t* bar, uint32_t parity, const int* abort) {
-    return bounded_wait_together<64>(PfWait<true, false>{bar, parity, abort});
+template <bool SLEEP> struct AtWait {
+    uint64_t* bar;
+    uint32_t parity;
+    const AtHead* h;
+    uint64_t t0 = 0;
+    __device__ __forceinline__ bool ready() const { return pf_bar_try(bar, parity); }
+    __device__ __forceinline__ bool late(uint32_t look) { return !(t0 = at_look(h, look, t0)); }
+    __device__ __forceinline__ void pause() const { if (SLEEP) __nanosleep(32); }
+    __device__ __forceinline__ bool all(bool v) const { return __all_sync(0xffffffffu, v); }
+};
+__device__ __forceinline__ bool at_wait(uint64_t* bar, uint32_t parity, const AtHead* h) {
+    return bounded_wait<64>(AtWait<false>{bar, parity, h});
+}
+template <bool SLEEP = false> __device__ __forceinline__ bool at_wait_warp(uint64_t* bar, uint32_t parity, const AtHead* h) {
+    return bounded_wait_together<64>(AtWait<SLEEP>{bar, parity, h});
 }
 // One lane's arrival for its warp, which is together again after it: what follows may be an instruction that
 // a whole warp has to execute at once (tcgen05.ld, .st), and a branch that one lane takes does not by
@@ -203,7 +221,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(const __grid_c
         for (int i = 0; i < 4; i++) { pf_bar_init(&H.s_full[i], 1); pf_bar_init(&H.p_half[i], 4); pf_bar_init(&H.p_full[i], 4); }
         for (int i = 0; i < AT_PAGES; i++) { pf_bar_init(&H.page_full[i], 1); pf_bar_init(&H.page_empty[i], 2 * CH); }
         pf_bar_init(&H.drained, 1);
-        H.abort = 0;
+        H.abort = H.mending = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == AT_MMA_WARP) {
@@ -251,7 +269,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(const __grid_c
                         known[i] = __ballot_sync(0xffffffffu, page[i] >= 0 || key > p_top);
                     }
                 }
-                if (!bounded_wait_together<64>(PfWait<true, true>{&H.page_empty[e], ((ktile / AT_PAGES) & 1) ^ 1, &H.abort})) {
+                if (!at_wait_warp<true>(&H.page_empty[e], ((ktile / AT_PAGES) & 1) ^ 1, &H)) {
                     give_up(AT_SITE_PAGES);
                     ok = false;
                     break;
@@ -284,8 +302,8 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(const __grid_c
                 const AtTurn turn = at_turn(i / CH, n, pair);
                 const int c = i % CH;
                 const uint32_t kt = ktile + turn.j;
-                if (!bounded_wait_together<64>(PfWait<true, true>{&H.page_full[kt % AT_PAGES], (kt / AT_PAGES) & 1, &H.abort}) ||
-                    !bounded_wait_together<64>(PfWait<true, true>{&H.empty[slot], ((gs / AT_SLOTS) & 1) ^ 1, &H.abort})) {
+                if (!at_wait_warp<true>(&H.page_full[kt % AT_PAGES], (kt / AT_PAGES) & 1, &H) ||
+                    !at_wait_warp<true>(&H.empty[slot], ((gs / AT_SLOTS) & 1) ^ 1, &H)) {
                     give_up(AT_SITE_COPY);
                     ok = false;
                     break;
@@ -339,7 +357,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(const __grid_c
             const bool pair = NT == 2 && x.rows > 128;
             if (pf_elect()) {
                 uint32_t cp[4] = {used[0], used[0], used[1], used[2]};
-                auto wait = [&](uint64_t* bar, uint32_t parity) { return ok = ok && at_wait(bar, parity, &H.abort); };
+                auto wait = [&](uint64_t* bar, uint32_t parity) { return ok = ok && at_wait(bar, parity, &H); };
                 auto slot_of = [&](int q, int c) { return (base + q * CH + c) % AT_SLOTS; };
                 // a tile of K or V, all its slots
                 auto landed = [&](int q) {
@@ -485,12 +503,12 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(const __grid_c
             for (int j = 0; j < n; j++) {
                 const int s = pair ? t : 2 + (j & 1);
                 uint32_t& count = pair ? cs[0] : j & 1 ? cs[2] : cs[1];
-                if (!at_wait_warp(&H.s_full[s], count & 1, &H.abort)) { ok = false; break; }
+                if (!at_wait_warp(&H.s_full[s], count & 1, &H)) { ok = false; break; }
                 count++;
                 // Every product's end is waited for, and before the next one can begin: a parity tells a phase
                 // from the one before or after it only.  (Pairs: the scores follow it.  Single tiles: it is
                 // followed by the next scores, so that the tensor cores do not wait for this.)
-                auto before = [&] { return !j || pair || at_wait_warp(&H.pv_done[t], (cpv + j - 1) & 1, &H.abort); };
+                auto before = [&] { return !j || pair || at_wait_warp(&H.pv_done[t], (cpv + j - 1) & 1, &H); };
                 if (any) {
                     pf_fence_after();
                     const uint32_t s_at = tmem + 256 + (s & 1) * 128 + lanes;
@@ -578,7 +596,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(const __grid_c
             if (!ok) { give_up(AT_SITE_ROWS); break; }
             ktile += n;
             if (n) {
-                if (!at_wait_warp(&H.pv_done[t], (cpv + n - 1) & 1, &H.abort)) { give_up(AT_SITE_ROWS); ok = false; break; }
+                if (!at_wait_warp(&H.pv_done[t], (cpv + n - 1) & 1, &H)) { give_up(AT_SITE_ROWS); ok = false; break; }
                 cpv += n;
                 pf_fence_after();
             }
@@ -624,7 +642,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(const __grid_c
                             sts128(at_piece(qs, row, c / 8 + i), make_uint4(two(8 * i), two(8 * i + 2), two(8 * i + 4), two(8 * i + 6)));
                     }
                 }
-                // (a row that is made again below is not written here: `out` may be where its q stands)
+                // (a row that may be made again below is not written here: `out` may be where its q stands)
                 const uint32_t again = cut ? 0u : __ballot_sync(0xffffffffu, odd != 0.0f);
                 __syncwarp();
 #pragma unroll 1
@@ -645,12 +663,18 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(const __grid_c
                 __syncwarp();
             }
             if (cut && mine) __stcg(a.part_ml + place0 + lane, make_float2(m * scale - lift, l));
-            for (uint32_t bad = __ballot_sync(0xffffffffu, mine && odd != 0.0f); bad; bad &= bad - 1) {
+            const uint32_t odd_rows = __ballot_sync(0xffffffffu, mine && odd != 0.0f);
+            if (odd_rows && lane == 0) atomicAdd(&H.mending, 1);
+            for (uint32_t bad = odd_rows; bad; bad &= bad - 1) {
                 __syncwarp();
                 const int of = __ffs(bad) - 1, r = r0 + of;
+                const int64_t out_of = __shfl_sync(0xffffffffu, out_at, of), at = place0 + of;
+                if (!met_hidden<D, T>(a, x, r, AT_KEYS)) {            // it stays as it is, and still stands in shared memory
+                    if (!cut && lane < PR) *(uint4*)(a.out + out_of + 16 * lane) = lds128(at_piece(qs, (warp & 3) * 32 + of, lane));
+                    continue;
+                }
                 float o[D / 32], cm, cl;
                 careful_row<D, T>(a, x, r, AT_KEYS, o, cm, cl);
-                const int64_t out_of = __shfl_sync(0xffffffffu, out_at, of), at = place0 + of;
                 const float inv = cl == 0.0f ? 0.0f : 1.0f / cl;
                 for (int e = 0; e < D / 32; e++) {
                     if (cut) __stcg(a.part_o + at * D + lane + 32 * e, o[e]);
@@ -658,6 +682,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(const __grid_c
                 }
                 if (cut && lane == 0) __stcg(a.part_ml + at, make_float2(cm, cl));
             }
+            if (odd_rows && lane == 0) atomicAdd(&H.mending, -1);
             if (!cut) continue;
             // the warp that is last with these 32 rows joins their pieces, in the pieces' order
             __threadfence();

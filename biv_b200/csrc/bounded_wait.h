@@ -35,6 +35,16 @@ BIV_WAIT_FN bool bounded_wait_together(W w) {
     return w.all(here);
 }
 
+// When a wait that looks at the clock gives up: kWaitNs after its first look, or after the last one at
+// which another role was at something that its own work bounds, however long that takes.
+struct WaitClock {
+    uint64_t t0 = 0;
+    BIV_WAIT_FN bool late(uint32_t look, uint64_t now_ns, bool at_work) {
+        if (look == 1 || at_work) t0 = now_ns;
+        return now_ns - t0 >= kWaitNs;
+    }
+};
+
 // What a warp does that gave up on a wait while others may meet at a barrier that counts it: it arrives
 // there for them (m.arrive()) until all have left (m.all_left()), each at its next wait; `turns` bounds
 // that.  An arrival too many only ends a meeting early, which spoils nothing but results that the

@@ -1,10 +1,12 @@
 """The paged cache at its edges: values that are not finite."""
 import math
+import os
+import subprocess
 
 import pytest
 import torch
 
-from test_cache import BF16, DEV, F16, Batch, cache, near
+from test_cache import BF16, DEV, F16, ROOT, Batch, cache, near
 
 
 # ---- values that are not finite ----------------------------------------------------------------------
@@ -52,3 +54,118 @@ def test_a_score_of_minus_infinity_is_a_weight_of_zero(dim, new):
     want = b.want(drop=[(0, 803)])
     near(got[:new], tuple(x[:new] for x in want), BF16)
     assert bool((got[new:] == 0).all())
+
+
+def sees(p, j, window, sinks):
+    return j <= p and (not window or p - j < window or j < sinks)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim, dtype", [(64, BF16), (128, F16), (256, BF16)])
+@pytest.mark.parametrize("new, past", [([4, 2], [700, 90]), ([300, 150], [50, 700])])
+@pytest.mark.parametrize("window, sinks", [(0, 0), (100, 0), (100, 70), (257, 3)])
+def test_values_at_the_edges_of_what_a_row_sees(window, sinks, new, past, dim, dtype):
+    # one value that is not finite, in places that some of the rows see: by their window's lower end, by the
+    # end of the first tokens that stay visible, by their own position
+    edges = {j + d for n, p in zip(new, past) for j in (p + n - 1, p + n // 2, p + n // 2 - window, p - window, sinks) for d in (-1, 0, 1)}
+    c = cache(8, 2, dim, 16, 2, 512, dtype)
+    b = Batch(new, past, 8, 2, dim, dtype, 16, seed=9)
+    want = b.want(window, sinks)
+    for j in sorted(edges):
+        kept = b.v.clone()
+        hit = [0 <= j < n + p for n, p in zip(new, past)]
+        for r in range(2):
+            if hit[r]:
+                b.v[int(b.table[r, j // 16]), j % 16, 1, 5] = (math.inf, math.nan)[j % 2]
+        got = b.run(c, window=window, sinks=sinks, max_new=max(new))
+        at = 0
+        for r, (n, p) in enumerate(zip(new, past)):
+            see = torch.tensor([hit[r] and sees(p + i, j, window, sinks) for i in range(n)], device=DEV)
+            rows = got[at:at + n]
+            odd = torch.zeros_like(rows, dtype=torch.bool)
+            odd[:, 4:, 5] = see[:, None]          # the heads of kv head 1, the value's place
+            assert torch.equal(~rows.isfinite(), odd), (j, r)
+            near(torch.where(odd, want[0][at:at + n].to(dtype), rows), tuple(x[at:at + n] for x in want), dtype)
+            at += n
+        b.v.copy_(kept)
+    c.status()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new, heads", [(256, 16), (4, 16)])
+def test_a_long_past_with_a_value_that_is_not_finite(new, heads):
+    # eight requests of 10^5 tokens: what one of them holds does not cost the others their results
+    seqs, past, dim = 8, 100_000, 128
+    b = Batch([new] * seqs, [past] * seqs, heads, 4, dim, BF16, 64, seed=3, junk=0.0)
+    c = cache(heads, 4, dim, 64, seqs, new * seqs, BF16)
+    clean = b.run(c, max_new=new)
+    # an early value that all rows of request 3 see: its place in them, and nothing else
+    at = (int(b.table[3, 1]), 7, 1, 9)
+    was = b.v[at].clone()
+    b.v[at] = math.inf
+    got = b.run(c, max_new=new)
+    c.status()
+    odd = torch.zeros_like(got, dtype=torch.bool)
+    odd[3 * new:4 * new, heads // 4:heads // 2, 9] = True
+    assert torch.equal(~got.isfinite(), odd) and torch.equal(got[~odd], clean[~odd])
+    b.v[at] = was
+    # each request's last token holds values that none of its other rows sees
+    last = past + new - 1
+    for r in range(seqs):
+        b.v[int(b.table[r, last // 64]), last % 64] = math.nan
+    got = b.run(c, max_new=new).view(seqs, new, heads, dim)
+    c.status()
+    assert bool(got[:, -1].isnan().all()) and bool(got[:, :-1].isfinite().all())
+    # against the run before: each is within `near`'s bound of the same, on values whose weights sum to one
+    far = (got[:, :-1].double() - clean.view(got.shape)[:, :-1].double()).abs()
+    o, mag = [x.view(got.shape)[:, :-1] for x in one_head(b, heads)]
+    at = [0, heads // 4 * 2]                      # the heads that one_head states
+    assert bool((far[:, :, at] <= 2 * (2.0 ** -8 * o[:, :, at].abs() + (2.0 ** -8 + 2.0 ** -13) * mag[:, :, at] + 1e-7)).all())
+
+
+def one_head(b, heads):
+    """`Batch.want` for the first head, and the first of kv head 2, alone."""
+    o, mag = torch.zeros(b.q.shape, dtype=torch.float64, device=DEV), torch.zeros(b.q.shape, dtype=torch.float64, device=DEV)
+    at = 0
+    for r, (n, p) in enumerate(zip(b.new, b.past)):
+        t = torch.arange(n + p, device=DEV)
+        pg = b.table[r].long()[t // b.page]
+        see = t[None] <= torch.arange(p, p + n, device=DEV)[:, None]
+        for h in (0, heads // 4 * 2):
+            k, v = [x[pg, t % b.page, h // b.g].double() for x in (b.k, b.v)]
+            w = torch.softmax((b.q[at:at + n, h].double() @ k.T / math.sqrt(k.shape[1])).masked_fill(~see, -math.inf), -1)
+            v = v.nan_to_num(0.0, 0.0, 0.0)
+            o[at:at + n, h], mag[at:at + n, h] = w @ v, w @ v.abs()
+        at += n
+    return o, mag
+
+
+def test_the_clock_of_a_wait_stands_while_another_role_is_at_work(tmp_path):
+    src, exe = tmp_path / "clock.cpp", str(tmp_path / "clock")
+    src.write_text(r"""
+#include <cstdio>
+#include <initializer_list>
+#include "bounded_wait.h"
+using namespace bivmoe;
+static uint64_t now;
+static int tries;
+struct Wait {                     // ready never; a look every 1000 ns; another role at work until `until`
+    uint64_t until; WaitClock clock{};
+    bool ready() { tries++; return false; }
+    bool late(uint32_t look) { return clock.late(look, now, now < until); }
+    void pause() { now += 1000; }
+};
+int main() {
+    for (uint64_t until : {0ull, 5ull * kWaitNs, 5ull * kWaitNs + 123456789}) {
+        now = 77;
+        tries = 0;
+        if (bounded_wait<1>(Wait{until})) return 1;
+        // gives up kWaitNs after the other role's end, and not without it
+        const uint64_t from = until > 77 ? until : 77;
+        if (now < from + kWaitNs - 2000 || now > from + kWaitNs + 2000) { printf("%llu\n", (unsigned long long)now); return 2; }
+    }
+    return 0;
+}
+""")
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-I", os.path.join(ROOT, "biv_b200", "csrc"), "-o", exe, str(src)], check=True)
+    assert subprocess.run([exe], timeout=60).returncode == 0
