@@ -292,6 +292,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(const __grid_c
         at_fewer_regs();
         // ---- copies
         uint32_t base = 0, ktile = 0;             // slots, key tiles of the pieces before
+        uint32_t last = 0, fills = 0;             // the last slot this warp filled, how many
         bool ok = true;
         for (Piece x; ok && walk.next(x);) {
             const int n = max(x.n, 0), total = 2 * n * CH;
@@ -308,6 +309,8 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(const __grid_c
                     ok = false;
                     break;
                 }
+                last = gs;
+                fills++;
                 const AtPlaces& pl = places[kt % AT_PAGES];
                 if (const int n_box = H.boxes[kt % AT_PAGES]) {
                     if (lane == 0) pf_bar_expect_tx(&H.full[slot], AT_SLOT);
@@ -343,7 +346,10 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(const __grid_c
             base += total;
             ktile += n;
         }
-        asm volatile("cp.async.wait_all;" ::: "memory");   // nothing is in flight when the block ends
+        // Nothing is in flight when the block ends, whatever ended the loops: nobody may have waited for the last slots.
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        wait_for_last_fills<AT_SLOTS, AT_COPY_WARPS>(last, fills, [&](uint32_t slot, uint32_t parity) { pf_bar_wait(&H.full[slot], parity); });
+        __syncwarp();
     } else if (warp == AT_MMA_WARP) {
         at_fewer_regs();
         // ---- products

@@ -45,6 +45,19 @@ struct WaitClock {
     }
 };
 
+// The last fills of a copying warp that may be under way yet.  It fills every STEP-th place of a line that goes
+// round a ring of SLOTS, and a slot again only after its fill before has landed and been used: so the last
+// SLOTS / STEP fills at most.  wait(slot, parity) of each, the oldest first; `last` is the place of the last one,
+// `fills` how many there were.
+template <int SLOTS, int STEP, class F>
+BIV_WAIT_FN void wait_for_last_fills(uint32_t last, uint32_t fills, F wait) {
+    static_assert(SLOTS % STEP == 0, "a warp's slots are its own");
+    for (uint32_t i = fills < SLOTS / STEP ? fills : SLOTS / STEP; i--;) {
+        const uint32_t at = last - STEP * i;
+        wait(at % SLOTS, (at / SLOTS) & 1);
+    }
+}
+
 // What a warp does that gave up on a wait while others may meet at a barrier that counts it: it arrives
 // there for them (m.arrive()) until all have left (m.all_left()), each at its next wait; `turns` bounds
 // that.  An arrival too many only ends a meeting early, which spoils nothing but results that the

@@ -169,3 +169,78 @@ int main() {
 """)
     subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-I", os.path.join(ROOT, "biv_b200", "csrc"), "-o", exe, str(src)], check=True)
     assert subprocess.run([exe], timeout=60).returncode == 0
+
+
+def test_a_copying_warp_stays_until_its_last_fills_have_landed(tmp_path):
+    # four warps fill a ring of eight; fills land late, by themselves; the consumer stops anywhere
+    src, exe = tmp_path / "fills.cpp", str(tmp_path / "fills")
+    src.write_text(r"""
+#include <atomic>
+#include <cstdio>
+#include <mutex>
+#include <random>
+#include <thread>
+#include <vector>
+#include "bounded_wait.h"
+using namespace bivmoe;
+constexpr int SLOTS = 8, WARPS = 4;
+struct Bar {                            // an mbarrier of one arrival
+    std::mutex m; unsigned phase = 0;
+    void arrive() { std::lock_guard<std::mutex> l(m); phase++; }
+    bool test(unsigned parity) { std::lock_guard<std::mutex> l(m); return (phase & 1) != parity; }
+};
+int main() {
+    std::mt19937 rng(2);
+    for (int run = 0; run < 200; run++) {
+        const int total = rng() % 50, used = rng() % (total + 1);
+        Bar full[SLOTS], empty[SLOTS];
+        std::atomic<bool> stop{false};
+        std::atomic<int> bad{0};
+        std::vector<std::thread> roles;
+        for (int w = 0; w < WARPS; w++) {
+            const unsigned seed = rng();
+            roles.emplace_back([&, w, seed] {
+                std::mt19937 r(seed);
+                std::atomic<int> under_way{0};
+                std::vector<std::thread> copies;
+                uint32_t last = 0, fills = 0;
+                for (int gs = w; gs < total; gs += WARPS) {
+                    bool ok = true;
+                    while (!empty[gs % SLOTS].test(((gs / SLOTS) & 1) ^ 1) && (ok = !stop)) std::this_thread::yield();
+                    if (!ok) break;
+                    last = gs;
+                    fills++;
+                    under_way++;
+                    copies.emplace_back([&, gs, late = r() % 300] {
+                        std::this_thread::sleep_for(std::chrono::microseconds(late));
+                        under_way--;
+                        full[gs % SLOTS].arrive();
+                    });
+                }
+                wait_for_last_fills<SLOTS, WARPS>(last, fills, [&](uint32_t slot, uint32_t parity) {
+                    while (!full[slot].test(parity)) std::this_thread::yield();
+                });
+                if (under_way) bad = 1;                     // it would land in memory that is another block's
+                for (auto& c : copies) c.join();
+            });
+        }
+        for (int gs = 0; gs < used; gs++) {                 // the consumer, until it gives up
+            while (!full[gs % SLOTS].test((gs / SLOTS) & 1)) std::this_thread::yield();
+            empty[gs % SLOTS].arrive();
+        }
+        stop = true;
+        for (auto& r : roles) r.join();
+        if (bad) { printf("run %d\n", run); return 1; }
+    }
+    return 0;
+}
+""")
+    subprocess.run(["g++", "-std=c++17", "-O1", "-pthread", "-Wall", "-I", os.path.join(ROOT, "biv_b200", "csrc"), "-o", exe, str(src)],
+                   check=True)
+    r = subprocess.run([exe], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0, r.stdout
+    # and the kernel's copying warps end with it
+    with open(os.path.join(ROOT, "biv_b200", "csrc", "attend_tc.cu")) as f:
+        code = f.read()
+    role = code[code.index("// ---- copies"):code.index("// ---- products")]
+    assert "wait_for_last_fills<AT_SLOTS, AT_COPY_WARPS>(last, fills" in role[role.index("cp.async.wait_all"):]
