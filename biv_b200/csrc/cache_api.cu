@@ -23,8 +23,10 @@ struct bivmoe_cache {
     int32_t* arrived = nullptr;
     int32_t* status = nullptr;
     size_t arrived_bytes = 0;
-    // the stream of the last call that used the workspace; for the end of what it did
+    // the stream of the last call that used the workspace, those of calls before it that it could not wait for
+    // (they were being captured); for the end of what they did
     cudaStream_t last = nullptr;
+    std::vector<cudaStream_t> behind;
     cudaEvent_t done = nullptr;
     bool used = false;
 };
@@ -219,23 +221,49 @@ extern "C" int bivmoe_cache_store(bivmoe_cache* c, const bivmoe_store_args* a, v
     return e == cudaSuccess ? BIVMOE_OK : cuda_fail(e, "bivmoe_cache_store");
 }
 
+// Has s wait for what `of` has been given.  Not where `of` is captured, which cannot be waited for from outside
+// the capture: `waited` is then false.
+static cudaError_t wait_for(bivmoe_cache* c, cudaStream_t of, cudaStream_t s, bool& waited) {
+    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    cudaError_t e = cudaStreamIsCapturing(of, &cap);
+    if (e == cudaErrorStreamCaptureImplicit) {    // the legacy stream, while one that it would wait for is captured
+        cudaGetLastError();
+        cap = cudaStreamCaptureStatusActive;
+        e = cudaSuccess;
+    }
+    waited = e == cudaSuccess && cap == cudaStreamCaptureStatusNone;
+    if (!waited) return e;
+    e = cudaEventRecord(c->done, of);
+    return e == cudaSuccess ? cudaStreamWaitEvent(s, c->done, 0) : e;
+}
+
 // The workspace is one: a call on another stream than the last one's waits for what that stream had been
-// given.  Not where a stream is captured: an event from outside a capture cannot be waited for in it.
+// given.  Not where a stream is captured: an event from outside a capture cannot be waited for in it, and one
+// from inside not outside of it.  What the stream had been given before its capture is waited for by the first
+// call after it.
 // (An event after every call would let the last stream be destroyed in between, but it kept the next
 // kernel from being scheduled early: 14.3 us a call of one token at 1000 instead of 12.)
 static cudaError_t take_turn(bivmoe_cache* c, cudaStream_t s) {
     cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
-    cudaError_t e = cudaStreamIsCapturing(s, &cap);
+    const cudaError_t e = cudaStreamIsCapturing(s, &cap);
     if (e != cudaSuccess || cap != cudaStreamCaptureStatusNone) return e;
     if (c->used && c->last != s) {
-        e = cudaStreamIsCapturing(c->last, &cap);
-        if (e != cudaSuccess || cap != cudaStreamCaptureStatusNone) return e;
-        e = cudaEventRecord(c->done, c->last);
-        if (e == cudaSuccess) e = cudaStreamWaitEvent(s, c->done, 0);
+        try {
+            c->behind.push_back(c->last);
+        } catch (const std::bad_alloc&) {
+            return cudaErrorMemoryAllocation;
+        }
     }
     c->last = s;
     c->used = true;
-    return e;
+    for (size_t i = 0; i < c->behind.size();) {
+        bool ordered = c->behind[i] == s;         // by the stream itself
+        if (!ordered)
+            if (cudaError_t f = wait_for(c, c->behind[i], s, ordered)) return f;
+        if (ordered) c->behind.erase(c->behind.begin() + i);
+        else i++;
+    }
+    return cudaSuccess;
 }
 
 static Pool pool_of(const bivmoe_pool& p) {

@@ -374,8 +374,9 @@ BIVMOE_API int bivmoe_ep_peer_wait_limit(bivmoe_layer* layer, uint64_t microseco
  * Pointers need the alignment of their type; pools, and attend's q and out, 16 bytes, strides that
  * are multiples of 8 values there.  Strides are in values; the head_dim values of a row's head are
  * neighbours.  The attend calls of one handle use one workspace: on several streams the handle orders
- * them one after another (not while a stream is captured: there the caller does), for which the stream
- * of the last call has to exist still. */
+ * them one after another (not calls that are captured, nor a call with one on a stream that is being captured
+ * meanwhile: there the caller does, as for the replays of a graph), for which the stream of the last call, and one
+ * that was captured since its last call, have to exist still. */
 typedef struct bivmoe_cache bivmoe_cache;
 
 typedef struct bivmoe_cache_desc {

@@ -244,3 +244,41 @@ int main() {
         code = f.read()
     role = code[code.index("// ---- copies"):code.index("// ---- products")]
     assert "wait_for_last_fills<AT_SLOTS, AT_COPY_WARPS>(last, fills" in role[role.index("cp.async.wait_all"):]
+
+
+# ---- streams -----------------------------------------------------------------------------------------
+@pytest.mark.gpu
+def test_a_call_waits_for_all_before_it_after_a_capture():
+    # a call on A; while A is captured a call on B; after it one on C, which uses the workspace of both
+    b = Batch([1, 2], [300, 20], 4, 2, 64, BF16, 16)
+    c = cache(4, 2, 64, 16, 2, 8, BF16)
+    want = b.run(c)
+    outs = [torch.zeros_like(b.q) for _ in range(3)]
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    ends = [torch.cuda.Event() for _ in range(3)]
+    torch.cuda.synchronize()
+
+    def call(i, wait):
+        with torch.cuda.stream(streams[i]):
+            if wait:
+                torch.cuda._sleep(wait)
+            b.run(c, out=outs[i])
+            ends[i].record()
+
+    graph = torch.cuda.CUDAGraph()
+    call(0, 50_000_000)                     # some 25 ms
+    with torch.cuda.stream(streams[0]):
+        graph.capture_begin(capture_error_mode="relaxed")
+        x = torch.zeros(1, device=DEV)
+        call(1, 400_000_000)                # ends long after A's
+        x += 1
+        graph.capture_end()
+    call(2, 0)
+    ends[2].synchronize()
+    assert ends[0].query() and ends[1].query()
+    for o in outs:
+        assert torch.equal(o, want)
+    call(0, 400_000_000)                    # and once more without a capture
+    call(1, 0)
+    ends[1].synchronize()
+    assert ends[0].query()
