@@ -52,7 +52,7 @@ class Step(NamedTuple):
     slots: torch.Tensor       # [n_tokens] int64: page * page_size + place, -1 without a page
     positions: torch.Tensor   # [n_tokens] int32
     left: torch.Tensor        # [2] int32: free pages that remain, pages that were missing
-    held: torch.Tensor        # [n_seq] int32: pages of each request
+    held: torch.Tensor        # [n_seq] int32: pages that each request's tokens take, missing ones among them
 
 
 class PagedCache:
@@ -105,7 +105,9 @@ class PagedCache:
         new entries of ``table`` [n_seq, pages], and returns the step.  ``n_tokens`` rows are laid out:
         more than the requests add (a padded batch) have slot -1.  ``held``: pages each request holds
         already, where that is not what ``past`` needs (drafted tokens that were taken back); ``out``:
-        a step to write into."""
+        a step to write into.  Tokens that got no slot (``unstored``) are not stored and not seen later: such a
+        step is made again, from the same lists with more free pages at their end or a wider table, before its
+        lengths are used."""
         r = _cache_calls.extend(self._geometry, past, added, held, free_pages, free_count, table, n_tokens, out)
         if r.__class__ is int:
             capi.check(r)
@@ -135,3 +137,10 @@ class PagedCache:
         """Waits for the current stream and raises if a kernel of this cache gave up on a bounded wait
         since the last report."""
         capi.check(capi.lib().bivmoe_cache_status(self._h, torch.cuda.current_stream(self.device).cuda_stream))
+
+    def unstored(self) -> int:
+        """Waits for the current stream; how many new tokens of ``extend`` calls got no slot since the last
+        report: for want of a free page, in this call or in an earlier one, or of a place in the table."""
+        n = C.c_uint64()
+        capi.check(capi.lib().bivmoe_cache_unstored(self._h, C.byref(n), torch.cuda.current_stream(self.device).cuda_stream))
+        return n.value

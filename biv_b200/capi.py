@@ -32,7 +32,7 @@ SYMBOLS = ["bivmoe_create", "bivmoe_destroy", "bivmoe_forward", "bivmoe_forward_
            "bivmoe_ep_peer_combine", "bivmoe_status", "bivmoe_last_oom_bytes", "bivmoe_ep_peer_signal",
            "bivmoe_ep_peer_wait", "bivmoe_ep_peer_barrier", "bivmoe_ep_peer_wait_limit",
            "bivmoe_cache_create", "bivmoe_cache_destroy", "bivmoe_cache_extend", "bivmoe_cache_store",
-           "bivmoe_cache_attend", "bivmoe_cache_status"]
+           "bivmoe_cache_attend", "bivmoe_cache_status", "bivmoe_cache_unstored"]
 
 
 class BivMoeError(RuntimeError):
@@ -158,6 +158,7 @@ def lib():
         L.bivmoe_cache_store.argtypes = [vp, C.POINTER(StoreArgs), vp]
         L.bivmoe_cache_attend.argtypes = [vp, C.POINTER(AttendArgs), vp]
         L.bivmoe_cache_status.argtypes = [vp, vp]
+        L.bivmoe_cache_unstored.argtypes = [vp, C.POINTER(C.c_uint64), vp]
         L.bivmoe_launch_count.restype = C.c_uint64
         L.bivmoe_last_error.argtypes = [vp]
         L.bivmoe_last_error.restype = C.c_char_p

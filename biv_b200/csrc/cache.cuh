@@ -468,7 +468,7 @@ __device__ __noinline__ void careful_row(const AttendCall& a, const Piece& x, in
 
 cudaError_t launch_attend_few(const AttendCall& a, int head_dim, int ggml_type, int sm_count, cudaStream_t stream);
 cudaError_t launch_attend_tc(const AttendCall& a, int head_dim, int ggml_type, int sm_count, cudaStream_t stream);
-cudaError_t launch_extend(const bivmoe_extend_args& a, int page_size, int sm_count, cudaStream_t stream);
+cudaError_t launch_extend(const bivmoe_extend_args& a, int page_size, unsigned long long* unstored, int sm_count, cudaStream_t stream);
 cudaError_t launch_store(const bivmoe_store_args& a, const RopePlan& rope, int ggml_type, int heads, int heads_kv, int head_dim,
                          int page_size, int sm_count, cudaStream_t stream);
 // what the workspace is sized for: rows of a tile, blocks to a multiprocessor

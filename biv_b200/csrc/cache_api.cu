@@ -17,12 +17,13 @@ struct bivmoe_cache {
     bivmoe_cache_desc d{};
     int sm_count = 0;
     RopePlan rope{};
-    uint8_t* mem = nullptr;          // one allocation: parts, arrivals, the rope's tables, the status word
+    uint8_t* mem = nullptr;          // one allocation: parts, arrivals, the rope's tables, the status word, the count
     float* part_o = nullptr;
     float2* part_ml = nullptr;
     int32_t* arrived = nullptr;
     int32_t* status = nullptr;
     size_t arrived_bytes = 0;
+    unsigned long long *unstored = nullptr, reported = 0;   // tokens without a slot so far (device); up to the last report
     // the stream of the last call that used the workspace, those of calls before it that it could not wait for
     // (they were being captured); for the end of what they did
     cudaStream_t last = nullptr;
@@ -121,7 +122,7 @@ extern "C" int bivmoe_cache_create(const bivmoe_cache_desc* d, bivmoe_cache** ou
     size_t off = 0;
     auto take = [&off](size_t bytes) { const size_t at = off; off += (bytes + 255) & ~(size_t)255; return at; };
     const size_t o = take(rows * d->head_dim * 4), ml = take(rows * sizeof(float2)), tt = take(turns.size() * 8 + 8),
-                 ax = take(axis.size() * 4 + 4), arr = take(counts * 4), st = take(16);
+                 ax = take(axis.size() * 4 + 4), arr = take(counts * 4), st = take(16), un = take(8);
     c->arrived_bytes = counts * 4;
     e = dev_alloc((void**)&c->mem, off);
     if (e == cudaSuccess) e = cudaMemset(c->mem + arr, 0, off - arr);
@@ -139,6 +140,7 @@ extern "C" int bivmoe_cache_create(const bivmoe_cache_desc* d, bivmoe_cache** ou
     c->rope = RopePlan{d->n_rot, d->rope_adjacent, (const double*)(c->mem + tt), (const int32_t*)(c->mem + ax)};
     c->arrived = (int32_t*)(c->mem + arr);
     c->status = (int32_t*)(c->mem + st);
+    c->unstored = (unsigned long long*)(c->mem + un);
     *out = c;
     return BIVMOE_OK;
 }
@@ -188,7 +190,7 @@ extern "C" int bivmoe_cache_extend(bivmoe_cache* c, const bivmoe_extend_args* a,
             if (i.p && o.p && (uintptr_t)i.p < (uintptr_t)o.p + 4 * o.n && (uintptr_t)o.p < (uintptr_t)i.p + 4 * i.n)
                 return fail(BIVMOE_ERR_ARGUMENT, "a list that is written lies over one that is read");
     DeviceScope on_device(c->d.device);
-    const cudaError_t e = launch_extend(*a, c->d.page_size, c->sm_count, (cudaStream_t)stream);
+    const cudaError_t e = launch_extend(*a, c->d.page_size, c->unstored, c->sm_count, (cudaStream_t)stream);
     return e == cudaSuccess ? BIVMOE_OK : cuda_fail(e, "bivmoe_cache_extend");
 }
 
@@ -341,4 +343,18 @@ extern "C" int bivmoe_cache_status(bivmoe_cache* c, void* stream) {
     if (e == cudaSuccess) e = cudaStreamSynchronize(s);
     if (e != cudaSuccess) return cuda_fail(e, "bivmoe_cache_status");
     return fail(BIVMOE_ERR_TIMEOUT, "a bounded wait of the attention kernel gave up (%d)", word);
+}
+
+extern "C" int bivmoe_cache_unstored(bivmoe_cache* c, uint64_t* tokens, void* stream) {
+    if (!c || !tokens) return fail(BIVMOE_ERR_ARGUMENT, "null cache or output");
+    *tokens = 0;
+    DeviceScope on_device(c->d.device);
+    unsigned long long now = 0;           // the count is never set back: calls on other streams may be adding to it
+    const cudaStream_t s = (cudaStream_t)stream;
+    cudaError_t e = cudaMemcpyAsync(&now, c->unstored, 8, cudaMemcpyDeviceToHost, s);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+    if (e != cudaSuccess) return cuda_fail(e, "bivmoe_cache_unstored");
+    *tokens = now - c->reported;
+    c->reported = now;
+    return BIVMOE_OK;
 }

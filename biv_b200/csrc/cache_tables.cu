@@ -19,6 +19,7 @@ constexpr int kExtendEach = kCacheSeqs / kExtendThreads;
 struct ExtendCall {
     bivmoe_extend_args a;
     FastDiv page;
+    unsigned long long* unstored;    // of the handle: new tokens without a slot so far
 };
 
 __device__ __forceinline__ int last_at_or_before(const int* first, int n, int v) {
@@ -98,6 +99,7 @@ __global__ void __launch_bounds__(kExtendThreads) extend_kernel(ExtendCall c) {
         const int b = last_at_or_before(s_page, n, i), at = s_have[b] + i - s_page[b];
         if (at < a.table_width) a.table[b * a.table_stride + at] = i < count ? a.free_pages[count - 1 - i] : -1;
     }
+    int lost = me == 0 ? max(all_t - a.n_tokens, 0) : 0;
     for (int t = me; t < a.n_tokens; t += step) {
         int64_t slot = -1;
         int p = 0;
@@ -111,14 +113,17 @@ __global__ void __launch_bounds__(kExtendThreads) extend_kernel(ExtendCall c) {
                 const int page = at < s_have[b] ? a.table[b * a.table_stride + at] : given ? a.free_pages[count - 1 - i] : -1;
                 if (page >= 0) slot = (int64_t)page * c.page.d + (p - at * (int)c.page.d);
             }
+            lost += slot < 0;
         }
         a.slots[t] = slot;
         a.positions[t] = p;
     }
+    lost = __reduce_add_sync(0xffffffffu, lost);
+    if (lane == 0 && lost) atomicAdd(c.unstored, (unsigned long long)lost);
 }
 
-cudaError_t launch_extend(const bivmoe_extend_args& a, int page_size, int sm_count, cudaStream_t stream) {
-    ExtendCall c{a, FastDiv((uint32_t)page_size)};
+cudaError_t launch_extend(const bivmoe_extend_args& a, int page_size, unsigned long long* unstored, int sm_count, cudaStream_t stream) {
+    ExtendCall c{a, FastDiv((uint32_t)page_size), unstored};
     // a few rows a thread: more blocks only repeat the sums
     const int blocks = (int)min((int64_t)sm_count, ((int64_t)a.n_tokens + 2 * kExtendThreads - 1) / (2 * kExtendThreads) + 1);
     count_launch();

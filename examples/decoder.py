@@ -113,9 +113,9 @@ def main():
     torch.cuda.synchronize()
     t = time.perf_counter() - t
     d.cache.status()
-    left, missing = last.left.tolist()
+    left, lost = int(last.left[0]), d.cache.unstored()
     print(f"prompts of {lengths} tokens, then {a.tokens} steps of {a.requests} tokens through {a.layers} layers: "
-          f"{t / a.tokens * 1e6:.0f} us a step; lengths {d.past.tolist()}, {left} pages left, {missing} missing, "
+          f"{t / a.tokens * 1e6:.0f} us a step; lengths {d.past.tolist()}, {left} pages left, {lost} tokens without one, "
           f"rows finite: {bool(rows.isfinite().all())}")
     d.close()
 

@@ -423,7 +423,14 @@ BIVMOE_API void bivmoe_cache_destroy(bivmoe_cache* cache);
  * first[n_seq], their number; for each of the n_tokens rows its slot (page * page_size + place; -1
  * without a page and for rows past first[n_seq]) and its position (0 there); left[0] = what remains
  * of the free list, left[1] = how many pages were missing; held_out[b] (may be null) = the pages
- * request b holds now.  The lists given are not changed: the next call's past is this call's length. */
+ * that request b's tokens take, whether or not there was one.  The lists given are not changed: the next
+ * call's past is this call's length.
+ * A new token gets no slot where the free list had no page for it, where an earlier call had none (the
+ * table has -1 there, and it is not asked for again), or where its page's place lies past table_width (the page
+ * leaves the free list all the same, and is written nowhere); bivmoe_cache_unstored counts them.  Its k and v are
+ * not stored and not seen later.  A step with such tokens is therefore better made again before its lengths are
+ * used: the same call, from the same lists, with pages added at the free list's end or a wider table, gives
+ * every token its slot, and no page is lost. */
 typedef struct bivmoe_extend_args {
     const int32_t *past, *added, *held;      /* device, [n_seq]; held may be null */
     const int32_t *free_pages, *free_count;  /* device, [n_free], [1] */
@@ -434,6 +441,10 @@ typedef struct bivmoe_extend_args {
     int64_t* slots;                          /* device, [n_tokens] */
 } bivmoe_extend_args;
 BIVMOE_API int bivmoe_cache_extend(bivmoe_cache* cache, const bivmoe_extend_args* args, void* stream);
+
+/* Waits for the stream; how many new tokens of the handle's extend calls have been given no slot since the
+ * last report (those past n_tokens, for which no rows were laid out, among them). */
+BIVMOE_API int bivmoe_cache_unstored(bivmoe_cache* cache, uint64_t* tokens, void* stream);
 
 /* q and k turned by the tokens' positions, q to q_out, k and v into the pages at the tokens' slots
  * (a negative slot, or one past the pool: only q).  positions [axes][positions_stride] int32, or null

@@ -6,7 +6,7 @@ import subprocess
 import pytest
 import torch
 
-from test_cache import BF16, DEV, F16, ROOT, Batch, cache, near
+from test_cache import BF16, DEV, F16, ROOT, Batch, cache, ints, near
 
 
 # ---- values that are not finite ----------------------------------------------------------------------
@@ -282,3 +282,48 @@ def test_a_call_waits_for_all_before_it_after_a_capture():
     call(1, 0)
     ends[1].synchronize()
     assert ends[0].query()
+
+
+# ---- lists that run out ------------------------------------------------------------------------------
+@pytest.mark.gpu
+def test_tokens_without_a_page_are_counted_and_the_step_can_be_made_again():
+    # three requests of pages of 4: 6, 1 and 5 new tokens on 0, 4 and 3; four pages are needed, two are there
+    c = cache(4, 2, 64, 4, 3, 16, BF16)
+    past, added, free = ints([0, 4, 3]), ints([6, 1, 5]), ints([9, 8, 7])
+    table = torch.full((3, 3), -1, dtype=torch.int32, device=DEV)
+    table[1, 0], table[2, 0] = 5, 6
+    s = c.extend(past, added, free[:2], ints([2]), table, 13)
+    assert s.left.tolist() == [0, 2] and s.slots.tolist() == [32, 33, 34, 35, 36, 37, -1, 27] + [-1] * 5
+    assert c.unstored() == 1 + 4 and c.unstored() == 0
+    # going on all the same: nothing new is needed, and the rows are lost without a missing page
+    t = c.extend(s.length, ints([0, 2, 0]), free, ints([1]), table, 2, held=s.held)
+    assert t.left.tolist() == [1, 0] and t.slots.tolist() == [-1, -1] and c.unstored() == 2
+    # made again, with pages added at the end: what it needs is what it gets
+    free = ints([9, 8, 7, 3])
+    s = c.extend(past, added, free, ints([4]), table, 13)
+    assert s.left.tolist() == [0, 0] and s.held.tolist() == [2, 2, 2] and c.unstored() == 0
+    assert table.tolist() == [[3, 7, -1], [5, 8, -1], [6, 9, -1]]
+    assert s.slots.tolist() == [12, 13, 14, 15, 28, 29, 32, 27, 36, 37, 38, 39, -1]
+
+
+@pytest.mark.gpu
+def test_tokens_past_the_table_or_the_rows_are_counted():
+    c = cache(1, 1, 64, 4, 2, 16, BF16)
+    past, added, free, count = ints([4, 0]), ints([5, 3]), ints([1, 2, 3]), ints([3])
+    narrow = torch.full((2, 2), -1, dtype=torch.int32, device=DEV)
+    narrow[0, 0] = 0
+    s = c.extend(past, added, free, count, narrow, 8)
+    assert s.slots.tolist() == [12, 13, 14, 15, -1, 4, 5, 6] and c.unstored() == 1
+    wide = torch.full((2, 3), -1, dtype=torch.int32, device=DEV)
+    wide[0, 0] = 0
+    s = c.extend(past, added, free, count, wide, 8)      # again, with room: the same pages, none lost
+    assert s.slots.tolist() == [12, 13, 14, 15, 8, 4, 5, 6] and s.left.tolist() == [0, 0] and c.unstored() == 0
+    c.extend(past, added, free, count, wide, 6)          # two of eight tokens have no rows
+    assert c.unstored() == 2
+    graph = torch.cuda.CUDAGraph()
+    c.extend(past, added, free, count, narrow, 8, out=s)
+    with torch.cuda.graph(graph):
+        c.extend(past, added, free, count, narrow, 8, out=s)
+    for _ in range(5):
+        graph.replay()
+    assert c.unstored() == 6                             # every replay's
