@@ -115,7 +115,7 @@ class PagedCache:
 
     def store(self, q, k, v, k_pool, v_pool, slots, positions=None, out=None):
         """q and k [n, heads, head_dim] (float32, float16 or bfloat16; any strides of the first two)
-        turned by ``positions`` ([n], or [axes, n]), k and v into the pages at ``slots``; returns the
+        turned by ``positions`` ([n], or [axes, n], which may be one row expanded), k and v into the pages at ``slots``; returns the
         turned q in the cache's type."""
         r = _cache_calls.store(self._geometry, q, k, v, k_pool, v_pool, slots, positions, out)
         if r.__class__ is int:

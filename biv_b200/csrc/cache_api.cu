@@ -214,7 +214,7 @@ extern "C" int bivmoe_cache_store(bivmoe_cache* c, const bivmoe_store_args* a, v
     if (!a->slots || !aligned(a->slots, 8)) return fail(BIVMOE_ERR_ARGUMENT, "slots: null or not aligned");
     if (c->d.n_rot) {
         if (!a->positions || !aligned(a->positions, 4)) return fail(BIVMOE_ERR_ARGUMENT, "positions: null or not aligned");
-        if (c->d.rope_axes > 1 && a->positions_stride < a->n_tokens)
+        if (c->d.rope_axes > 1 && a->positions_stride && a->positions_stride < a->n_tokens)
             return fail(BIVMOE_ERR_ARGUMENT, "positions_stride %lld below n_tokens = %d", (long long)a->positions_stride, a->n_tokens);
     }
     DeviceScope on_device(c->d.device);

@@ -447,8 +447,8 @@ BIVMOE_API int bivmoe_cache_extend(bivmoe_cache* cache, const bivmoe_extend_args
 BIVMOE_API int bivmoe_cache_unstored(bivmoe_cache* cache, uint64_t* tokens, void* stream);
 
 /* q and k turned by the tokens' positions, q to q_out, k and v into the pages at the tokens' slots
- * (a negative slot, or one past the pool: only q).  positions [axes][positions_stride] int32, or null
- * where n_rot is 0.  Computed in f32 (the angle in f64, in turns), rounded once. */
+ * (a negative slot, or one past the pool: only q).  positions [axes][positions_stride] int32 (stride 0: one row
+ * for all axes), or null where n_rot is 0.  Computed in f32 (the angle in f64, in turns), rounded once. */
 typedef struct bivmoe_store_args {
     bivmoe_rows q, k, v, q_out;
     bivmoe_pool k_pool, v_pool;

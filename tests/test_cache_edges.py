@@ -6,7 +6,7 @@ import subprocess
 import pytest
 import torch
 
-from test_cache import BF16, DEV, F16, ROOT, Batch, cache, ints, near
+from test_cache import BF16, DEV, F16, ROOT, UNIT, Batch, cache, ints, near, turned64
 
 
 # ---- values that are not finite ----------------------------------------------------------------------
@@ -327,3 +327,22 @@ def test_tokens_past_the_table_or_the_rows_are_counted():
     for _ in range(5):
         graph.replay()
     assert c.unstored() == 6                             # every replay's
+
+
+# ---- rows that are views -----------------------------------------------------------------------------
+@pytest.mark.gpu
+def test_positions_may_be_expanded_over_the_axes():
+    # text tokens: the same position on every axis, one row of memory
+    from biv_b200.cache import Rope
+    rope, n = Rope(64, 1e6, [12, 10, 10], True), 33
+    c = cache(4, 2, 64, 16, 1, n, BF16, rope=rope)
+    x = torch.randn((n, 8, 64), generator=torch.Generator(device=DEV).manual_seed(2), device=DEV)
+    k, v = [p.zero_() for p in c.pools(3)]
+    pos = torch.arange(1000, 1000 + n, device=DEV, dtype=torch.int32)
+    slots = torch.arange(n, device=DEV)
+    got = c.store(x[:, :4], x[:, 4:6], x[:, 6:], k, v, slots, pos.expand(3, n))
+    want = turned64(x[:, :4], pos.expand(3, n), rope, 64)
+    # one rounding, and a turn in f32 before it (2^-21 of values of at most 8)
+    assert bool(((got.double() - want).abs() <= UNIT[BF16] * want.abs() + 2.0 ** -21 * 8).all())
+    again = c.store(x[:, :4], x[:, 4:6], x[:, 6:], k, v, slots, pos.expand(3, n).contiguous())
+    assert torch.equal(got, again)
