@@ -51,19 +51,22 @@ Table table(const Geometry& g, PyObject* o, int64_t n_seq) {
         throw Wrong{"table: [n_seq, pages] int32 with neighbouring pages is wanted"};
     return {(int32_t*)t.data_ptr(), t.stride(0), (int32_t)t.size(1)};
 }
+// A dimension's stride; where there is one place or none, which torch may give any stride, `dense`.
+int64_t stride(const at::Tensor& t, int dim, int64_t dense) { return t.size(dim) > 1 ? t.stride(dim) : dense; }
 bivmoe_pool pool(const Geometry& g, PyObject* o, const char* what) {
     const at::Tensor& t = tensor(o, what);
     if (t.scalar_type() != g.type || !here(g, t) || t.dim() != 4 || t.size(1) != g.page_size || t.size(2) != g.n_head_kv ||
         t.size(3) != g.head_dim || t.stride(3) != 1)
         throw Wrong{std::string(what) + ": [pages, " + std::to_string(g.page_size) + ", " + std::to_string(g.n_head_kv) + ", " +
                     std::to_string(g.head_dim) + "] of the cache's type is wanted"};
-    return {t.data_ptr(), t.stride(0), t.stride(1), t.stride(2), t.size(0)};
+    const int64_t token = (int64_t)g.n_head_kv * g.head_dim;
+    return {t.data_ptr(), stride(t, 0, g.page_size * token), stride(t, 1, token), stride(t, 2, g.head_dim), t.size(0)};
 }
 bivmoe_rows rows(const Geometry& g, const at::Tensor& t, const char* what, int heads, int64_t n, int ggml_type) {
     if (!here(g, t) || t.dim() != 3 || t.size(0) != n || t.size(1) != heads || t.size(2) != g.head_dim || t.stride(2) != 1)
         throw Wrong{std::string(what) + ": [tokens, " + std::to_string(heads) + ", " + std::to_string(g.head_dim) +
                     "] rows on the cache's device are wanted"};
-    return {t.data_ptr(), t.stride(0), t.stride(1), ggml_type, 0};
+    return {t.data_ptr(), stride(t, 0, (int64_t)heads * g.head_dim), stride(t, 1, g.head_dim), ggml_type, 0};
 }
 int32_t count(int64_t n, const char* what) {
     if (n < 0 || n > INT32_MAX) throw Wrong{std::string(what) + ": out of range"};

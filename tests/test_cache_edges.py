@@ -346,3 +346,23 @@ def test_positions_may_be_expanded_over_the_axes():
     assert bool(((got.double() - want).abs() <= UNIT[BF16] * want.abs() + 2.0 ** -21 * 8).all())
     again = c.store(x[:, :4], x[:, 4:6], x[:, 6:], k, v, slots, pos.expand(3, n).contiguous())
     assert torch.equal(got, again)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new", [1, 40])
+def test_strides_of_a_single_token_head_or_page_do_not_count(new):
+    # where there is one of something, its stride says nothing, and torch leaves it at anything
+    def odd(t):      # the same memory; strides of 1 and 3 where a dimension has one place
+        return t.as_strided(t.shape, [s if n > 1 else 1 + 2 * (i & 1) for i, (n, s) in enumerate(zip(t.shape, t.stride()))])
+
+    b = Batch([new], [0], 1, 1, 64, BF16, 64)
+    c = cache(1, 1, 64, 64, 1, 64, BF16)
+    want = b.run(c)
+    out = torch.zeros_like(b.q)
+    k, v = [x[b.table[0, :1].long()].contiguous() for x in (b.k, b.v)]
+    got = c.attend(odd(b.q), odd(k), odd(v), ints([[0]]), b.first, b.length, out=odd(out))
+    assert torch.equal(got, want) and torch.equal(out, want)
+    rows = torch.randn((new, 1, 64), device=DEV)
+    slots = torch.arange(new, device=DEV)
+    q = c.store(odd(rows), odd(rows), odd(rows), odd(k), odd(v), slots, out=odd(out))
+    assert torch.equal(q, rows.to(BF16)) and torch.equal(k[0, :new], rows.to(BF16))
