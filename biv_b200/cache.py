@@ -25,7 +25,7 @@ try:
     from . import _cache_calls
 except ImportError as e:
     raise ImportError("biv_b200/_cache_calls.so is missing or was built for another torch: build it with `python -c "
-                      "'import __graft_entry__ as g; g.build()'` (or `make -C biv_b200/csrc`); there is no fallback") from e
+                      "'import __graft_entry__ as g; g.build()'` (or `make -C biv_b200/csrc all`); there is no fallback") from e
 
 _GGML = {torch.float16: 1, torch.bfloat16: 30}
 

@@ -366,3 +366,13 @@ def test_strides_of_a_single_token_head_or_page_do_not_count(new):
     slots = torch.arange(new, device=DEV)
     q = c.store(odd(rows), odd(rows), odd(rows), odd(k), odd(v), slots, out=odd(out))
     assert torch.equal(q, rows.to(BF16)) and torch.equal(k[0, :new], rows.to(BF16))
+
+
+# ---- the build ---------------------------------------------------------------------------------------
+def test_the_library_is_built_without_python():
+    # the default target is what a caller of the C ABI needs: no interpreter is asked for anything
+    make = ["make", "-n", "-B", "-C", os.path.join(ROOT, "biv_b200", "csrc"), "PYTHON=/nowhere/python"]
+    r = subprocess.run(make, capture_output=True, text=True)
+    assert r.returncode == 0 and "libbivmoe.so" in r.stdout and "_cache_calls" not in r.stdout and "nowhere" not in r.stderr
+    r = subprocess.run(make[:-1] + ["all"], capture_output=True, text=True)
+    assert r.returncode == 0 and "libbivmoe.so" in r.stdout and "_cache_calls.so" in r.stdout
