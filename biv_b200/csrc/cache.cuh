@@ -69,7 +69,7 @@ struct AttendCall {
 struct Request {
     int begin, rows, past;           // first row (token), rows * group, position of the first row's token
 };
-__device__ __forceinline__ Request request_of(const AttendCall& a, int b) {
+__host__ __device__ __forceinline__ Request request_of(const AttendCall& a, int b) {
     const int f0 = a.first[b], f1 = a.first[b + 1], len = a.length[b];
     const int lo = max(f0, 0), hi = min(f1, a.n_tokens);
     Request r;
@@ -83,9 +83,9 @@ __device__ __forceinline__ Request request_of(const AttendCall& a, int b) {
 // consecutive ones from `from` on.
 struct TileList {
     int ns, from, n;
-    __device__ __forceinline__ int tile(int i) const { return i < ns ? i : i - ns + from; }
+    __host__ __device__ __forceinline__ int tile(int i) const { return i < ns ? i : i - ns + from; }
 };
-template <int KT> __device__ __forceinline__ TileList tiles_of(const AttendCall& a, int p0, int p1) {
+template <int KT> __host__ __device__ __forceinline__ TileList tiles_of(const AttendCall& a, int p0, int p1) {
     TileList t{0, 0, 0};
     if (p1 < 0) return t;
     const int last = p1 / KT;
@@ -125,22 +125,46 @@ __device__ __forceinline__ int page_of(const AttendCall& a, const int32_t* row, 
 // that others share, so that the room for pieces is two to a block.  Every block finds its share by
 // itself from the lengths: no list in memory, no launch before.
 // a / b for a >= 0, b > 0; most are short
-__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+__host__ __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
     return (a | b) >> 31 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
+}
+// (the shares' arithmetic is tested on the host, where the block is this one)
+inline int& host_block() {
+    static thread_local int block = 0;
+    return block;
 }
 struct Share {
     int64_t lo, hi;                  // this block's units
     int64_t each, longer;            // units of a block; those of the first blocks, which have one more
     const int64_t* before;           // shared, [n_seq + 1]: units of the requests before
+    __host__ __device__ __forceinline__ int block() const {
+#ifdef __CUDA_ARCH__
+        return (int)blockIdx.x;
+#else
+        return host_block();
+#endif
+    }
+    // this block's of `units`, of which `least` are worth a block, shared out over up to `blocks`
+    __host__ __device__ __forceinline__ void take(int64_t units, int least, int blocks) {
+        const int64_t worth = quotient(units + least - 1, least);
+        const int g = (int)(worth < blocks ? worth : blocks), c = block();
+        lo = hi = each = longer = 0;
+        if (c >= g) return;
+        each = quotient(units, g);
+        const int more = (int)(units - each * g);
+        longer = more * (each + 1);
+        lo = each * c + min(c, more);
+        hi = lo + each + (c < more);
+    }
     // the block that has unit u
-    __device__ __forceinline__ int owner(int64_t u) const {
+    __host__ __device__ __forceinline__ int owner(int64_t u) const {
         return u < longer ? (int)quotient(u, each + 1) : (int)(quotient(longer, each + 1) + quotient(u - longer, each));
     }
 };
-template <int KT, int TR> __device__ __forceinline__ TileList tile_list(const AttendCall& a, const Request& r, int t) {
+template <int KT, int TR> __host__ __device__ __forceinline__ TileList tile_list(const AttendCall& a, const Request& r, int t) {
     return tiles_of<KT>(a, r.past + (int)a.group.div(t * TR), r.past + (int)a.group.div(min((t + 1) * TR, r.rows) - 1));
 }
-template <int KT, int TR, int EXTRA> __device__ __forceinline__ int tile_units(const AttendCall& a, const Request& r, int t) {
+template <int KT, int TR, int EXTRA> __host__ __device__ __forceinline__ int tile_units(const AttendCall& a, const Request& r, int t) {
     return EXTRA + max(tile_list<KT, TR>(a, r, t).n, 1);
 }
 constexpr size_t share_smem(int n_seq, int threads) { return (((size_t)n_seq + 1 + threads / 32) * 8 + 15) / 16 * 16; }
@@ -189,16 +213,7 @@ __device__ __forceinline__ Share find_share(const AttendCall& a, int least, int6
     __syncthreads();
     Share s;
     s.before = before;
-    const int64_t worth = quotient(carry + least - 1, least);
-    const int g = (int)(worth < gridDim.x ? worth : gridDim.x);
-    s.lo = s.hi = s.each = s.longer = 0;
-    if ((int)blockIdx.x < g) {
-        s.each = quotient(carry, g);
-        const int more = (int)(carry - s.each * g), c = (int)blockIdx.x;
-        s.longer = more * (s.each + 1);
-        s.lo = s.each * c + min(c, more);
-        s.hi = s.lo + s.each + (c < more);
-    }
+    s.take(carry, least, (int)gridDim.x);
     return s;
 }
 struct Piece {
@@ -210,7 +225,7 @@ struct Piece {
     int c0;                          // the block that has the first one
     // where a piece's unfinished sums stand: a block is the first of at most one cut tile, and has
     // at most one piece of a tile that began before it
-    __device__ __forceinline__ int slot(int p) const { return p == 0 ? 2 * c0 + 1 : 2 * (c0 + p); }
+    __host__ __device__ __forceinline__ int slot(int p) const { return p == 0 ? 2 * c0 + 1 : 2 * (c0 + p); }
 };
 // The pieces of a block's share, one after another: every warp goes through them by itself.
 // A share's end that lies at most SNAP units behind a tile's beginning, or before its end, is moved there:
@@ -222,7 +237,7 @@ template <int KT, int TR, int EXTRA, int SNAP> struct Walk {
     int64_t at;                      // the next unit
     int b, head, t, nt, off;         // where it lies: of which tile, and how far in
     Request r;
-    __device__ __forceinline__ Walk(const AttendCall& call, const Share& share) : a(call), s(share), at(share.lo) {
+    __host__ __device__ __forceinline__ Walk(const AttendCall& call, const Share& share) : a(call), s(share), at(share.lo) {
         if (at >= s.hi) return;
         int lo = 0, hi = a.n_seq;    // the request: the last one that begins at or before the unit
         while (hi - lo > 1) {
@@ -233,8 +248,23 @@ template <int KT, int TR, int EXTRA, int SNAP> struct Walk {
         const int64_t rest = at - s.before[b], each = quotient(s.before[b + 1] - s.before[b], a.heads_kv);
         head = (int)quotient(rest, each);
         int64_t in = rest - head * each;
+        find_tile(in);
+        off = (int)in;
+        const int units = tile_units<KT, TR, EXTRA>(a, r, t);
+        if (off <= SNAP) {
+            at -= off;
+            off = 0;
+        } else if (units - off <= SNAP) {
+            at += units - off;
+            step();
+        }
+    }
+    // t: the tile that has unit `in` of its request's head, and which of its own units that is
+    __host__ __device__ __forceinline__ void find_tile(int64_t& in) {
+        t = 0;
+#ifdef __CUDA_ARCH__
         const int lane = threadIdx.x & 31;
-        for (t = 0; nt > 1 && t < nt;) {   // the tile: 32 of them at a time
+        while (nt > 1 && t < nt) {   // 32 of them at a time
             const int mine = t + lane < nt ? tile_units<KT, TR, EXTRA>(a, r, t + lane) : 0;
             int64_t x = mine;
             for (int d = 1; d < 32; d <<= 1) {
@@ -251,23 +281,17 @@ template <int KT, int TR, int EXTRA, int SNAP> struct Walk {
             in -= __shfl_sync(0xffffffffu, x, 31);
             t += 32;
         }
-        off = (int)in;
-        const int units = tile_units<KT, TR, EXTRA>(a, r, t);
-        if (off <= SNAP) {
-            at -= off;
-            off = 0;
-        } else if (units - off <= SNAP) {
-            at += units - off;
-            step();
-        }
+#else
+        for (int u; nt > 1 && in >= (u = tile_units<KT, TR, EXTRA>(a, r, t)); t++) in -= u;
+#endif
     }
-    __device__ __forceinline__ void open(int request) {
+    __host__ __device__ __forceinline__ void open(int request) {
         b = request;
         r = request_of(a, b);
         nt = (r.rows + TR - 1) / TR;
     }
     // to the beginning of the tile that follows, at `at`
-    __device__ __forceinline__ void step() {
+    __host__ __device__ __forceinline__ void step() {
         off = 0;
         if (++t < nt) return;
         t = 0;
@@ -279,7 +303,7 @@ template <int KT, int TR, int EXTRA, int SNAP> struct Walk {
         open(next);
     }
     // The next piece; false at the share's end.
-    __device__ __forceinline__ bool next(Piece& x) {
+    __host__ __device__ __forceinline__ bool next(Piece& x) {
         if (at >= s.hi) return false;
         x.tiles = tile_list<KT, TR>(a, r, t);
         const int units = EXTRA + max(x.tiles.n, 1);
@@ -302,11 +326,11 @@ template <int KT, int TR, int EXTRA, int SNAP> struct Walk {
         x.n = min(end - EXTRA, x.tiles.n) - x.i0;
         x.part = 0;
         x.parts = 1;
-        x.c0 = (int)blockIdx.x;
+        x.c0 = s.block();
         if (off > 0 || end < units) {
             x.c0 = s.owner(u0 + SNAP);
             x.parts = s.owner(u0 + units - SNAP - 1) - x.c0 + 1;
-            x.part = (int)blockIdx.x - x.c0;
+            x.part = s.block() - x.c0;
         }
         at = u0 + end;
         off = end;

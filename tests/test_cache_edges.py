@@ -376,3 +376,122 @@ def test_the_library_is_built_without_python():
     assert r.returncode == 0 and "libbivmoe.so" in r.stdout and "_cache_calls" not in r.stdout and "nowhere" not in r.stderr
     r = subprocess.run(make[:-1] + ["all"], capture_output=True, text=True)
     assert r.returncode == 0 and "libbivmoe.so" in r.stdout and "_cache_calls.so" in r.stdout
+
+
+# ---- the shares of the work --------------------------------------------------------------------------
+SHARES = r"""
+#include <cstdio>
+#include <map>
+#include <random>
+#include <set>
+#include <tuple>
+#include <vector>
+#include "cache.cuh"
+using namespace bivmoe;
+static int bad;
+#define CHECK(x) do { if (!(x)) { printf("line %d: %s (batch %d)\n", __LINE__, #x, batch); if (++bad > 5) return; } } while (0)
+
+// The pieces that the blocks take of random batches, by the kernels' own code.
+template <int KT, int TR, int EXTRA, int SNAP, int LEAST> void check(int blocks, unsigned seed) {
+    std::mt19937 rng(seed);
+    auto up_to = [&](int n) { return (int)(rng() % (n + 1)); };
+    for (int batch = 0; batch < 120; batch++) {
+        AttendCall a{};
+        a.n_seq = 1 + up_to(batch % 3 ? 30 : 3);
+        a.heads_kv = 1 + up_to(7);
+        a.group = FastDiv(1 + up_to(16));
+        a.window = up_to(2) ? 0 : 1 + up_to(3000);
+        a.sinks = up_to(300);
+        std::vector<int32_t> first(1, 0), length;
+        for (int b = 0; b < a.n_seq; b++) {
+            const int rows = up_to(2) ? up_to(3) : up_to(400), past = up_to(3) ? up_to(5000) : up_to(60000);
+            first.push_back(first.back() + rows);
+            length.push_back(past + rows - (up_to(9) ? 0 : 1 + up_to(past + rows)));     // rows before the beginning
+        }
+        a.n_tokens = first.back() - (up_to(9) ? 0 : up_to(first.back()));               // fewer rows than the lists say
+        a.first = first.data();
+        a.length = length.data();
+        std::vector<int64_t> before(1, 0);
+        std::set<std::tuple<int, int, int>> tiles;
+        for (int b = 0; b < a.n_seq; b++) {
+            const Request r = request_of(a, b);
+            int64_t units = 0;
+            for (int t = 0; t * TR < r.rows; t++) {
+                units += tile_units<KT, TR, EXTRA>(a, r, t);
+                for (int h = 0; h < a.heads_kv; h++) tiles.insert({b, h, t});
+            }
+            before.push_back(before.back() + units * a.heads_kv);
+        }
+        std::map<std::tuple<int, int, int>, std::vector<Piece>> found;
+        std::set<int> places, counts;
+        int64_t most = 0, total = 0;
+        for (int block = 0; block < blocks; block++) {
+            Share s{};
+            host_block() = block;
+            s.before = before.data();
+            s.take(before.back(), LEAST, blocks);
+            CHECK(s.lo == total || s.lo == s.hi);
+            total += s.hi - s.lo;
+            for (int64_t u = s.lo; u < s.hi; u += 1 + up_to(5)) CHECK(s.owner(u) == block);
+            Walk<KT, TR, EXTRA, SNAP> walk(a, s);
+            int64_t mine = 0;
+            for (Piece x; walk.next(x);) {
+                found[{x.b, x.head, x.row0 / TR}].push_back(x);
+                mine += EXTRA + x.n;
+                CHECK(x.row0 % TR == 0 && x.part == block - x.c0);
+                CHECK(x.rows == std::min(TR, x.r.rows - x.row0) && x.rows > 0);
+                if (x.parts == 1) continue;
+                CHECK(x.slot(x.part) >= 0 && x.slot(x.part) < 2 * blocks);              // the workspace: two to a block
+                CHECK(places.insert(x.slot(x.part)).second);
+                if (x.part == 0) CHECK(counts.insert(x.c0).second && x.c0 < blocks);    // a tile's count of arrivals is its own
+            }
+            most = std::max(most, mine);
+        }
+        CHECK(total == before.back());
+        CHECK(found.size() == tiles.size());
+        for (auto& f : found) {                       // every key tile of every tile is in one piece
+            std::vector<Piece>& p = f.second;
+            CHECK(tiles.count(f.first) && (int)p.size() == p[0].parts);
+            int next = 0;
+            for (size_t i = 0; i < p.size(); i++) {   // (the blocks were gone through in order)
+                CHECK(p[i].part == (int)i && p[i].parts == p[0].parts && p[i].c0 == p[0].c0 && p[i].tiles.n == p[0].tiles.n);
+                CHECK(p[i].i0 == next && (p[i].n > 0 || (p.size() == 1 && p[0].tiles.n == 0)));
+                next += p[i].n;
+            }
+            CHECK(next == p[0].tiles.n);
+            // and no key that a row sees is in another tile
+            const Piece& x = p[0];
+            const int p0 = x.r.past + (int)a.group.div(x.row0), p1 = x.r.past + (int)a.group.div(x.row0 + x.rows - 1);
+            std::set<int> list;
+            for (int i = 0; i < x.tiles.n; i++) CHECK(list.insert(x.tiles.tile(i)).second);
+            for (int k = 0; k < 20; k++) {
+                const int row = p0 + up_to(p1 - p0), j = row < 0 ? 0 : up_to(row);
+                const bool sees = j <= row && (a.window <= 0 || row - j < a.window || j < a.sinks);
+                if (sees) CHECK(list.count(j / KT));
+            }
+        }
+        // a block's pieces are its share, apart from ends that were moved and what a tile costs besides
+        CHECK(most <= (before.back() + blocks - 1) / blocks + LEAST + 2 * SNAP + EXTRA);
+    }
+}
+int main() {
+    check<64, 16, 1, 1, 2>(148, 1);       // tiles of 16 rows, one to three blocks a multiprocessor
+    check<64, 16, 1, 1, 2>(444, 2);
+    check<128, 256, 3, 5, 1>(148, 3);     // tcgen05, heads of up to 128 and of 256
+    check<128, 128, 4, 6, 1>(148, 4);
+    check<128, 128, 0, 1, 1>(7, 5);
+    check<64, 16, 2, 6, 4>(33, 6);
+    printf("done\n");
+    return bad;
+}
+"""
+
+
+def test_the_kernels_own_shares_cover_every_tile_once(tmp_path):
+    src, exe = tmp_path / "shares.cu", str(tmp_path / "shares")
+    src.write_text(SHARES)
+    nvcc = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
+    subprocess.run([nvcc, "-std=c++17", "-O1", "-gencode", "arch=compute_100a,code=sm_100a", "-I",
+                    os.path.join(ROOT, "biv_b200", "csrc"), "-o", exe, str(src)], check=True)
+    r = subprocess.run([exe], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0 and "done" in r.stdout, r.stdout + r.stderr
