@@ -26,7 +26,7 @@
 // 128 KB, longer on its way from L2 than in the products: a prompt of 4096, 16 / 2 heads, 182 us.
 // m is not the running maximum itself but one that follows it when it has grown by more than 2^8:
 // O is then scaled in tensor memory, which happens a few times at a piece's start and rarely after (P
-// is at most 2^8, or 2^15 in f16, its sum and O are held in f32).
+// is lifted with room for that; its sum and O are held in f32).
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <stddef.h>
@@ -482,7 +482,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(const __grid_c
             const int p_first = x.r.past + (int)a.group.div(min(x.row0 + t * 128, last)),
                       p_top = x.r.past + (int)a.group.div(min(x.row0 + t * 128 + 127, last));
             float m = -INFINITY, l = 0.0f;
-            constexpr float lift = weight_lift<T>() == 0.0f ? 0.0f : weight_lift<T>() - AT_GROWTH;   // below f16's 2^16 with the growth
+            constexpr float lift = weight_lift<T>() - AT_GROWTH;  // so high with the growth
             const uint32_t qs = pf_smem(q_sm + t * At<D>::q_tile);
             constexpr int PR = D / 8, RPI = 32 / PR;              // pieces of a row, rows of a warp's access
             if (n) {

@@ -363,11 +363,12 @@ __device__ __forceinline__ float exp2_of(float x) {
     return y;
 }
 
-// The powers of two by which the weights that go into the second product are lifted above one (up to
-// 2^15 in all): f16 keeps its 11 bits down to 2^-14 and nothing below 2^-25, and the many small weights beside one
-// large key count together.  The maximum that a piece is written with is lowered by as much, so that pieces join as they are.
-// bf16 has f32's exponents.
-template <class T> __device__ __forceinline__ constexpr float weight_lift() { return 0.0f; }
+// The powers of two by which the weights that go into the second product are lifted above one.
+// f16 keeps its 11 bits down to 2^-14 and nothing below 2^-25, and the many small weights beside one large key
+// count together: up to 2^15.  bf16 has f32's exponents, and so have its values: weights of at most 2^-24 keep
+// the sums over up to 2^24 keys in f32 whatever the values are, where the weights' sum is yet to be divided by.
+// The maximum that a piece is written with is lowered by as much, so that pieces join as they are.
+template <class T> __device__ __forceinline__ constexpr float weight_lift() { return -24.0f; }
 template <> __device__ __forceinline__ constexpr float weight_lift<__half>() { return 15.0f; }
 
 // ---- the careful row -------------------------------------------------------------------------------
@@ -463,7 +464,7 @@ __device__ __noinline__ void careful_row(const AttendCall& a, const Piece& x, in
             float mn = s;
             for (int d = 16; d; d >>= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, d));
             mn = fmaxf(m, mn);
-            const float c = mn == -INFINITY ? 1.0f : exp2_of(m - mn), e2 = mn == -INFINITY ? 0.0f : exp2_of(s - mn);
+            const float c = mn == -INFINITY ? 1.0f : exp2_of(m - mn), e2 = mn == -INFINITY ? 0.0f : exp2_of(s - mn + weight_lift<T>());
             float sum = e2;
             for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
             m = mn;
@@ -486,7 +487,7 @@ __device__ __noinline__ void careful_row(const AttendCall& a, const Piece& x, in
     }
 #pragma unroll
     for (int e = 0; e < D / 32; e++) o_out[e] = o[e];
-    m_out = m;
+    m_out = m - weight_lift<T>();
     l_out = l;
 }
 

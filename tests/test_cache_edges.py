@@ -140,6 +140,21 @@ def one_head(b, heads):
     return o, mag
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("new", [1, 140])
+def test_values_near_the_largest_there_are(dim, new):
+    # all values 2^124 or minus that, where f32 ends at 2^128; one key's weight is 2^7 times any other's and comes
+    # after many of them
+    b = Batch([new, new], [900, 60], 8, 2, dim, BF16, 16, seed=21)
+    b.q.fill_(1.0)
+    b.k.copy_(torch.where(b.k.isnan(), b.k, 0.0))
+    b.k[int(b.table[0, 200 // 16]), 200 % 16] = 7.0 * math.log(2.0) / math.sqrt(dim)
+    b.v.copy_(torch.where(b.v.isnan(), b.v, b.v.sign() * 2.0 ** 124))
+    c = cache(8, 2, dim, 16, 2, 512, BF16)
+    near(b.run(c, max_new=new), b.want(), BF16)
+
+
 def test_the_clock_of_a_wait_stands_while_another_role_is_at_work(tmp_path):
     src, exe = tmp_path / "clock.cpp", str(tmp_path / "clock")
     src.write_text(r"""
