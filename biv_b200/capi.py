@@ -68,8 +68,8 @@ class CacheDesc(C.Structure):
 
 
 def _flat(prefix, kind):
-    """The fields of a ``bivmoe_rows`` or ``bivmoe_pool`` inside an argument struct, one by one: a call's
-    arguments are packed into it from a flat list."""
+    """The fields of a ``bivmoe_rows`` or ``bivmoe_pool`` inside an argument struct, one by one.  (For callers
+    that have no torch tensors; ``cache.PagedCache`` goes through its extension module.)"""
     names = {"rows": ("stride_token", "stride_head"), "pool": ("stride_page", "stride_token", "stride_head", "n_pages")}[kind]
     fields = [(prefix, C.c_void_p)] + [(prefix + "_" + n, C.c_int64) for n in names]
     return fields + ([(prefix + "_type", C.c_int32), (prefix + "_reserved", C.c_int32)] if kind == "rows" else [])

@@ -25,10 +25,6 @@ constexpr int kFewWarps = 4, kFewThreads = 32 * kFewWarps, kFewStages = 3;
 // windowed step of 128 requests 70.2 / 69.8 / 70.5 / 72.2.
 constexpr int kFewLeast = 2, kFewExtra = 1;
 
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool there) {
-    // nothing is read, and zeros are written, where there is nothing
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
-}
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void ldm4(uint32_t a, uint32_t (&r)[4]) {

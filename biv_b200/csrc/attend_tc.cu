@@ -124,9 +124,6 @@ __device__ __forceinline__ void at_arrive(uint64_t* bar) {
     if ((threadIdx.x & 31) == 0) pf_bar_arrive(bar);
     __syncwarp();
 }
-__device__ __forceinline__ void at_cp16(uint32_t dst, const void* src, bool there) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
-}
 // the thread's arrival, once its copies so far have landed
 __device__ __forceinline__ void at_cp_arrive(uint64_t* bar) {
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(pf_smem(bar)) : "memory");
@@ -336,7 +333,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(const __grid_c
 #pragma unroll
                     for (int s = 0; s < 8; s++) {
                         const int r = 4 * (s0 + s) + (lane >> 3);
-                        at_cp16((dst + r * 128) ^ ((r & 7) << 4), from + max(o[s], (int64_t)0), o[s] >= 0);
+                        cp16((dst + r * 128) ^ ((r & 7) << 4), from + max(o[s], (int64_t)0), o[s] >= 0);
                     }
                 }
                 at_cp_arrive(&H.full[slot]);
@@ -490,7 +487,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attend_tc_kernel(const __grid_c
 #pragma unroll 8
                 for (int i = 0; i < 32 / RPI; i++) {
                     const int r = (warp & 3) * 32 + i * RPI + lane / PR, Q = min(x.row0 + t * 128 + r, last), qt = (int)a.group.div(Q);
-                    at_cp16(at_piece(qs, r, lane % PR),
+                    cp16(at_piece(qs, r, lane % PR),
                             a.q + (int64_t)(x.r.begin + qt) * a.q_token + (int64_t)(x.head * (int)a.group.d + Q - qt * (int)a.group.d) * a.q_head +
                                 (lane % PR) * 16, x.row0 + t * 128 + r <= last);
                 }

@@ -362,6 +362,11 @@ __device__ __forceinline__ float exp2_of(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// 16 bytes into shared memory, under way until the thread waits for it: nothing is read, and zeros are
+// written, where there is nothing
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
 
 // The powers of two by which the weights that go into the second product are lifted above one.
 // f16 keeps its 11 bits down to 2^-14 and nothing below 2^-25, and the many small weights beside one large key

@@ -68,8 +68,9 @@ extern "C" int bivmoe_cache_create(const bivmoe_cache_desc* d, bivmoe_cache** ou
     if (d->max_tokens < 1 || d->max_tokens > kCacheTokens)
         return fail(BIVMOE_ERR_ARGUMENT, "max_tokens %d outside 1..%d", d->max_tokens, kCacheTokens);
     if (d->n_rot < 0 || d->n_rot > d->head_dim) return fail(BIVMOE_ERR_ARGUMENT, "n_rot %d outside 0..head_dim %d", d->n_rot, d->head_dim);
-    std::vector<double> turns;
-    std::vector<int32_t> axis;
+    double turns[kRopePairs];
+    int32_t axis[kRopePairs];
+    int pairs = 0;
     if (d->n_rot) {
         if (d->n_rot % 16) return fail(BIVMOE_ERR_UNSUPPORTED, "n_rot %d is not a multiple of 16", d->n_rot);
         if (d->rope_axes < 1 || d->rope_axes > 4) return fail(BIVMOE_ERR_ARGUMENT, "rope_axes %d outside 1..4", d->rope_axes);
@@ -92,8 +93,8 @@ extern "C" int bivmoe_cache_create(const bivmoe_cache_desc* d, bivmoe_cache** ou
                 of = a;
             }
             found[of]++;
-            axis.push_back(of);
-            turns.push_back(pow(d->rope_base, -2.0 * i / d->n_rot) / (2.0 * M_PI));
+            axis[pairs] = of;
+            turns[pairs++] = pow(d->rope_base, -2.0 * i / d->n_rot) / (2.0 * M_PI);
         }
         for (int a = 0; a < d->rope_axes; a++)
             if (found[a] != d->rope_sections[a])
@@ -121,13 +122,13 @@ extern "C" int bivmoe_cache_create(const bivmoe_cache_desc* d, bivmoe_cache** ou
                  rows = few > tc ? few : tc, counts = 8 * (size_t)c->sm_count;
     size_t off = 0;
     auto take = [&off](size_t bytes) { const size_t at = off; off += (bytes + 255) & ~(size_t)255; return at; };
-    const size_t o = take(rows * d->head_dim * 4), ml = take(rows * sizeof(float2)), tt = take(turns.size() * 8 + 8),
-                 ax = take(axis.size() * 4 + 4), arr = take(counts * 4), st = take(16), un = take(8);
+    const size_t o = take(rows * d->head_dim * 4), ml = take(rows * sizeof(float2)), tt = take(pairs * 8 + 8),
+                 ax = take(pairs * 4 + 4), arr = take(counts * 4), st = take(16), un = take(8);
     c->arrived_bytes = counts * 4;
     e = dev_alloc((void**)&c->mem, off);
     if (e == cudaSuccess) e = cudaMemset(c->mem + arr, 0, off - arr);
-    if (e == cudaSuccess && d->n_rot) e = cudaMemcpy(c->mem + tt, turns.data(), turns.size() * 8, cudaMemcpyHostToDevice);
-    if (e == cudaSuccess && d->n_rot) e = cudaMemcpy(c->mem + ax, axis.data(), axis.size() * 4, cudaMemcpyHostToDevice);
+    if (e == cudaSuccess && d->n_rot) e = cudaMemcpy(c->mem + tt, turns, pairs * 8, cudaMemcpyHostToDevice);
+    if (e == cudaSuccess && d->n_rot) e = cudaMemcpy(c->mem + ax, axis, pairs * 4, cudaMemcpyHostToDevice);
     if (e == cudaSuccess) e = cudaEventCreateWithFlags(&c->done, cudaEventDisableTiming);
     if (e == cudaSuccess) e = cudaDeviceSynchronize();   // the clears, before a call on any stream
     if (e != cudaSuccess) {

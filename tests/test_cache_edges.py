@@ -1,4 +1,6 @@
-"""The paged cache at its edges: values that are not finite."""
+"""The paged cache at its edges: values that are not finite or near that, lists that run out, views, streams and
+waits that meet, the shares of the work, the build."""
+import ctypes as C
 import math
 import os
 import subprocess
@@ -6,7 +8,8 @@ import subprocess
 import pytest
 import torch
 
-from test_cache import BF16, DEV, F16, ROOT, UNIT, Batch, cache, ints, near, turned64
+from biv_b200 import capi
+from test_cache import BF16, DEV, F16, F32, ROOT, UNIT, Batch, cache, ints, near, turned64
 
 
 # ---- values that are not finite ----------------------------------------------------------------------
@@ -259,6 +262,44 @@ int main() {
         code = f.read()
     role = code[code.index("// ---- copies"):code.index("// ---- products")]
     assert "wait_for_last_fills<AT_SLOTS, AT_COPY_WARPS>(last, fills" in role[role.index("cp.async.wait_all"):]
+
+
+@pytest.mark.gpu
+def test_the_c_abi_s_argument_structs():
+    # the calls by the structs that a ctypes caller fills, against the ones that take tensors
+    from biv_b200.cache import Rope
+    L, b = capi.lib(), Batch([3, 2], [0, 0], 4, 2, 64, BF16, 16, junk=0.0)
+    c = cache(4, 2, 64, 16, 2, 8, BF16, rope=Rope(64))
+    s = c.extend(ints([0, 0]), ints([3, 2]), ints([5, 6]), ints([2]), b.table, 5)
+    x = torch.randn((5, 8, 64), device=DEV)
+    k, v = [torch.zeros((8, 16, 2, 64), dtype=BF16, device=DEV) for _ in range(2)]
+    q = c.store(x[:, :4], x[:, 4:6], x[:, 6:], k, v, s.slots, s.positions)
+    want = c.attend(q, k, v, b.table, s.first, s.length)
+
+    def rows(t):
+        return (t.data_ptr(), t.stride(0), t.stride(1), {F32: 0, BF16: 30}[t.dtype], 0)
+
+    def pool(t):
+        return (t.data_ptr(), t.stride(0), t.stride(1), t.stride(2), t.shape[0])
+
+    table, k2, v2, q2, o2 = b.table.clone().fill_(-1), torch.zeros_like(k), torch.zeros_like(v), torch.zeros_like(q), torch.zeros_like(q)
+    lists = [torch.zeros(n, dtype=torch.int32, device=DEV) for n in (2, 3, 5, 2, 2)]
+    length, first, positions, left, held = lists
+    slots = torch.zeros(5, dtype=torch.int64, device=DEV)
+    ins = [ints([0, 0]), ints([3, 2]), ints([5, 6]), ints([2])]
+    e = capi.ExtendArgs(ins[0].data_ptr(), ins[1].data_ptr(), None, ins[2].data_ptr(), ins[3].data_ptr(), table.data_ptr(), table.stride(0),
+                        table.shape[1], 2, 2, 5, *[t.data_ptr() for t in lists], slots.data_ptr())
+    stream = torch.cuda.current_stream().cuda_stream
+    capi.check(L.bivmoe_cache_extend(c._h, C.byref(e), stream))
+    assert [t.tolist() for t in (length, first, slots, positions, left, held)] == [t.tolist() for t in s]
+    a = capi.StoreArgs(*rows(x[:, :4]), *rows(x[:, 4:6]), *rows(x[:, 6:]), *rows(q2), *pool(k2), *pool(v2), slots.data_ptr(),
+                       positions.data_ptr(), 5, 5, 0)
+    capi.check(L.bivmoe_cache_store(c._h, C.byref(a), stream))
+    assert torch.equal(q2, q) and torch.equal(k2, k) and torch.equal(v2, v)
+    t = capi.AttendArgs(*rows(q2), *rows(o2), *pool(k2), *pool(v2), table.data_ptr(), table.stride(0), table.shape[1], 2, 5, 0,
+                        first.data_ptr(), length.data_ptr(), 64 ** -0.5, 0, 0, 0)
+    capi.check(L.bivmoe_cache_attend(c._h, C.byref(t), stream))
+    assert torch.equal(o2, want)
 
 
 # ---- streams -----------------------------------------------------------------------------------------
