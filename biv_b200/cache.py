@@ -127,7 +127,8 @@ class PagedCache:
         """Attention of the rows q [n, n_head, head_dim], request b's from first[b] to first[b + 1] - 1,
         the last tokens of its length[b] tokens.  A token at position p sees p and what is before it;
         with ``window`` the last ``window`` positions up to its own and the first ``sinks``.  ``max_new``:
-        the most new rows of a request, where the caller knows it."""
+        the most new rows of a request; pass it where it is known: it decides the kernel, and a decode step without it
+        may take twice as long."""
         r = _cache_calls.attend(self._geometry, q, k_pool, v_pool, table, first, length, max_new, scale, window, sinks, out)
         if r.__class__ is int:
             capi.check(r)

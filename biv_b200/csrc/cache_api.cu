@@ -313,7 +313,10 @@ extern "C" int bivmoe_cache_attend(bivmoe_cache* c, const bivmoe_attend_args* a,
     cudaError_t e = take_turn(c, s);
     // Which kernel, by the most rows a request has to a kv head (max_new is the caller's word and decides the
     // speed alone: both kernels take any number).  Up to 16 rows a tile of the first reads the keys once; up to
-    // 32 it reads them twice, mostly from L2, and still ends sooner unless heads of 256 have many requests.
+    // 32 it reads them twice, from L2 as long as that holds them, and ends sooner with few requests or short ones.  Lengths
+    // are not known here, so that two choices below are not the faster one: heads of 128, 32 rows, where many long
+    // requests pass L2 by (90.2 against 82.2), and 48 rows where there are few or short ones.  Without max_new the
+    // whole batch counts as one request: a decode step of 64 requests, 32 / 8 heads of 128, 249 us instead of 186.
     // us, tiles of 16 rows / tcgen05 (heads_kv 4, 4 and 2; requests x tokens):
     //   rows  heads of    1 x 300      8 x 1000     32 x 4000     4 x 20000
     //    32      64      9.9 / 13.1  13.5 / 21.1   58.4 / 67.1   41.5 / 56.8
