@@ -269,6 +269,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunks_kernel(const __grid
                 }
                 dec.bad[quarter * 32 + lane] = (uint8_t)bad;
                 fence_async();
+                __syncwarp();                                 // what a lane has taken out, before another loads it
                 if (!__any_sync(0xffffffffu, bad != 255)) break;
             }
             wait_st();
