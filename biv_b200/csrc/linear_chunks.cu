@@ -49,7 +49,7 @@ struct alignas(16) Decays {                          // of a chunk
     uint8_t bad[D];                                  // the first token whose value of v is not finite, or 255
 };
 struct Head {
-    uint64_t full[kStages], empty[kStages], known[kRing], qk_full, qk_free, p_full[2], w_full[2], w_free[2], u_full, u_free, s_full, r_done,
+    uint64_t full[kStages], empty[kStages], known[kRing], qk_full, qk_free, p_full[2], w_full[kRing], w_free[2], u_full, u_free, s_full, r_done,
         n_full, o_free, out_done, given, read, drained;
     uint32_t tmem;
     int abort;
@@ -91,8 +91,8 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunks_kernel(const __grid
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 416) {
         for (int i = 0; i < kStages; i++) { pf_bar_init(&H.full[i], 1); pf_bar_init(&H.empty[i], 1); }
-        for (int i = 0; i < kRing; i++) pf_bar_init(&H.known[i], 1);
-        for (int i = 0; i < 2; i++) { pf_bar_init(&H.w_full[i], 4); pf_bar_init(&H.w_free[i], 1); }
+        for (int i = 0; i < kRing; i++) { pf_bar_init(&H.known[i], 1); pf_bar_init(&H.w_full[i], 4); }
+        for (int i = 0; i < 2; i++) pf_bar_init(&H.w_free[i], 1);
         for (uint64_t* one : {&H.qk_full, &H.u_full, &H.r_done, &H.n_full, &H.drained}) pf_bar_init(one, 1);
         for (uint64_t* four : {&H.u_free, &H.s_full, &H.o_free, &H.out_done, &H.read}) pf_bar_init(four, 4);
         for (uint64_t* two : {&H.qk_free, &H.p_full[0], &H.p_full[1]}) pf_bar_init(two, 2);
@@ -125,6 +125,14 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunks_kernel(const __grid
             atomicExch(c.status, site);
             *(volatile int*)&H.abort = 1;
         }
+    };
+    // A chunk's decays, and where its values are not finite, come from other warps than the product whose end a role has waited for.  Both
+    // have long been told by then: a wait for either that returns at once, and puts what they wrote before what is read of it.  (A place of
+    // the ring is told again eight chunks on, which no role's own chunk is left behind by: so a look after the product's end sees this
+    // chunk's phase, or none.)
+    auto told = [&](int k) {
+        const uint32_t parity = (k / kRing) & 1;
+        return wait_here(&H.known[k % kRing], parity, &H) && wait_here(&H.w_full[k % kRing], parity, &H);
     };
     // this block's chunks; those that it goes through twice
     const int chunks = (seq.n + C - 1) / C, c0 = (int)((int64_t)chunks * rank / blocks), own = (int)((int64_t)chunks * (rank + 1) / blocks) - c0;
@@ -186,7 +194,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunks_kernel(const __grid
                 arrive_warp(&H.s_full);
             }
             // the chunk's sum joins it
-            if (!wait_here(&H.u_full, k & 1, &H)) { ok = false; break; }
+            if (!wait_here(&H.u_full, k & 1, &H) || !told(k)) { ok = false; break; }
             pf_fence_after();
             const Decays& dec = H.ring[k % kRing];
             const float by = dec.bad[tid] == 255 ? dec.whole : __int_as_float(0x7fffffff);   // (NaN: so becomes the row)
@@ -275,7 +283,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunks_kernel(const __grid
             wait_st();
             pf_fence_before();
             __syncwarp();
-            arrive_warp(&H.w_full[k & 1]);
+            arrive_warp(&H.w_full[k % kRing]);
         }
     } else if (warp < 12) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
@@ -285,7 +293,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunks_kernel(const __grid
         uint8_t* out = c.out.data + (int64_t)(seq.first + c0 * C) * c.out.token + h * c.out.head + (warp & 3) * 64;
         for (int j = 0; j < own; j++, out += C * c.out.token) {
             const int k = twice + j, n = min(C, seq.n - (c0 + j) * C);
-            if (!wait_warp(&H.n_full, j & 1, &H)) { give_up(SITE_OUT); break; }
+            if (!wait_warp(&H.n_full, j & 1, &H) || !told(k)) { give_up(SITE_OUT); break; }
             pf_fence_after();
             const Decays& dec = H.ring[k % kRing];
             write_out(tmem + kAtR + lanes, tmem + kAtN + lanes, dec.upto, c.scale, [&](int r) { return (int)dec.bad[(warp & 3) * 32 + r]; },
@@ -316,7 +324,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunks_kernel(const __grid
                 auto stage = [&](int k) { return stages + (k % kStages) * kStage; };
                 auto u_of = [&](int k) {
                     wait(&H.full[k % kStages], (k / kStages) & 1);
-                    wait(&H.w_full[k & 1], (k >> 1) & 1);
+                    wait(&H.w_full[k % kRing], (k / kRing) & 1);
                     if (k) wait(&H.u_free, (k - 1) & 1);
                     if (!ok) return;
                     pf_fence_after();

@@ -21,3 +21,48 @@ def test_values_that_a_lane_takes_out_are_seen_by_the_lanes_that_load_them():
     w = between(code("linear_chunks.cu"), "for (int again = 0;", "arrive_warp(&H.w_full")
     assert "ldmatrix" in w
     assert "__syncwarp()" in w[w.index("st.shared.u16"):w.index("wait_st()")]
+
+
+def test_roles_wait_for_those_whose_words_they_read():
+    """A chunk's decays come from the copying warp (`known`), where its values are not finite from the weights' warps (`w_full`): a product's
+    end, told by the issuing thread, puts neither before a read of them."""
+    text = code("linear_chunks.cu")
+    told = between(text, "auto told", "};")
+    assert "wait_here(&H.known[k % kRing], parity" in told and "wait_here(&H.w_full[k % kRing], parity" in told
+    for start, end, product in (("for (int k = 0;; k++)", "arrive_warp(&H.u_free)", "u_full"),
+                                ("for (int j = 0; j < own; j++, out +=", "write_out(", "n_full")):
+        role = between(text, start, end)
+        wait = re.search(r"if \(!wait_\w+\(&H\.%s, \w & 1, &H\) \|\| !told\(k\)\)" % product, role)
+        assert wait and wait.end() < role.index("dec = H.ring")
+
+
+def test_no_place_of_the_ring_is_told_twice_while_a_role_looks():
+    """The parity of a phase says which of two it is: a role that looks at chunk k's must not be eight chunks behind.  The roles of a
+    block as the waits between them order them, in many orders: whoever looks finds chunk k's phase the last one that ended."""
+    import random
+    ring, stages = 8, 3
+    for seed in range(60):
+        rng = random.Random(seed)
+        twice, own = rng.randint(0, 40), rng.randint(1, 40)
+        n = twice + own
+        done = {name: 0 for name in ("copy", "w", "u", "state", "n", "out")}     # chunks (n, out: of the second pass) that a role has ended
+        speed = {name: rng.random() ** 3 + 1e-3 for name in done}
+        may = dict(
+            copy=lambda k: k < stages or (done["u"] > k - stages and (k - stages < twice or done["n"] > k - stages - twice)),
+            w=lambda k: done["copy"] > k and (k < 2 or done["u"] > k - 2),
+            # products in the issuing thread's order: U of a chunk behind N of the one before
+            u=lambda k: done["w"] > k and done["state"] >= k and (k <= twice or done["n"] >= k - twice),
+            state=lambda k: done["u"] > k,
+            n=lambda j: done["u"] > twice + j and done["state"] >= twice + j and (j == 0 or done["out"] >= j),
+            out=lambda j: done["n"] > j)
+        total = {name: own if name in ("n", "out") else n for name in done}
+        while any(done[r] < total[r] for r in done):
+            ready = [r for r in done if done[r] < total[r] and may[r](done[r])]
+            assert ready, (twice, own, done)
+            r = rng.choices(ready, [speed[x] for x in ready])[0]
+            if r in ("state", "out"):
+                k = done[r] + (twice if r == "out" else 0)
+                for teller in ("copy", "w"):
+                    told = [c for c in range(done[teller]) if c % ring == k % ring]
+                    assert told and told[-1] == k, (r, k, done)
+            done[r] += 1
