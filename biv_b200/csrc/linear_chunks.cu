@@ -308,7 +308,9 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunks_kernel(const __grid
             const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
             for (int j = 0; j < own; j++) {
                 const int k = twice + j;
-                if (!wait_warp(&H.known[k % kRing], (k / kRing) & 1, &H) || !wait_warp(&H.qk_full, j & 1, &H)) { give_up(SITE_P); break; }
+                // (The product first: these warps have not seen the places of the ring that the first pass went round, and of those the parity
+                // alone says nothing.  Behind the product, which waits for the decays, too, the place's last phase is this chunk's.)
+                if (!wait_warp(&H.qk_full, j & 1, &H) || !wait_warp(&H.known[k % kRing], (k / kRing) & 1, &H)) { give_up(SITE_P); break; }
                 pf_fence_after();
                 // (two P: this one's place was read by the product two chunks ago, which ended before this Q K^T did)
                 weights_row(tmem + kAtQK + lanes, H.ring[k % kRing].log2, r, weights_of(j) + r * 128, &H.qk_free);

@@ -66,3 +66,12 @@ def test_no_place_of_the_ring_is_told_twice_while_a_role_looks():
                     told = [c for c in range(done[teller]) if c % ring == k % ring]
                     assert told and told[-1] == k, (r, k, done)
             done[r] += 1
+
+
+def test_warps_that_sit_out_the_first_pass_look_at_its_ring_behind_a_product():
+    """A wait for odd parity returns at once while a barrier is in its first phase: with eight to fifteen chunks gone through twice a wait
+    for `known` by warps that have not followed the ring would prove nothing if it came first."""
+    text = code("linear_chunks.cu")
+    for product, role in (("qk_full", between(text, "const int r = tid - 384", "weights_row(")), ("n_full", between(text, "j < own; j++, out +=", "write_out("))):
+        waits = [m.group(1) for m in re.finditer(r"wait_\w+\(&H\.(\w+)|!told\(k\)", role)]
+        assert waits[0] == product and len(waits) == 2, waits
