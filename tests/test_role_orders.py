@@ -75,3 +75,11 @@ def test_warps_that_sit_out_the_first_pass_look_at_its_ring_behind_a_product():
     for product, role in (("qk_full", between(text, "const int r = tid - 384", "weights_row(")), ("n_full", between(text, "j < own; j++, out +=", "write_out("))):
         waits = [m.group(1) for m in re.finditer(r"wait_\w+\(&H\.(\w+)|!told\(k\)", role)]
         assert waits[0] == product and len(waits) == 2, waits
+
+
+def test_the_chain_waits_for_the_warp_that_has_the_other_half_of_its_rows():
+    """With the delta rule two warps take places of a row out of rhs and u, by halves of the chunk's tokens; each then reads whether the row
+    has any.  (The next w_full wants these warps' own arrivals, so that the phase seen is this chunk's.)"""
+    chain = between(code("linear_delta.cu"), "for (int k = 0; k < chunks && ok; k++)", "store_state(")
+    wait = re.search(r"wait_here\(&H\.u_full, k & 1, &H\) \|\| !wait_here\(&H\.w_full, k & 1, &H\)", chain)
+    assert wait and chain.index("arrive_warp(&H.w_full)") < wait.start() < chain.index("dec.bad[row]")
