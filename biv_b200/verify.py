@@ -31,7 +31,8 @@ def verify(p, tokens, uniform, sample, first, q=None, length=None) -> Verified:
     vocabulary]: the one that the draft after row r was drawn from; without it the drafts are certain (looked up, or a greedy
     choice).  Draft d after row r is accepted while ``uniform[r] * q[r, d] < p[r, d]``; then a token is drawn by ``sample[b]`` from
     max(p - q, 0) of the first row whose draft failed, or from p of the request's last row.  ``length`` [n_seq]: the requests' tokens
-    with all of the rows (``Step.length``); ``kept`` is then the next step's ``past``.  Random numbers are float32 in [0, 1)."""
+    with all of the rows (``Step.length``); ``kept`` is then the next step's ``past``.  Random numbers are float32 in [0, 1).  A draft
+    whose q or p is NaN is not accepted, a weight that is NaN counts as zero, and of infinite weights the last positive one is drawn."""
     global _call
     if _call is None:
         _call = C.cast(capi.lib().bivmoe_verify, C.c_void_p).value

@@ -580,7 +580,10 @@ BIVMOE_API int bivmoe_norm(const bivmoe_norm_args* args, void* stream);
  * positive weight).  Written: accepted[b], token[b] (-1 where no weight of p is positive, or the request has no rows), and, where
  * length is given (each request's tokens with all rows, as bivmoe_cache_extend leaves it), kept[b] = length[b] less its
  * drafts that were not accepted: the next call's past.
- * A draft outside 0..vocab - 1 is not accepted and has no weight to lose.  NaN counts as zero. */
+ * A draft outside 0..vocab - 1 is not accepted and has no weight to lose.
+ * What is not finite: a draft whose q or p is NaN is not accepted (no comparison with NaN holds), and a weight that is NaN counts as
+ * zero, whichever of p and q brought it (a NaN, or infinity less infinity).  Infinite weights make their sum infinite, which no
+ * running sum passes: the token is then the last of positive weight, whatever the sample. */
 typedef struct bivmoe_verify_args {
     const void *p, *q;                     /* device, [n_tokens][vocab]; q may be null */
     int64_t p_stride, q_stride;            /* from row to row, in values */

@@ -250,3 +250,82 @@ def test_arguments_are_checked_without_a_device():
 
 def test_the_calls_module_is_built():
     assert importlib.util.find_spec("biv_b200._step_calls") is not None
+
+
+def decided(p, q, tokens, uniform, sample, vocab):
+    """One request's (accepted, token), value by value as the header has it: comparisons that NaN never passes, weights of NaN zero."""
+    k, n = 0, len(tokens)
+    while k < n - 1:
+        d = tokens[k + 1]
+        if not (0 <= d < vocab and (uniform[k] * q[k][d] if q else uniform[k]) < p[k][d]):
+            break
+        k += 1
+    for residual in ([True, False] if k < n - 1 else [False]):
+        w = []
+        for t in range(vocab):
+            x = p[k][t]
+            if residual:
+                x = x - q[k][t] if q else (0.0 if t == tokens[k + 1] else x)
+            w.append(x if x > 0 else 0.0)                    # (NaN is not)
+        if sum(w) > 0:
+            break
+    else:
+        return k, -1
+    upto, border = 0.0, sample * sum(w)
+    for t, x in enumerate(w):
+        upto += x
+        if upto > border:
+            return k, t
+    return k, max(t for t, x in enumerate(w) if x > 0)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vocab", [40, 1503, 9001])
+@pytest.mark.parametrize("drafted", [True, False])
+def test_what_is_not_finite_as_the_header_has_it(vocab, dtype, drafted):
+    """Weights of whole numbers, whose sums are exact, with NaN and infinities at the drafts and among the weights; both ways that p and q
+    may lie to one another."""
+    g = torch.Generator().manual_seed(vocab)
+    bad = [math.nan, math.inf, -math.inf]
+    n, rows, drafts = 48, 3, 5
+    p, q = (torch.randint(0, 4, (n * rows, vocab), generator=g).double() for _ in range(2))
+    tokens = torch.randint(0, drafts, (n * rows,), generator=g) * (vocab // drafts)
+    for r in range(n * rows):
+        d = int(tokens[min(r + 1, n * rows - 1)])
+        if r % 4 == 0:
+            p[r, d] = bad[r // 4 % 3]
+        if r % 4 == 1:
+            q[r, d] = bad[r // 4 % 3]
+        if r % 3 == 0:                                       # NaN in many places, of p, of q, of both
+            p[r, r % 7::7] = math.nan
+            q[r, r % 5::5] = math.nan
+        if r % 5 == 0:                                       # some infinite weights, infinity less infinity
+            p[r, vocab // 3:vocab // 2:3] = math.inf
+            q[r, vocab // 3:vocab // 2:6] = math.inf
+    uniform = torch.randint(0, 3, (n * rows,), generator=g).float() / 2
+    sample = torch.randint(0, 16, (n,), generator=g).float() / 16
+    want = []
+    for b in range(n):
+        at = slice(b * rows, (b + 1) * rows)
+        want.append(decided(p[at].tolist(), q[at].tolist() if drafted else None, tokens[at].tolist(), uniform[at].tolist(), float(sample[b]), vocab))
+    assert len({k for k, _ in want}) == 3                    # (drafts pass and fail)
+    ints = dict(dtype=torch.int32, device="cuda")
+    for apart in (8, 9):                                     # q and p alike within 16 bytes, and not
+        both = torch.zeros((n * rows, 2, 8 + vocab + apart), dtype=dtype, device="cuda")
+        rows_p, rows_q = both[:, 0, 8:8 + vocab], both[:, 1, apart:apart + vocab]
+        rows_p.copy_(p)
+        rows_q.copy_(q)
+        x = dict(p=rows_p, q=rows_q if drafted else None, tokens=tokens.to(**ints), uniform=uniform.cuda(), sample=sample.cuda(),
+                 first=torch.arange(0, n * rows + 1, rows, **ints), length=None)
+        got = run(x)
+        assert list(zip(got.accepted.tolist(), got.token.tolist())) == want
+
+
+def test_the_definition_of_these_tests():
+    inf, nan = math.inf, math.nan
+    p, q = [[1.0, 2.0, 1.0], [nan, 3.0, 1.0]], [[1.0, 4.0, 0.0], [1.0, nan, 1.0]]
+    assert decided(p, q, [0, 1], [0.25, 0.0], 0.0, 3) == (1, 1)               # accepted; then p's own, without its NaN
+    assert decided(p, q, [0, 1], [0.5, 0.0], 0.9, 3) == (0, 2)                # 2 < 2 is not: what p has over q
+    assert decided([[1.0, 2.0], [0.0, 0.0]], [[1.0, nan], [0.0, 0.0]], [0, 1], [0.0, 0.0], 0.5, 2) == (0, 1)   # 0 * NaN: not accepted; p itself
+    assert decided([[inf, 1.0, inf, 1.0]], None, [0], [0.0], 0.0, 4) == (0, 3)
