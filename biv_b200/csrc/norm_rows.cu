@@ -121,7 +121,9 @@ __device__ __forceinline__ float root_of(double sum, const NormCall& c) {
 }
 // The eight codes of y in Q8: halves away from zero, for |q| < 2^23: what is below one half stays below it when the largest number below one
 // half is added, and a half reaches the next whole number by rounding; what is behind the point falls off as 2^23 is added.  (A
-// conversion to an integer is one for 16 lanes a clock.)
+// conversion to an integer is one for 16 lanes a clock.)  A scale of few bits, among f32's smallest numbers, may be rounded by up to half of
+// itself, so that quotients pass 127 (2^-149 for a largest value of 190 of it): they stay at 127, which elsewhere none passes, the scale being off
+// by 2^-24 of itself at most.
 __device__ __forceinline__ uint2 q8_codes(const float (&y)[8], float scale) {
     const float inv = scale != 0.0f ? __fdiv_rn(1.0f, scale) : 0.0f;
     float q[8];
@@ -132,6 +134,7 @@ __device__ __forceinline__ uint2 q8_codes(const float (&y)[8], float scale) {
 #pragma unroll
             for (int i = 1; i < 8; i++) x = i == j ? y[i] : x;
             x = __fdiv_rn(x, scale);
+            x = x > 127.0f ? 127.0f : x < -127.0f ? -127.0f : x;
 #pragma unroll
             for (int i = 0; i < 8; i++) q[i] = i == j ? x : q[i];
         }

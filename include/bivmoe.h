@@ -556,7 +556,8 @@ BIVMOE_API int bivmoe_linear_status(bivmoe_linear* layer, void* stream);
  *                       to the last bit but one
  *     BIVMOE_NORM_E4M3  8-bit floats, block 128 or 0 (the row), scale = max|y| * (1 / 448), code = y / scale rounded to the
  *                       nearest
- * each step in f32. A block of zeros has scale 0 and codes 0. */
+ * each step in f32.  A block whose scale is 0 (zeros, or values whose scale f32 does not hold) has codes 0.  Where f32 does not hold 1 / scale (below
+ * 2^-128) NORM_Q8 divides by the scale instead; such a scale has few bits, and quotients that pass 127, or E4M3's 448, are kept at it. */
 enum { BIVMOE_NORM_Q8 = 1000, BIVMOE_NORM_E4M3 = 1001 };
 typedef struct bivmoe_norm_args {
     bivmoe_rows x, add, gate, out;   /* add.data and gate.data may be null; out's type: F32, F16, BF16 or one of the above */
