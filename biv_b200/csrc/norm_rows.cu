@@ -74,11 +74,6 @@ template <int TY> __device__ __forceinline__ void load8_of(const uint8_t* p, flo
     x.load(p);
     x.values(v);
 }
-__device__ __forceinline__ void load8(const uint8_t* p, int ty, float (&v)[8]) {
-    if (ty == BIVMOE_F32) load8_of<BIVMOE_F32>(p, v);
-    else if (ty == BIVMOE_BF16) load8_of<BIVMOE_BF16>(p, v);
-    else load8_of<BIVMOE_F16>(p, v);
-}
 __device__ __forceinline__ void store8(uint8_t* p, int ty, const float (&v)[8]) {
     if (ty == BIVMOE_F32) {
         *(float4*)p = make_float4(v[0], v[1], v[2], v[3]);
@@ -413,10 +408,7 @@ cudaError_t launch_norm(const NormCall& c, bool vector, int sm_count, cudaStream
     while (tpr < pieces || tpr < least) tpr *= 2;
     // Many rows: four pieces to a thread, for more bytes under way, and because the root, in f64, costs a warp as much as some
     // tens of pieces.
-    if (tpr > 1024 || (c.rows * tpr >= sm_count * 4096 && tpr >= 4 * least && tpr > 4)) {
-        if (tpr >= 4 * least && tpr > 4) return launch<4>(c, tpr / 4, stream);
-        return launch<2>(c, tpr / 2, stream);
-    }
+    if (tpr > 1024 || (c.rows * tpr >= sm_count * 4096 && tpr >= 4 * least && tpr > 4)) return launch<4>(c, tpr / 4, stream);
     return launch<1>(c, tpr, stream);
 }
 
