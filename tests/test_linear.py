@@ -513,3 +513,67 @@ def test_what_lies_over_one_another_is_not_written():
     states = x["states"].clone()
     out = lay.attend(same["q"], same["k"], same["v"], same["decay"], states, same["slots"], same["first"])
     check(same, out, states, torch.bfloat16)
+
+
+# Slots that are not there, one that is taken, past zero and not, without `keep`: by the kernels for prompts.  Lengths of one chunk, of
+# some, and of as many as make clusters of two, four and eight blocks (148 multiprocessors; with them requests of one chunk, whose
+# clusters have blocks without any).  A [700], above, is eleven chunks and has one block: clusters begin with sixteen.
+SLOTS = [
+    # lengths, heads, heads of q and k
+    ([30, 70, 200, 0, 17, 1, 64, 300], 4, 2),
+    ([1100], 40, 20),                              # two: 80 blocks; by four they would not run at once
+    ([1100, 5, 1300], 14, 7),                      # two
+    ([2100, 40, 1, 1500], 3, 1),                   # four, or as many as there is room for
+    ([4300, 3, 64, 0, 4200, 130], 1, 1),           # eight
+]
+
+
+@gpu
+@pytest.mark.parametrize("which", [0, 1, 2])
+@pytest.mark.parametrize("delta", [False, True])
+@pytest.mark.parametrize("shape", SLOTS)
+def test_prompts_whose_slots_are_not_there(shape, delta, which):
+    """`which` turns the parts about: every length once has a state, none, and a slot that an earlier request has."""
+    lengths, h, hk = shape
+    x = make(lengths, h, hk, 128, 128, torch.bfloat16, delta, seed=sum(lengths) + which)
+    slots = x["slots"].tolist()
+    n = len(lengths)
+    for b in range(n):
+        part = (b + which) % 3
+        if part == 1:
+            slots[b] = (-1, 10 ** 6, x["states"].shape[0])[b % 3]
+        elif part == 2 and b:
+            slots[b] = slots[b - 1] if slots[b - 1] >= 0 else slots[0]
+    past = [(0, 9, 4)[(b + b // 3 + which) % 3] for b in range(n)]
+    x["slots"] = torch.tensor(slots, dtype=torch.int32, device="cuda")
+    lay = layer(x, torch.bfloat16)
+    states = x["states"].clone()
+    out = lay.attend(x["q"], x["k"], x["v"], x["decay"], states, x["slots"], x["first"], beta=x["beta"],
+                     past=torch.tensor(past, dtype=torch.int32, device="cuda"), max_new=max(lengths))
+    lay.status()
+    check(x, out, states, torch.bfloat16, past=past, prompt=True)
+    kept = {s for b, s in enumerate(slots) if 0 <= s < states.shape[0] and s not in slots[:b] and lengths[b]}
+    left = [s for s in range(states.shape[0]) if s not in kept]
+    assert torch.equal(states[left], x["states"][left])
+
+
+@gpu
+@pytest.mark.parametrize("delta", [False, True])
+@pytest.mark.parametrize("where", [0, 63, 64, 700, 1099])
+def test_what_is_not_finite_in_clusters_and_at_the_ends_of_chunks(where, delta):
+    """A value of v that is not finite, in the first pass of a cluster's stretch or the second, at the ends of chunks."""
+    x = make([1100], 40, 20, 128, 128, torch.bfloat16, delta, seed=3)
+    lay = layer(x, torch.bfloat16)
+    call = lambda v, s: lay.attend(x["q"], x["k"], v, x["decay"], s, x["slots"], x["first"], beta=x["beta"], max_new=1100)  # noqa: E731
+    s0, s1 = x["states"].clone(), x["states"].clone()
+    clean = call(x["v"], s0)
+    v = x["v"].clone()
+    v[where, 7, 100], v[where, 7, 31] = math.inf, math.nan
+    got = call(v, s1)
+    lay.status()
+    slot = int(x["slots"][0])
+    rest = [i for i in range(128) if i not in (31, 100)]
+    assert not got[where:, 7, [31, 100]].isfinite().any() and not s1[slot, 7, [31, 100]].isfinite().any()
+    assert torch.equal(got[:where], clean[:where]) and torch.equal(got[:, 7, rest], clean[:, 7, rest]) and torch.equal(s1[slot, 7, rest], s0[slot, 7, rest])
+    others = [i for i in range(40) if i != 7]
+    assert torch.equal(got[:, others], clean[:, others]) and torch.equal(s1[slot, others], s0[slot, others])
