@@ -117,6 +117,11 @@ extern "C" int bivmoe_linear_attend(bivmoe_linear* l, const bivmoe_linear_args* 
             return fail(BIVMOE_ERR_ARGUMENT, "%s: not aligned to 16 bytes, or a stride is not a multiple of them", x.name);
     }
     if (a->q.data && over_one_another(a->out, a->n_tokens, d.n_head)) return fail(BIVMOE_ERR_ARGUMENT, "out: rows lie over one another");
+    // q and k are read by the blocks of all heads that share them, v by those alone that write its place of out, and before they do
+    if (a->q.data && (a->out.data == a->q.data || a->out.data == a->k.data ||
+                      (a->out.data == a->v.data && ((a->n_tokens > 1 && a->out.stride_token != a->v.stride_token) ||
+                                                    (d.n_head > 1 && a->out.stride_head != a->v.stride_head)))))
+        return fail(BIVMOE_ERR_ARGUMENT, "out may be v, with its strides, but not q or k");
     if (!a->decay || !aligned(a->decay, 4) || !aligned(a->beta, 4)) return fail(BIVMOE_ERR_ARGUMENT, "decay or beta: null or not aligned");
     if (!a->states || !aligned(a->states, 16) || a->stride_slot % 4 || a->stride_head % 4)
         return fail(BIVMOE_ERR_ARGUMENT, "states: null, not aligned to 16 bytes, or a stride is not a multiple of 4 values");

@@ -528,7 +528,8 @@ BIVMOE_API void bivmoe_linear_destroy(bivmoe_linear* layer);
  * round the weights of a chunk's tokens among one another to bf16 once, and take the state, which they keep in f32, to its
  * product with q in bf16 (with beta in two terms of it).
  * Pointers are 16-byte aligned and strides multiples of 16 bytes for rows and states; the head's values of a row, and a state's
- * dim_k values, are neighbours; states' rows follow one another. */
+ * dim_k values, are neighbours; states' rows follow one another.  `out` may be v itself (same data and strides); what is written, rows
+ * and states, must not lie over anything else that the call reads or writes. */
 typedef struct bivmoe_linear_args {
     bivmoe_rows q, k, v, out;
     const float *decay, *beta;                   /* device, [n_tokens][n_head]; beta may be null */

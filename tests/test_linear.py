@@ -577,3 +577,26 @@ def test_what_is_not_finite_in_clusters_and_at_the_ends_of_chunks(where, delta):
     assert torch.equal(got[:where], clean[:where]) and torch.equal(got[:, 7, rest], clean[:, 7, rest]) and torch.equal(s1[slot, 7, rest], s0[slot, 7, rest])
     others = [i for i in range(40) if i != 7]
     assert torch.equal(got[:, others], clean[:, others]) and torch.equal(s1[slot, others], s0[slot, others])
+
+
+@gpu
+@pytest.mark.parametrize("dtype,lengths,dim", [(torch.bfloat16, [1, 1, 1], 128), (torch.float32, [5, 40], 64), (torch.bfloat16, [300, 30], 128),
+                                               (torch.bfloat16, [2100], 128)])
+@pytest.mark.parametrize("delta", [False, True])
+def test_out_may_be_v_and_nothing_else(lengths, dim, dtype, delta):
+    """Each kernel reads a row of v, of a head, in the block that writes that place of out, and before it does."""
+    x = make(lengths, 4, 4, dim, dim, dtype, delta, seed=len(lengths))
+    lay = layer(x, dtype)
+    call = lambda s, **more: lay.attend(**{**{k: x[k] for k in ("q", "k", "v", "decay", "slots", "first", "beta")}, "states": s,  # noqa: E731
+                                           "max_new": max(lengths), **more})
+    s0, s1 = x["states"].clone(), x["states"].clone()
+    want = call(s0)
+    wide = torch.zeros((sum(lengths), 9, dim), dtype=dtype, device="cuda")
+    v = wide[:, 2:6]
+    v.copy_(x["v"])
+    for bad in (dict(out=x["q"]), dict(out=x["k"]), dict(v=v, out=wide[:, 2::2])):
+        with pytest.raises(capi.BivMoeError):
+            call(s1, **bad)
+    got = call(s1, v=v, out=v)
+    assert got is v and torch.equal(v, want) and torch.equal(s1, s0)
+    assert not wide[:, :2].any() and not wide[:, 6:].any()
