@@ -318,8 +318,8 @@ __global__ void __launch_bounds__(kThreads, 1) linear_delta_kernel(const __grid_
             pf_fence_before();
             __syncwarp();
             arrive_warp(&H.w_full);
-            // (w_full has long been told: it puts the places that the other half's warp has taken out before they are read)
-            if (!wait_here(&H.u_full, k & 1, &H) || !wait_here(&H.w_full, k & 1, &H)) { ok = false; break; }
+            // (what the warp of the other half of the tokens has taken out of this one's rows comes with w_full)
+            if (!wait_told_here(&H.u_full, k & 1, &H.w_full, k & 1, &H)) { ok = false; break; }
             pf_fence_after();
             const float by = dec.bad[row] >= C ? dec.whole : __int_as_float(0x7fffffff);     // (NaN: so becomes the row)
             const f32x2 by2 = pk(by, by);

@@ -63,6 +63,24 @@ template <class H, bool CLUSTER, bool HERE> struct Wait {
     __device__ __forceinline__ void pause() const {}
     __device__ __forceinline__ bool all(bool v) const { return __all_sync(0xffffffffu, v); }
 };
+// A product's end, and behind it the word of the warp whose writes are read then (not by way of the issuing thread, which tells the
+// product's end).  It has long been given, and both are asked for in one turn, so that it costs no trip of its own.
+template <class H, bool HERE> struct WaitTold : Wait<H, false, HERE> {
+    uint64_t* word;
+    uint32_t word_parity;
+    __device__ __forceinline__ WaitTold(uint64_t* bar, uint32_t parity, uint64_t* word, uint32_t word_parity, const H* h)
+        : Wait<H, false, HERE>{bar, parity, h}, word(word), word_parity(word_parity) {}
+    __device__ __forceinline__ bool ready() const {
+        const bool ended = pf_bar_try(this->bar, this->parity), told = pf_bar_try(word, word_parity);      // (in this order)
+        return ended && told;
+    }
+};
+template <class H> __device__ __forceinline__ bool wait_told(uint64_t* bar, uint32_t parity, uint64_t* word, uint32_t word_parity, const H* h) {
+    return bounded_wait_together<64>(WaitTold<H, false>{bar, parity, word, word_parity, h});
+}
+template <class H> __device__ __forceinline__ bool wait_told_here(uint64_t* bar, uint32_t parity, uint64_t* word, uint32_t word_parity, const H* h) {
+    return bounded_wait_together<64>(WaitTold<H, true>{bar, parity, word, word_parity, h});
+}
 template <class H> __device__ __forceinline__ bool wait_one(uint64_t* bar, uint32_t parity, const H* h) {
     return bounded_wait<64>(Wait<H, false, false>{bar, parity, h});
 }
