@@ -212,9 +212,10 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunks_kernel(const __grid
             __syncwarp();
             arrive_warp(&H.u_free);
         }
-        // (the last products have read the state and P, and the last outputs have left, when the state's place is taken for its way out)
+        // (the last products have read the state and P, and the last outputs have left, when the state's place is taken for its way out; the
+        // outputs' word first, since these warps have not followed n_full and its parity alone says nothing)
         if (ok && rank + 1 == blocks && seq.to && !taken) {
-            if (wait_here(&H.n_full, (own - 1) & 1, &H) && wait_here(&H.out_done, 0, &H)) store_state(s, seq.to + at, room, 0);
+            if (wait_here(&H.out_done, 0, &H) && wait_here(&H.n_full, (own - 1) & 1, &H)) store_state(s, seq.to + at, room, 0);
             else ok = false;
         }
         asm volatile("cp.async.wait_all;" ::: "memory");      // (where a wait gave up before it was looked at)

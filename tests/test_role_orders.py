@@ -88,3 +88,9 @@ def test_the_chain_waits_for_the_warp_that_has_the_other_half_of_its_rows():
     chain = between(code("linear_delta.cu"), "for (int k = 0; k < chunks && ok; k++)", "store_state(")
     wait = re.search(TOLD % ("u_full", "k", "w_full", "k & 1"), chain)
     assert wait and chain.index("arrive_warp(&H.w_full)") < wait.start() < chain.index("dec.bad[row]")
+
+
+def test_the_state_leaves_behind_the_outputs_word():
+    """The state's warps have not followed the last product's barrier: behind the outputs' last word the phase that ended last is the last one."""
+    way_out = between(code("linear_chunks.cu"), "if (ok && rank + 1 == blocks && seq.to", "store_state(")
+    assert 0 < way_out.index("wait_here(&H.out_done, 0") < way_out.index("wait_here(&H.n_full, (own - 1) & 1")
