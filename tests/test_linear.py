@@ -600,3 +600,24 @@ def test_out_may_be_v_and_nothing_else(lengths, dim, dtype, delta):
     got = call(s1, v=v, out=v)
     assert got is v and torch.equal(v, want) and torch.equal(s1, s0)
     assert not wide[:, :2].any() and not wide[:, 6:].any()
+
+
+@gpu
+@pytest.mark.parametrize("delta", [False, True])
+def test_prompts_and_single_tokens_of_one_batch_in_two_calls(delta):
+    """The rows of a batch, its prompts first: each call takes a part of the lists, the offsets of the second begin behind the first's rows, and
+    each leaves the other's rows and states alone."""
+    lengths = [200, 33, 90] + [1] * 20
+    x = make(lengths, 4, 2, 128, 128, torch.bfloat16, delta, seed=9)
+    lay = layer(x, torch.bfloat16)
+    states, out = x["states"].clone(), torch.full_like(x["v"], 5.0)
+    call = lambda part, told: lay.attend(x["q"], x["k"], x["v"], x["decay"], states, x["slots"][part], x["first"][part.start:part.stop + 1],  # noqa: E731
+                                         beta=x["beta"], max_new=told, out=out)
+    call(slice(3, 23), 1)
+    prompts = x["slots"][:3].long()
+    assert (out[:323] == 5).all() and torch.equal(states[prompts], x["states"][prompts])
+    singles, rows = states.clone(), out[323:].clone()
+    call(slice(0, 3), 200)
+    others = [s for s in range(states.shape[0]) if s not in prompts.tolist()]
+    assert torch.equal(out[323:], rows) and torch.equal(states[others], singles[others])
+    check(x, out, states, torch.bfloat16, prompt=True)
