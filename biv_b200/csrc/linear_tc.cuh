@@ -168,7 +168,9 @@ template <int N> __device__ __forceinline__ void store_state(const float (&s)[N]
 }
 
 // P = Q K^T and its decays of a token (a row of tensor memory, in its own thread), rounded to bf16, in a row of 128 bytes of shared
-// memory (128-byte swizzle).  After its last load from tensor memory the warp arrives at `free`.
+// memory (128-byte swizzle).  After its last load from tensor memory the warp arrives at `free`.  The exponent is a difference of sums in
+// f32, of up to 64 x 128 log2(e) (tokens whose decays are all at the end of their range): off by 2^-10 then, and the weight by 7e-4 of
+// itself, where bf16 rounds it by up to 2^-9; sums of some hundreds, as decays have them in earnest, by 2^-16.
 __device__ __forceinline__ void weights_row(uint32_t from, const float* log2, int r, uint32_t row, uint64_t* free) {
     const float g = log2[r];
 #pragma unroll 1

@@ -66,7 +66,8 @@ class LinearAttention:
         with ``past[b]`` 0 starts from zeros whatever its slot holds.  ``keep[b]``: the state is kept as it is after that many
         of the call's tokens, with 0 left as it was: drafted tokens are computed with 0, and ``advance`` takes the accepted ones.
         Slots below zero, past the states, or that an earlier request has already: from zeros, and not kept.  ``max_new``: the
-        most new tokens of a request; it decides the kernel, and so the speed.  ``out`` may be v itself."""
+        most new tokens of a request; it decides the kernel for all of them, and so the speed: single tokens are best not given in one call
+        with prompts.  ``out`` may be v itself."""
         r = _step_calls.attend(self._geometry, q, k, v, decay, states, slots, first, beta, past, keep, max_new, scale, out)
         if r.__class__ is int:
             capi.check(r)

@@ -523,8 +523,8 @@ BIVMOE_API void bivmoe_linear_destroy(bivmoe_linear* layer);
  * Decays are logarithms, at most zero: one above counts as zero, and below -128 as -128, whose exponential is zero in f32.
  * What is not finite (a value of v: in its place of the rows and of the state from its token on) does not reach tokens before it,
  * nor other requests or heads.
- * max_new: no request has more new tokens (0: not known, and reckoned as n_tokens); it decides the kernel, and with that the
- * speed alone.  All sums and the state are f32.  The kernels for prompts (BF16, dims of 128, out wanted, no keep, more than 16 tokens)
+ * max_new: no request has more new tokens (0: not known, and reckoned as n_tokens); it decides the kernel for all requests of the call, and with
+ * that the speed, and whether there are the roundings named next.  All sums and the state are f32.  The kernels for prompts (BF16, dims of 128, out wanted, no keep, more than 16 tokens)
  * round the weights of a chunk's tokens among one another to bf16 once, and take the state, which they keep in f32, to its
  * product with q in bf16 (with beta in two terms of it).
  * Pointers are 16-byte aligned and strides multiples of 16 bytes for rows and states; the head's values of a row, and a state's
@@ -549,7 +549,7 @@ BIVMOE_API int bivmoe_linear_status(bivmoe_linear* layer, void* stream);
 /* Root-mean-square norm of rows (ops::rms_norm, engine/src/ops.rs:136-149; with the silu gate metal/kernels.metal:890-957):
  *     x += add                                   where there is add: rounded to x's type and kept in x
  *     y = x * rsqrt(mean(x^2) + eps) * weight    weight null: 1
- *     y *= gate / (1 + exp(-gate))               where there is gate
+ *     y *= gate / (1 + exp(-gate))               where there is gate (below -87 times zero)
  * The squares are summed in f64 and the root rounded once to f32; the products are f32, in this order; y is rounded once to the
  * output's type.  As 8-bit rows a block of values shares a scale (f32), and stands for scale * code:
  *     BIVMOE_NORM_Q8    int8, block 32, scale = max|y| * (1 / 127), code = y * (1 / scale) rounded, halves away from zero: as
@@ -558,7 +558,8 @@ BIVMOE_API int bivmoe_linear_status(bivmoe_linear* layer, void* stream);
  *     BIVMOE_NORM_E4M3  8-bit floats, block 128 or 0 (the row), scale = max|y| * (1 / 448), code = y / scale rounded to the
  *                       nearest
  * each step in f32.  A block whose scale is 0 (zeros, or values whose scale f32 does not hold) has codes 0.  Where f32 does not hold 1 / scale (below
- * 2^-128) NORM_Q8 divides by the scale instead; such a scale has few bits, and quotients that pass 127, or E4M3's 448, are kept at it. */
+ * 2^-128) NORM_Q8 divides by the scale instead; such a scale has few bits, and quotients that pass 127, or E4M3's 448, are kept at it.  Where a block holds NaN or an
+ * infinity, its scale is not finite either and its codes stand for nothing; other blocks, and of E4M3 by rows other rows, are as they are. */
 enum { BIVMOE_NORM_Q8 = 1000, BIVMOE_NORM_E4M3 = 1001 };
 typedef struct bivmoe_norm_args {
     bivmoe_rows x, add, gate, out;   /* add.data and gate.data may be null; out's type: F32, F16, BF16 or one of the above */
