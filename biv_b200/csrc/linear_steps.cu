@@ -258,7 +258,12 @@ template <int DK, int R, int TB> cudaError_t launch(const LinearCall& c, cudaStr
     count_launch();
     const dim3 grid(c.n_head * (c.dim_v / Steps<DK, R, TB>::rows), c.n_seq);
     const size_t smem = sizeof(typename Steps<DK, R, TB>::Shared);
-    return launch_with(pdl_mode() != 0, stream, c.beta ? linear_steps_kernel<DK, R, TB, true> : linear_steps_kernel<DK, R, TB, false>, grid,
+    // Scheduled early, except where long requests' blocks would all run at once: those would be put where the kernel before leaves room, several
+    // to one multiprocessor, and stay there.  (One request of 2048 tokens, 32 heads of f32, calls one after another: early 697 to 839 us, else 554; with
+    // the delta rule 888 to 1099 and 672; 12 tokens 9.5 and 8.4.  Of more blocks, 8 requests of 9 tokens 19.8 and 20.8, 64 of 16 184 and 186, 16 of
+    // 512 and heads of 64 362 and 365; drafts of few blocks, one request of 5, 4.7 and 6.9, single tokens of two 4.8 and 6.1.)
+    const bool early = TB < 16 || (int64_t)grid.x * grid.y >= 4 * c.sms;
+    return launch_with(pdl_mode() == 1 || (pdl_mode() != 0 && early), stream, c.beta ? linear_steps_kernel<DK, R, TB, true> : linear_steps_kernel<DK, R, TB, false>, grid,
                        dim3(kThreads), smem, c);
 }
 // Rows to a thread, and tokens brought in together.  us with one, two, four rows: 64 single tokens, 32 heads of 128: 59, 46, 47; 128 of 16

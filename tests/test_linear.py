@@ -621,3 +621,28 @@ def test_prompts_and_single_tokens_of_one_batch_in_two_calls(delta):
     others = [s for s in range(states.shape[0]) if s not in prompts.tolist()]
     assert torch.equal(out[323:], rows) and torch.equal(states[others], singles[others])
     check(x, out, states, torch.bfloat16, prompt=True)
+
+
+@gpu
+@pytest.mark.parametrize("delta", [False, True])
+def test_a_long_request_takes_no_longer_behind_another(delta):
+    """Blocks that are scheduled before the call ahead has ended go where that leaves room: those of a long request, which all run at once, were
+    put several to one multiprocessor, for one and a half times the time."""
+    x = make([1024], 32, 16, 128, 128, torch.float32, delta, seed=1)
+    lay = layer(x, torch.float32)
+    states, out = x["states"].clone(), torch.empty_like(x["v"])
+    call = lambda: lay.attend(x["q"], x["k"], x["v"], x["decay"], states, x["slots"], x["first"], beta=x["beta"], max_new=1024, out=out)  # noqa: E731
+
+    def time(n):
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        torch.cuda.synchronize()
+        a.record()
+        for _ in range(n):
+            call()
+        b.record()
+        torch.cuda.synchronize()
+        return a.elapsed_time(b) / n
+
+    time(3)
+    alone, behind = (sorted(time(n) for _ in range(7))[3] for n in (1, 30))
+    assert behind < 1.08 * alone, (alone, behind)
