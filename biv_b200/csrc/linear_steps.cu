@@ -10,8 +10,8 @@
 // and the update is not on the way to the output.  Arithmetic is f32, two values to an instruction.
 //
 // Single tokens are bound by the states' way from memory and back (64 requests x 32 heads of 128 x 128: 268 MB in 46 us, 0.89 of the
-// measured rate), drafts by the products as well, long requests by the way of a token through its products and shuffles: 570
-// clocks, 2048 tokens of 32 heads in 615 us.
+// measured rate), drafts by the products as well, long requests by the way of a token through its products and shuffles: 530
+// clocks, 2048 tokens of 32 heads in 555 us.
 #include "common.cuh"
 #include "launch.cuh"
 #include "linear.cuh"
@@ -268,11 +268,11 @@ template <int DK, int R, int TB> cudaError_t launch(const LinearCall& c, cudaStr
 }
 // Rows to a thread, and tokens brought in together.  us with one, two, four rows: 64 single tokens, 32 heads of 128: 59, 46, 47; 128 of 16
 // heads of 64: 32, 18, 15; 32 of 16 heads of 256: 64, 49, -; 32 requests of 5 tokens, delta rule, 65, 42, 38.  Long requests, eight
-// tokens together and sixteen: one of 2048, f32: 720 and 719, 613 and 557, 821; 16 of 512, 32 heads of 64: 499 and 500, 375 and 340, 292 and
-// 341; one of 2048, 16 heads of 256, delta rule: 962 and 963, 1167 and
-// 1078.  The loop with two tokens in hand (four for prompts and heads of 64; one for single tokens) took 37.0 us for the 32 drafts, with
+// tokens together and sixteen: one of 2048, 32 heads, f32: 737 and 619, 690 and 555, 999 and 741; 16 of 512, 32 heads of 64: 584 and 527, 401 and
+// 363, 342 and 327 (one of 2048, 16 heads, sixteen tokens: 442, 481, 587); one of 2048, 16 heads of 256, delta rule: 1172 and 1028, 1139 and 988 (4
+// heads: 777, 985; eight of 500 by 16 heads: 1750, 1222).  The loop with two tokens in hand (four for prompts and heads of 64; one for single tokens) took 37.0 us for the 32 drafts, with
 // one 41.9, with four 37.7; the single tokens with four 48.3 and not 46.
-// (Prompts before what f32 leaves of a decay went along, which takes a tenth: 557 to 615 us; nine requests of up to 1224 tokens, f32, delta
+// (Prompts before what f32 leaves of a decay went along, which takes a tenth: 507 to 555 us; nine requests of up to 1224 tokens, f32, delta
 // rule, were off by 1.1e-6 without it and are by 2.5e-7.)
 template <int DK> cudaError_t launch_rows(const LinearCall& c, int max_new, int sm_count, cudaStream_t stream) {
     constexpr int single = DK == 64 ? 4 : 2, drafts = DK == 256 ? 2 : 4, prompts = DK == 256 ? 1 : 2;

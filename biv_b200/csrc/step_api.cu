@@ -53,8 +53,8 @@ static int device_of(int device, const char* what, int* sms) {
 // ---- linear attention ----
 
 // New tokens of a request up to which they are taken one by one.  (us of 32 heads of 128, one by one and by the kernels for prompts: one
-// request of 16 tokens 8.4 and 11.7, of 24 11.7 and 11.6; 16 of 16 37.9 and 39.2, of 24 54 and 39; 64 of 16 139 and 139.  With the delta rule:
-// 10.0 and 16.6, 14.1 and 16.7; 46.7 and 59.7, 66 and 60; 169 and 204, of 24 247 and 203.)
+// request of 24 tokens 10.4 and 11.9; 16 of 16 39 and 39, of 24 58 and 39; 64 of 16 150 and 140, of 24 225 and 141.  With the delta rule: 12.4 and
+// 16.5; 48 and 59, 72 and 59; 183 and 203, 273 and 203.)
 constexpr int kSteps = 16;
 
 extern "C" void bivmoe_linear_destroy(bivmoe_linear* l) {
