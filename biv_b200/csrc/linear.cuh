@@ -6,6 +6,7 @@
 #include <stdint.h>
 
 #include "../../include/bivmoe.h"
+#include "rows_of.h"
 
 namespace bivmoe {
 
@@ -43,8 +44,9 @@ __device__ __forceinline__ bool slot_taken(const LinearCall& c, int b, int threa
 }
 __device__ __forceinline__ LinearSeq linear_seq(const LinearCall& c, int b) {
     LinearSeq s;
-    s.first = min(max(c.first[b], 0), c.n_tokens);
-    s.n = max(min(c.first[b + 1], c.n_tokens) - s.first, 0);
+    const RowsOf rows = rows_of(c.first[b], c.first[b + 1], c.n_tokens);
+    s.first = rows.first;
+    s.n = rows.n;
     s.kept = c.keep ? min(max(c.keep[b], 0), s.n) : s.n;
     const int slot = c.slots[b];
     float* at = slot >= 0 && slot < c.n_slots ? c.states + slot * c.slot : nullptr;

@@ -25,7 +25,7 @@ __device__ __forceinline__ int request_at(const LinearCall& c, int at) {
     const int lane = threadIdx.x & 31;
     int n[2], rank[2] = {0, 0};
 #pragma unroll
-    for (int i = 0; i < 2; i++) n[i] = lane + 32 * i < c.n_seq ? c.first[lane + 32 * i + 1] - c.first[lane + 32 * i] : INT_MIN;
+    for (int i = 0; i < 2; i++) n[i] = lane + 32 * i < c.n_seq ? rows_of(c.first[lane + 32 * i], c.first[lane + 32 * i + 1], c.n_tokens).n : INT_MIN;
     const int any = __shfl_sync(0xffffffffu, n[0], 0);
     if (__all_sync(0xffffffffu, (n[0] == any || n[0] == INT_MIN) && (n[1] == any || n[1] == INT_MIN))) return at;
     for (int j = 0; j < c.n_seq; j++) {

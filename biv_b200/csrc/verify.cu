@@ -17,6 +17,7 @@
 
 #include "common.cuh"
 #include "launch.cuh"
+#include "rows_of.h"
 #include "verify.cuh"
 
 namespace bivmoe {
@@ -116,7 +117,8 @@ template <class T> __global__ void __launch_bounds__(kThreads, 4) verify_kernel(
     const int blocks = cluster.num_blocks(), rank = cluster.block_rank(), b = blockIdx.x / blocks;
     // that all blocks of the cluster have begun is waited for before the first writes into another
     if (blocks > 1) asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
-    const int first = min(max(a.first[b], 0), a.n_tokens), n = max(min(a.first[b + 1], a.n_tokens) - first, 0);
+    const RowsOf rows = rows_of(a.first[b], a.first[b + 1], a.n_tokens);
+    const int first = rows.first, n = rows.n;
     const T *p = (const T*)a.p, *q = (const T*)a.q;
     // every warp for itself: the first draft that fails
     int kept = max(n - 1, 0);

@@ -513,8 +513,8 @@ typedef struct bivmoe_linear_desc {
 BIVMOE_API int bivmoe_linear_create(const bivmoe_linear_desc* desc, bivmoe_linear** out);
 BIVMOE_API void bivmoe_linear_destroy(bivmoe_linear* layer);
 
-/* Rows first[b] to first[b + 1] - 1 are the new tokens of request b (offsets that decrease or pass n_tokens count as none and as
- * n_tokens); rows past first[n_seq] are not written.  The request's state is slot slots[b]: it is read unless past[b] is 0 (past
+/* Rows first[b] to first[b + 1] - 1 are the new tokens of request b (offsets below zero or past n_tokens count as zero and as
+ * n_tokens, those that decrease as no tokens); rows past first[n_seq] are not written.  The request's state is slot slots[b]: it is read unless past[b] is 0 (past
  * null: always read; a request that starts needs no cleared slot), and written once, as it is after the first keep[b] of the
  * call's tokens (keep null: after all; 0 of them, or a request without new tokens: the slot is left as it was).  So drafted
  * tokens that may be taken back are computed with keep 0, and the call is made again with those that were accepted, without q.
@@ -573,7 +573,7 @@ typedef struct bivmoe_norm_args {
 /* `out` may be x itself (same data, type and strides); other buffers that are written must not lie over others. */
 BIVMOE_API int bivmoe_norm(const bivmoe_norm_args* args, void* stream);
 
-/* Drafted tokens against the target's probabilities.  Rows first[b] to first[b + 1] - 1 belong to request b: tokens[first[b]] is
+/* Drafted tokens against the target's probabilities.  Rows first[b] to first[b + 1] - 1 belong to request b (offsets as above): tokens[first[b]] is
  * its current token, the ones after it its drafts.  p[r] is the target's distribution of the token after row r's, and q[r] the
  * one that the draft after row r was drawn from (q null: the drafts are certain, as looked up or greedy ones are).
  * From the first draft on, d = tokens[r + 1] is accepted while uniform[r] * q[r][d] < p[r][d] (exact, in f64; q null: while uniform[r] <

@@ -646,3 +646,56 @@ def test_a_long_request_takes_no_longer_behind_another(delta):
     time(3)
     alone, behind = (sorted(time(n) for _ in range(7))[3] for n in (1, 30))
     assert behind < 1.08 * alone, (alone, behind)
+
+
+@gpu
+@pytest.mark.parametrize("delta", [False, True])
+@pytest.mark.parametrize("lengths,h,hk", [([65, 130], 4, 2), ([30, 1, 200], 3, 1), ([1100], 40, 20), ([2100, 40], 3, 1)])
+def test_prompts_in_wide_rows_and_rows_behind_the_last(lengths, h, hk, delta):
+    """q, k and v as parts of wider rows, every second one; decays and states with gaps; behind the last sequence, and before the first, rows of
+    NaN, which a chunk's copies may bring in but nothing may reach, and outputs that stay."""
+    d, n, before = 128, sum(lengths), 5
+    x = make(lengths, h, hk, d, d, torch.bfloat16, delta, seed=n)
+    t = before + n + 70
+    rows = torch.full((t, 2, 2 * hk + h + 1, d), math.nan, dtype=torch.bfloat16, device="cuda")[:, 1]
+    views = dict(q=rows[:, :hk], k=rows[:, hk:2 * hk], v=rows[:, 2 * hk:2 * hk + h])
+    for name, view in views.items():
+        view[before:before + n] = x[name]
+    scalars = torch.full((t, 3 * h), math.nan, device="cuda")
+    scalars[before:before + n, :h] = x["decay"]
+    if delta:
+        scalars[before:before + n, h:2 * h] = x["beta"]
+    big = torch.full((x["states"].shape[0], 2, h + 1, d, d), 7.0, device="cuda")
+    big[:, 1, :h] = x["states"]
+    states = big[:, 1, :h]
+    wide_out = torch.full((t, h + 2, d), 3.0, dtype=torch.bfloat16, device="cuda")
+    out = wide_out[:, 1:h + 1]
+    lay = layer(x, torch.bfloat16)
+    first = x["first"] + before
+    lay.attend(views["q"], views["k"], views["v"], scalars[:, :h], states, x["slots"], first, beta=scalars[:, h:2 * h] if delta else None,
+               scale=-0.3, max_new=max(lengths), out=out)
+    lay.status()
+    check(x, out[before:before + n], states, torch.bfloat16, scale=-0.3, prompt=True)
+    assert (wide_out[:, 0] == 3).all() and (wide_out[:, h + 1] == 3).all() and (out[:before] == 3).all() and (out[before + n:] == 3).all()
+    assert (big[:, 0] == 7).all() and (big[:, 1, h] == 7).all()
+
+
+@gpu
+@pytest.mark.parametrize("delta", [False, True])
+@pytest.mark.parametrize("max_new", [0, 16, 200])
+def test_offsets_that_pass_the_rows_or_decrease(max_new, delta):
+    """Past n_tokens they count as n_tokens, decreasing ones as no tokens, negative ones as zero."""
+    x = make([90, 0, 40], 4, 2, 128, 128, torch.bfloat16, delta, seed=4)
+    lay = layer(x, torch.bfloat16)
+    run = lambda first, s: lay.attend(x["q"], x["k"], x["v"], x["decay"], s, x["slots"],  # noqa: E731
+                                      torch.tensor(first, dtype=torch.int32, device="cuda"), beta=x["beta"], max_new=max_new)
+    s0, s1, s2 = (x["states"].clone() for _ in range(3))
+    want = run([0, 90, 90, 130], s0)
+    check(x, want, s0, torch.bfloat16, prompt=max_new != 16)
+    assert torch.equal(run([-7, 90, 90, 2 ** 31 - 1], s1), want) and torch.equal(s1, s0)
+    got = run([90, 20, 130, -(2 ** 31)], s2)                 # only the second request has rows: 20 to 129
+    y = {**x, "first": torch.tensor([20, 20, 130, 130], dtype=torch.int32, device="cuda")}
+    out, states, _ = reference(y)
+    assert torch.equal(s2[x["slots"][[0, 2]].long()], x["states"][x["slots"][[0, 2]].long()])
+    err = (s2.double().cpu() - states).norm() / states.norm()
+    assert err < 1e-5 and (got[20:].double().cpu() - out[20:]).norm() / out[20:].norm() < 1e-2

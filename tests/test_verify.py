@@ -329,3 +329,21 @@ def test_the_definition_of_these_tests():
     assert decided(p, q, [0, 1], [0.5, 0.0], 0.9, 3) == (0, 2)                # 2 < 2 is not: what p has over q
     assert decided([[1.0, 2.0], [0.0, 0.0]], [[1.0, nan], [0.0, 0.0]], [0, 1], [0.0, 0.0], 0.5, 2) == (0, 1)   # 0 * NaN: not accepted; p itself
     assert decided([[inf, 1.0, inf, 1.0]], None, [0], [0.0], 0.0, 4) == (0, 3)
+
+
+@gpu
+def test_offsets_that_pass_the_rows_or_decrease():
+    """Past n_tokens they count as n_tokens, decreasing ones as no rows, negative ones as zero."""
+    x = make([4, 0, 5, 3], 1003, torch.float32, True, seed=6)
+    want = run(x)
+    x["first"] = torch.tensor([-9, 4, 4, 9, 2 ** 31 - 1], dtype=torch.int32, device="cuda")
+    got = run(x)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    x["first"] = torch.tensor([9, 4, 12, -(2 ** 31), 3], dtype=torch.int32, device="cuda")       # rows 4 to 11, and 0 to 2
+    got, length = run(x), x["length"]
+    x["first"], x["length"], x["sample"] = torch.tensor([4, 12], dtype=torch.int32, device="cuda"), length[1:2], x["sample"][[1, 3]]
+    accepted, token, kept = reference({**x, "sample": x["sample"][:1]})
+    more = reference({**x, "first": torch.tensor([0, 3], dtype=torch.int32), "length": length[3:], "sample": x["sample"][1:]})
+    assert got.accepted.tolist() == [0, accepted[0], 0, more[0][0]]
+    assert got.token.tolist() == [-1, token[0], -1, more[1][0]]
+    assert got.kept.tolist() == [int(length[0]), kept[0], int(length[2]), more[2][0]]
