@@ -699,3 +699,30 @@ def test_offsets_that_pass_the_rows_or_decrease(max_new, delta):
     assert torch.equal(s2[x["slots"][[0, 2]].long()], x["states"][x["slots"][[0, 2]].long()])
     err = (s2.double().cpu() - states).norm() / states.norm()
     assert err < 1e-5 and (got[20:].double().cpu() - out[20:]).norm() / out[20:].norm() < 1e-2
+
+
+@gpu
+@pytest.mark.parametrize("delta", [False, True])
+@pytest.mark.parametrize("lengths,told", [([1, 3, 2], 3), ([100, 1, 70], 100)])
+def test_rows_and_states_more_than_32_bits_apart(lengths, told, delta):
+    """Rows 2^24 + 2^20 values from one another, 171 of them; slots of 2^18 values, the last of 9000 among them."""
+    n, h, d, apart = sum(lengths), 4, 128, 2 ** 24 + 2 ** 20
+    x = make(lengths, h, h, d, d, torch.bfloat16, delta, seed=2)
+    room = torch.empty(n * apart, dtype=torch.bfloat16, device="cuda")
+    views = {name: room[i * h * d:].as_strided((n, h, d), (apart, d, 1)) for i, name in enumerate(("q", "k", "v", "out"))}
+    for name in ("q", "k", "v"):
+        views[name].copy_(x[name])
+    slots = [8999, 3, 8192]
+    far = torch.empty((9000, 4, h, d, d), device="cuda")[:, 1]     # 2^18 values a slot: past 2^31 from the 8192nd on
+    kept = torch.zeros((9, h, d, d), device="cuda")
+    for i, (a, b) in enumerate(zip(slots, x["slots"].tolist())):
+        far[a] = x["states"][b]
+        kept[i] = x["states"][b]
+    ints = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    lay = layer(x, torch.bfloat16)
+    out = lay.attend(views["q"], views["k"], views["v"], x["decay"], far, ints(slots), x["first"], beta=x["beta"], max_new=told, out=views["out"])
+    lay.status()
+    y = {**x, "states": kept, "slots": ints([0, 1, 2])}
+    got = kept.clone()
+    got[:3] = far[slots]
+    check(y, out, got, torch.bfloat16, prompt=told > 16)

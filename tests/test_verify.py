@@ -347,3 +347,15 @@ def test_offsets_that_pass_the_rows_or_decrease():
     assert got.accepted.tolist() == [0, accepted[0], 0, more[0][0]]
     assert got.token.tolist() == [-1, token[0], -1, more[1][0]]
     assert got.kept.tolist() == [int(length[0]), kept[0], int(length[2]), more[2][0]]
+
+
+@gpu
+def test_rows_more_than_32_bits_apart():
+    x = make([5] * 28, 1003, torch.bfloat16, True, seed=8)
+    apart = 2 ** 24 + 2 ** 10 + 1                            # (a row of p now and then begins on 16 bytes)
+    room = torch.empty(140 * apart, dtype=torch.bfloat16, device="cuda")
+    for i, name in enumerate(("p", "q")):
+        view = room[4096 * i:].as_strided((140, 1003), (apart, 1))
+        view.copy_(x[name])
+        x[name] = view
+    check(x)
